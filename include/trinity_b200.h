@@ -312,6 +312,97 @@ typedef struct {
 int64_t tb200_kv_compact_max_keep(const tb200_kv_compact_args* args);
 int tb200_kv_compact(const tb200_kv_compact_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The KV cache in 4 bits.  New relative to the reference, whose caches are 16-bit (H, P+M, D)
+ * tensors (convert_eval_rms.py:82-83); this is the same cache at 4.5 bits per value, rows =
+ * (batch, kv head, position).
+ *
+ * A group is 64 consecutive values x of a row.  lo = min x, s = (max x - min x) / 15, computed in
+ * fp32 and rounded to the cache's 16-bit type; c = the whole number nearest to (x - lo) / s in [0, 15]
+ * (halves to even; 0 where s is 0).  The group stands for lo + c * s.  A group that holds an infinity
+ * or a NaN, or whose max - min is not finite in fp32, stands for NaN throughout.
+ *   codes  (B, Hkv, cache_len, D/2) bytes: element 2i in the low, 2i+1 in the high four bits of byte i
+ *   meta   (B, Hkv, cache_len, D/64, 2) of the cache's type: s, lo
+ * cache_len is a multiple of 4; codes and meta are contiguous and 16-byte aligned.
+ *
+ * tb200_kv4_append quantises new rows into the cache, tb200_kv4_read turns cache rows back into
+ * 16-bit rows (lo + c * s rounded once, at most the type's largest number).  Row i < n_rows[b] of sequence b is cache position
+ * start[b] + i.  Rows i >= n_rows[b] and rows whose position lies outside [0, cache_len) are left as
+ * they are (append: the cache; read: k and v).  n_rows[b] outside [0, rows] is taken as the nearer end.
+ * k and v are addressed by element strides of their batch, head and row axes (multiples of 8; head_dim
+ * contiguous); the rows of a tensor that is written must not overlap one another. */
+typedef struct {
+  int dtype;                 /* TB200_F16 or TB200_BF16: k, v, meta */
+  int batch, n_kv_heads, rows, head_dim; /* head_dim 64 or 128 */
+  int cache_len;             /* positions per (sequence, head) in the cache, a multiple of 4 */
+  int start_all;             /* first position of every sequence when start is NULL */
+  int reserved;              /* 0 */
+  const int32_t* start;      /* (B) or NULL */
+  const int32_t* n_rows;     /* (B) or NULL: all `rows` */
+  void* k;                   /* append: read; read: written */
+  void* v;
+  int64_t k_stride[3];       /* batch, head, row */
+  int64_t v_stride[3];
+  void* k_codes;
+  void* v_codes;
+  void* k_meta;
+  void* v_meta;
+} tb200_kv4_rows_args;
+int tb200_kv4_append(const tb200_kv4_rows_args* args, void* stream);
+int tb200_kv4_read(const tb200_kv4_rows_args* args, void* stream);
+/* The host-side argument checks of the two alone: nothing is launched, no device is needed. */
+int tb200_kv4_rows_check(const tb200_kv4_rows_args* args);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention over a cache that already holds the new rows, per-sequence lengths.  New relative to the
+ * reference, whose attention modules (evaluation/vanilla/vanilla_falcon_benchmark28173.py:19-144)
+ * read every position of one uniformly filled 16-bit cache.
+ *
+ * Sequence b has kv_lens[b] = n positions in the cache, the last q_rows[b] = r of which are the new
+ * ones (their k and v already written).  Query row i < r stands at position n - r + i and sees the
+ * positions j up to its own; with window > 0 only those of them with j > n - r + i - window or
+ * j < sinks (window 0: no window, sinks is then 0).  o = softmax(sm_scale * q K^T) V over what it
+ * sees; a row that sees nothing (n < r, n = 0) gives zeros.  Rows i >= r of o are left as they are.
+ * kv_lens[b] outside [0, cache_len] and q_rows[b] outside [0, rows] are taken as the nearer end.
+ * Cache rows that no query row of their sequence sees have no influence, whatever they hold; an
+ * infinity or a NaN in a row that some query row sees may also reach the other new rows of that
+ * sequence in the same call.
+ *
+ * tb200_attn_window: 16-bit caches, tb200_kv4_attn: 4-bit caches as above.  q, o and the 16-bit caches
+ * are addressed by element strides (multiples of 8, head_dim contiguous).  Workspace: as the
+ * *_workspace_bytes queries say for the same arguments (pointers and lengths are not looked at). */
+typedef struct {
+  int dtype;                 /* TB200_F16 or TB200_BF16: q, o, 16-bit caches, meta */
+  int batch, rows;           /* rows: new rows per sequence at most (S) */
+  int n_q_heads, n_kv_heads, head_dim; /* head_dim 64 or 128 */
+  int cache_len;             /* positions per (sequence, head); 4-bit: a multiple of 4 */
+  int window, sinks;
+  float sm_scale;
+  const void* q;             /* (B, Hq, rows, D) */
+  void* o;                   /* (B, Hq, rows, D) */
+  int64_t q_stride[3];       /* batch, head, row */
+  int64_t o_stride[3];
+  const int32_t* kv_lens;    /* (B) */
+  const int32_t* q_rows;     /* (B) or NULL: all `rows` */
+  const void* k_cache;       /* tb200_attn_window: (B, Hkv, cache_len, D) */
+  const void* v_cache;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const void* k_codes;       /* tb200_kv4_attn */
+  const void* v_codes;
+  const void* k_meta;
+  const void* v_meta;
+  void* workspace;
+  size_t workspace_bytes;
+} tb200_cache_attn_args;
+size_t tb200_attn_window_workspace_bytes(const tb200_cache_attn_args* args);
+int tb200_attn_window(const tb200_cache_attn_args* args, void* stream);
+size_t tb200_kv4_attn_workspace_bytes(const tb200_cache_attn_args* args);
+int tb200_kv4_attn(const tb200_cache_attn_args* args, void* stream);
+/* The host-side argument checks alone (workspace excepted): nothing is launched, no device is needed. */
+int tb200_attn_window_check(const tb200_cache_attn_args* args);
+int tb200_kv4_attn_check(const tb200_cache_attn_args* args);
+
 #ifdef __cplusplus
 }
 #endif

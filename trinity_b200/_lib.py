@@ -71,6 +71,29 @@ class KvCompactArgs(C.Structure):
     ]
 
 
+class Kv4RowsArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("batch", C.c_int), ("n_kv_heads", C.c_int), ("rows", C.c_int), ("head_dim", C.c_int),
+        ("cache_len", C.c_int), ("start_all", C.c_int), ("reserved", C.c_int),
+        ("start", C.c_void_p), ("n_rows", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_meta", C.c_void_p), ("v_meta", C.c_void_p),
+    ]
+
+
+class CacheAttnArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("batch", C.c_int), ("rows", C.c_int),
+        ("n_q_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("cache_len", C.c_int),
+        ("window", C.c_int), ("sinks", C.c_int), ("sm_scale", C.c_float),
+        ("q", C.c_void_p), ("o", C.c_void_p), ("q_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3),
+        ("kv_lens", C.c_void_p), ("q_rows", C.c_void_p),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_meta", C.c_void_p), ("v_meta", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # every symbol include/trinity_b200.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "tb200_strerror": (C.c_char_p, [C.c_int]),
@@ -103,6 +126,15 @@ SYMBOLS = {
     "tb200_topk": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p]),
     "tb200_kv_compact_max_keep": (C.c_int64, [C.POINTER(KvCompactArgs)]),
     "tb200_kv_compact": (C.c_int, [C.POINTER(KvCompactArgs), C.c_void_p]),
+    "tb200_kv4_rows_check": (C.c_int, [C.POINTER(Kv4RowsArgs)]),
+    "tb200_kv4_append": (C.c_int, [C.POINTER(Kv4RowsArgs), C.c_void_p]),
+    "tb200_kv4_read": (C.c_int, [C.POINTER(Kv4RowsArgs), C.c_void_p]),
+    "tb200_attn_window_check": (C.c_int, [C.POINTER(CacheAttnArgs)]),
+    "tb200_attn_window_workspace_bytes": (C.c_size_t, [C.POINTER(CacheAttnArgs)]),
+    "tb200_attn_window": (C.c_int, [C.POINTER(CacheAttnArgs), C.c_void_p]),
+    "tb200_kv4_attn_check": (C.c_int, [C.POINTER(CacheAttnArgs)]),
+    "tb200_kv4_attn_workspace_bytes": (C.c_size_t, [C.POINTER(CacheAttnArgs)]),
+    "tb200_kv4_attn": (C.c_int, [C.POINTER(CacheAttnArgs), C.c_void_p]),
 }
 
 _lib = None

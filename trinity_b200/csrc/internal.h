@@ -236,4 +236,10 @@ int launch_cast_f32(const float* src, void* dst, int64_t n, int dtype, cudaStrea
 // ---------------------------------------------------------------- evict.cu
 int launch_kv_compact(const tb200_kv_compact_args& a, cudaStream_t stream);
 
+// ---------------------------------------------------------------- kv4.cu
+// Element strides of the (batch, head, row) axes with extents ext: steps of 16 bytes, and with `written` rows that do
+// not overlap.  Axes of one element are not looked at.
+int check_strides(const int64_t (&stride)[3], const int64_t (&ext)[3], int head_dim, bool written);
+int launch_kv4_rows(const tb200_kv4_rows_args& a, bool append, int num_sms, cudaStream_t stream);
+
 }  // namespace tb200

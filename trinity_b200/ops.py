@@ -7,7 +7,7 @@ been cached, so they can be captured in a CUDA graph after one warm-up call.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Dict, Optional
+from typing import Dict, NamedTuple, Optional, Union
 
 import torch
 
@@ -297,6 +297,170 @@ def kv_compact(k_src: torch.Tensor, v_src: torch.Tensor, idx: torch.Tensor, kv_l
     args.k_dst, args.v_dst, args.kept_pos, args.new_len = _ptr(k_dst), _ptr(v_dst), _ptr(kept_pos), _ptr(new_len)
     L.check(lib.tb200_kv_compact(C.byref(args), _stream()), "tb200_kv_compact")
     return k_dst, v_dst, kept_pos, new_len
+
+
+class Kv4Cache(NamedTuple):
+    """A KV cache in 4 bits: groups of 64 values of a row as codes ``c`` of 4 bits and a pair ``(s, lo)`` of the cache's
+    16-bit type, standing for ``lo + c * s`` (include/trinity_b200.h has the definition).
+
+    ``k_codes, v_codes``: uint8 ``(B, Hkv, L, D / 2)``, element ``2 i`` in the low and ``2 i + 1`` in the high four bits
+    of byte ``i``; ``k_meta, v_meta``: ``(B, Hkv, L, D / 64, 2)``.  ``L`` is a multiple of 4."""
+    k_codes: torch.Tensor
+    v_codes: torch.Tensor
+    k_meta: torch.Tensor
+    v_meta: torch.Tensor
+
+
+def kv4_cache(batch: int, kv_heads: int, cache_len: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device="cuda") -> Kv4Cache:
+    """An empty 4-bit cache of at least ``cache_len`` positions (rounded up to a multiple of 4)."""
+    if head_dim % 64:
+        raise ValueError(f"head_dim must be a multiple of 64, not {head_dim}")
+    length = (cache_len + 3) // 4 * 4
+    codes = [torch.zeros(batch, kv_heads, length, head_dim // 2, dtype=torch.uint8, device=device) for _ in range(2)]
+    meta = [torch.zeros(batch, kv_heads, length, head_dim // 64, 2, dtype=dtype, device=device) for _ in range(2)]
+    return Kv4Cache(*codes, *meta)
+
+
+def _rows4(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device):
+    """Pointer and element strides (batch, head, row) of a ``(B, heads, rows, D)`` tensor whose last axis is contiguous."""
+    if not t.is_cuda:
+        raise ValueError("trinity_b200 operators take CUDA tensors (there is no CPU path)")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the call's first tensor on {device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous")
+    return t.data_ptr(), (C.c_int64 * 3)(*t.stride()[:3])
+
+
+def _ints(t: Optional[torch.Tensor], name: str, batch: int, device: torch.device) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != (batch,):
+        raise TypeError(f"{name} must be int32 of shape ({batch},)")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the call's first tensor on {device}")
+    return _ptr(t)
+
+
+def _kv4_parts(cache: Kv4Cache, device: torch.device):
+    """(batch, kv heads, cache length, head_dim, type) of a 4-bit cache and its pointers."""
+    b, h, length, half = cache.k_codes.shape
+    d, dt = 2 * half, cache.k_meta.dtype
+    for name in ("k_codes", "v_codes", "k_meta", "v_meta"):
+        t = getattr(cache, name)
+        shape, want = ((b, h, length, half), torch.uint8) if name.endswith("codes") else ((b, h, length, d // 64, 2), dt)
+        if tuple(t.shape) != shape or t.dtype != want:
+            raise ValueError(f"{name} must be {want} of shape {shape}, not {t.dtype} of shape {tuple(t.shape)}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call's first tensor on {device}")
+    return (b, h, length, d, dt), {n: _ptr(getattr(cache, n)) for n in Kv4Cache._fields}
+
+
+def _kv4_rows_args(cache: Kv4Cache, k, v, start, rows, device):
+    (b, h, length, d, dt), ptrs = _kv4_parts(cache, device)
+    count = int(k.shape[2]) if k.dim() == 4 else -1
+    kp, ks = _rows4(k, "k", (b, h, count, d), dt, device)
+    vp, vs = _rows4(v, "v", (b, h, count, d), dt, device)
+    one = isinstance(start, int)
+    return L.Kv4RowsArgs(dtype=_dt(k), batch=b, n_kv_heads=h, rows=count, head_dim=d, cache_len=length, start_all=start if one else 0,
+                         start=None if one else _ints(start, "start", b, device), n_rows=_ints(rows, "rows", b, device),
+                         k=kp, v=vp, k_stride=ks, v_stride=vs, **ptrs)
+
+
+def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor], rows: Optional[torch.Tensor] = None) -> None:
+    """Quantise new rows into a 4-bit cache: row ``i`` of ``k, v (B, Hkv, S, D)`` becomes position ``start[b] + i``.
+
+    ``k`` and ``v`` may have any strides (multiples of 8, last axis contiguous): what a projection leaves,
+    ``(x @ wk).view(B, S, Hkv, D).transpose(1, 2)``, needs no copy.  ``start``: an int for all sequences or int32 ``(B,)``;
+    ``rows`` int32 ``(B,)``: how many of the ``S`` rows of each sequence are meant (default all).  Other rows, and rows
+    whose position lies outside the cache, are not written."""
+    with torch.cuda.device(_cuda_device(k)):
+        args = _kv4_rows_args(cache, k, v, start, rows, k.device)
+        L.check(L.load().tb200_kv4_append(C.byref(args), _stream()), "tb200_kv4_append")
+
+
+def kv4_read(cache: Kv4Cache, start: Union[int, torch.Tensor], count: int, rows: Optional[torch.Tensor] = None,
+             k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
+    """Rows ``[start[b], start[b] + count)`` of a 4-bit cache as 16-bit rows ``(B, Hkv, count, D)``: ``lo + c * s`` rounded
+    once (at most the type's largest number).  ``rows`` int32 ``(B,)`` limits how many are read of each sequence; the others, and positions outside the cache,
+    are left as they are in ``k_out, v_out`` (zero when these are not given).  Returns ``(k_out, v_out)``."""
+    dev = _cuda_device(cache.k_codes)
+    with torch.cuda.device(dev):
+        b, h, _, half = cache.k_codes.shape
+        make = lambda: torch.zeros(b, h, count, 2 * half, dtype=cache.k_meta.dtype, device=dev)
+        k_out = make() if k_out is None else k_out
+        v_out = make() if v_out is None else v_out
+        if k_out.dim() != 4 or k_out.shape[2] != count:
+            raise ValueError(f"k_out must have shape {(b, h, count, 2 * half)}, not {tuple(k_out.shape)}")
+        args = _kv4_rows_args(cache, k_out, v_out, start, rows, dev)
+        L.check(L.load().tb200_kv4_read(C.byref(args), _stream()), "tb200_kv4_read")
+    return k_out, v_out
+
+
+def _cuda_device(t: torch.Tensor) -> torch.device:
+    if not t.is_cuda:
+        raise ValueError("trinity_b200 operators take CUDA tensors (there is no CPU path)")
+    return t.device
+
+
+def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, **cache):
+    lib = L.load()
+    b, h, length, d, dt = dims
+    dev = q.device
+    if q.dim() != 4:
+        raise ValueError(f"q must have shape (B, Hq, S, D), not {tuple(q.shape)}")
+    hq, s = int(q.shape[1]), int(q.shape[2])
+    if kv_lens is None:
+        raise TypeError("kv_lens must be an int32 tensor")
+    if out is None:
+        out = torch.empty(b, s, hq, d, dtype=dt, device=dev).transpose(1, 2)
+        if q_rows is not None:
+            out.zero_()
+    qp, qs = _rows4(q, "q", (b, hq, s, d), dt, dev)
+    op, os_ = _rows4(out, "out", (b, hq, s, d), dt, dev)
+    args = L.CacheAttnArgs(dtype=_dt(q), batch=b, rows=s, n_q_heads=hq, n_kv_heads=h, head_dim=d, cache_len=length, window=window, sinks=sinks,
+                           sm_scale=sm_scale, q=qp, o=op, q_stride=qs, o_stride=os_, kv_lens=_ints(kv_lens, "kv_lens", b, dev),
+                           q_rows=_ints(q_rows, "q_rows", b, dev), **cache)
+    L.check(getattr(lib, name + "_check")(C.byref(args)), name)
+    need = getattr(lib, name + "_workspace_bytes")(C.byref(args))
+    ws = Workspace.get(dev, need, name)
+    args.workspace, args.workspace_bytes = _ptr(ws), need
+    L.check(getattr(lib, name)(C.byref(args), _stream()), name)
+    return out
+
+
+def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_lens: torch.Tensor, *, window: int = 0, sinks: int = 0,
+                sm_scale: float = 1.0, q_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``softmax(sm_scale * q K^T) V`` over 16-bit caches that already hold the new rows, with per-sequence lengths.
+
+    ``q (B, Hq, S, D)``, ``k_cache, v_cache (B, Hkv, L, D)``: any strides (multiples of 8, last axis contiguous).
+    ``kv_lens`` int32 ``(B,)``: positions in the cache, the new ones included; ``q_rows`` int32 ``(B,)``: how many of the
+    ``S`` query rows belong to the sequence (default all); they are the last positions.  A query sees the positions up to
+    its own, with ``window > 0`` only the last ``window`` of these and the first ``sinks`` ones.  A row that sees nothing
+    gives zeros.  Rows from ``q_rows`` on are left as they are in ``out`` (zero when it is not given).  Returns ``out``,
+    ``(B, Hq, S, D)``; by default laid out so that ``out.transpose(1, 2).reshape(B, S, Hq * D)`` is a view."""
+    dev = _cuda_device(q)
+    if k_cache.dim() != 4:
+        raise ValueError(f"k_cache must have shape (B, Hkv, L, D), not {tuple(k_cache.shape)}")
+    b, h, length, d = k_cache.shape
+    with torch.cuda.device(dev):
+        kp, ks = _rows4(k_cache, "k_cache", (b, h, length, d), q.dtype, dev)
+        vp, vs = _rows4(v_cache, "v_cache", (b, h, length, d), q.dtype, dev)
+        return _cache_attn("tb200_attn_window", q, out, kv_lens, q_rows, window, sinks, sm_scale, (b, h, length, d, q.dtype),
+                           k_cache=kp, v_cache=vp, k_stride=ks, v_stride=vs)
+
+
+def kv4_attn(q: torch.Tensor, cache: Kv4Cache, kv_lens: torch.Tensor, *, window: int = 0, sinks: int = 0, sm_scale: float = 1.0,
+             q_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attn_window`` over a 4-bit cache: the same arguments and the same result, with ``cache`` a :class:`Kv4Cache`."""
+    dev = _cuda_device(q)
+    with torch.cuda.device(dev):
+        dims, ptrs = _kv4_parts(cache, dev)
+        return _cache_attn("tb200_kv4_attn", q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, **ptrs)
 
 
 def device_status() -> int:
