@@ -1,7 +1,26 @@
 // Attention over a cache that already holds the new rows: tb200_attn_window (16-bit caches) and tb200_kv4_attn (4-bit
 // caches), per-sequence lengths, an optional sliding window with a few first positions that stay visible.
 //
-// One warp per (sequence, query head, query row): the keys one after the other, running maximum and sum.
+// cache_decode_kernel: few query rows per sequence.  Bound: HBM (the visible cache rows are read once per key/value
+// head), and the instructions that turn 4-bit codes into matrix operands.
+//
+//   unit     (sequence, kv head, R query rows): the rows of a unit are (new token, query head of the group) pairs, so
+//            that a cache row is read once for all query heads that share it.  R = 8 or 16 columns of an MMA.
+//   work     the key tiles of all units form one line, dealt out in equal stretches over the CTAs (each computes the
+//            line's layout from kv_lens itself): long and short sequences load the SMs evenly, with no host knowledge
+//            of the lengths.  A unit that lies within one CTA's stretch is finished there; the others leave a partial
+//            result (accumulator, maximum, sum) per stretch, which cache_combine_kernel merges in the order of the keys.
+//   warp     takes every fourth tile of a stretch: its own ring of bulk copies, no CTA-wide barrier inside a stretch.
+//   math     transposed: S^T = K Q^T (keys are the rows of the MMA, query rows its 8 columns), O^T = V^T P^T.
+//   4 bits   a code c needs no conversion: the bits c in the low mantissa of an otherwise zero fp16 are the number
+//            c * 2^-24, one nibble higher c * 2^-20, and the tensor core takes such (subnormal) numbers exactly.  One
+//            AND per two codes makes an operand.  With K = lo + c s per group of 64:  q.k = sum_g s_g (q.c)_g + lo_g sum(q)_g,
+//            so s and lo meet the scores in fp32 and no key is ever rounded.  With V:  o = sum_g [sum_j (p_j s_jg)(c_jd - 8) +
+//            sum_j p_j (lo_jg + 8 s_jg)]: the scale goes into the probability (rounded to fp16, after a power of two that
+//            keeps the largest p s below 2^14), the second sum is fp32, and the 8 is taken out with the SAME rounded
+//            probabilities (an MMA against a constant -8 into the same accumulator): the rounding error is that of centred codes,
+//            and the accumulator stays small, which matters because the tensor core's additions truncate.
+//            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 #include <math.h>
 
 #include "common.cuh"
@@ -12,39 +31,647 @@ namespace tb200 {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
 
 struct CacheAttnParams {
-  int B, S, Hq, Hkv, cache_len, window, sinks;
+  int B, S, Hq, Hkv, group, cache_len, window, sinks;
+  int row_tiles;             // units per (sequence, kv head) at most
   float scale_log2;
   const uint8_t* q;
   uint8_t* o;
   long long qs[3], os[3];
   const int32_t* kv_lens;
   const int32_t* q_rows;
-  const uint8_t* k16;
-  const uint8_t* v16;
-  long long ks[3], vs[3];
   const uint8_t *k_codes, *v_codes, *k_meta, *v_meta;
+  float* part_o;             // (2 grid, R, D)
+  float* part_ml;            // (2 grid, R, 2)
+  int stretches;             // CTAs of the decode kernel
+  int* err;
+  long long wait_limit;
 };
 
-template <typename T> __device__ __forceinline__ float to_f(T x) { return static_cast<float>(x); }
+// What a sequence asks for.
+struct Seq {
+  int n, r;                  // positions, new rows
+  int few;                   // first positions that stay visible, below the window
+  int sink_tiles, win_tile;  // tiles [0, sink_tiles) and from win_tile on
+  int tiles;                 // tiles of a unit
+  int units;                 // units of the sequence: kv heads x row tiles
+};
+__device__ __forceinline__ Seq load_seq(const CacheAttnParams& p, int b, int tile, int unit_rows) {
+  Seq s;
+  s.n = max(0, min(__ldg(p.kv_lens + b), p.cache_len));
+  s.r = p.q_rows ? max(0, min(__ldg(p.q_rows + b), p.S)) : p.S;
+  const int low = p.window > 0 ? max(0, s.n - s.r - p.window + 1) : 0;
+  s.few = min(p.sinks, low);
+  s.win_tile = low / tile;
+  s.sink_tiles = min((s.few + tile - 1) / tile, s.win_tile);
+  s.tiles = max(1, s.sink_tiles + (s.n + tile - 1) / tile - s.win_tile);   // a sequence without keys: one masked tile writes the zeros
+  s.units = s.r > 0 ? p.Hkv * ((s.r * p.group + unit_rows - 1) / unit_rows) : 0;
+  return s;
+}
 
-template <typename T, int D, bool KV4>
-__global__ void __launch_bounds__(kThreads) cache_attn_kernel(const CacheAttnParams p) {
+// The line of all tiles: its length, and how it is dealt out.  Every lane of a warp calls these and gets the same.
+struct Line {
+  int total;    // tiles of all units
+  int per;      // tiles of a stretch
+  int seq;      // the sequence in which position x lies
+  int base;     // the line's position of that sequence's first tile
+};
+// pick(total, per) chooses x, the position to look for (x >= total: seq and base are not set).
+template <typename Pick>
+__device__ __forceinline__ Line walk_line(const CacheAttnParams& p, int tile, int unit_rows, int min_tiles, Pick pick) {
+  const int lane = static_cast<int>(lane_id());
+  Line ln;
+  ln.seq = ln.base = 0;
+  int sum = 0, own = 0, total = 0;
+  auto scan = [&](int b0) {   // inclusive sums over 32 sequences
+    const int b = b0 + lane;
+    own = 0;
+    if (b < p.B) {
+      const Seq s = load_seq(p, b, tile, unit_rows);
+      own = s.tiles * s.units;
+    }
+    sum = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+  };
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    scan(b0);
+    total += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  ln.total = total;
+  ln.per = max((total + p.stretches - 1) / p.stretches, min_tiles);
+  const int x = pick(ln);
+  if (x >= total) return ln;
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    if (p.B > 32) scan(b0);   // else the sums are still there
+    const unsigned hit = __ballot_sync(0xffffffffu, before + sum > x);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      ln.seq = b0 + l;
+      ln.base = before + __shfl_sync(0xffffffffu, sum - own, l);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return ln;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// (s, lo) of a row's groups as floats
+template <typename T, int NG> __device__ __forceinline__ void load_meta(const uint8_t* at, float2 (&m)[NG]) {
+  if constexpr (NG == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(at);
+    m[0] = Pack2<T>::unpack(u.x);
+    m[1] = Pack2<T>::unpack(u.y);
+  } else {
+    m[0] = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(at));
+  }
+}
+
+constexpr int kTile = 64;     // keys of a tile
+constexpr int kStages = 2;
+constexpr float kSlack = 8.f; // the exponent reference of a row moves only when its maximum has grown by more than 2^kSlack
+constexpr int kMinTiles = kWarps;
+
+template <int D, int NT> struct DecSmem {
+  static constexpr int kR = 8 * NT;
+  static constexpr int kCodes = kTile * D / 2;             // bytes of one tile's codes
+  static constexpr int kMeta = kTile * (D / 64) * 4;
+  static constexpr int kStage = 2 * (kCodes + kMeta);      // K codes, V codes, K meta, V meta
+  static constexpr int kRing = kStages * kStage;           // per warp
+  static constexpr int kMergePitch = D + 4;                // floats per row: 4 keep the rows' banks apart
+  // the merge buffers take the place of the rings, which are empty by then
+  static constexpr int kMergeOff = 0;                      // float [warps][R][pitch]
+  static constexpr int kMlOff = kMergeOff + kWarps * kR * kMergePitch * 4;   // float2 [warps][R]
+  static constexpr int kBarOff = kWarps * kRing;
+  static_assert(kMlOff + kWarps * kR * 8 <= kBarOff, "the merge buffers must fit where the rings were");
+  static constexpr int kTotal = kBarOff + kWarps * kStages * 8 + 16;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel(const __grid_constant__ CacheAttnParams p) {
+  using L = DecSmem<D, NT>;
+  constexpr int NG = D / 64;
+  constexpr int R = L::kR;
+  extern __shared__ __align__(128) uint8_t smem[];
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * L::kRing;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff) + warp * kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kBarOff + kWarps * kStages * 8);
+  const AbortCtx ctx{p.err, abort_flag, p.wait_limit};
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&bars[i], 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  const Line ln = walk_line(p, kTile, R, kMinTiles, [&](const Line& l) { return l.per * static_cast<int>(blockIdx.x); });
+  int x = ln.per * static_cast<int>(blockIdx.x);
+  const int x_end = min(x + ln.per, ln.total);
+  if (x >= x_end) return;
+  int base = ln.base, b = ln.seq;
+  Seq sq = load_seq(p, b, kTile, R);
+  uint32_t used = 0;    // tiles this warp has taken through its ring
+  bool ok = true;
+
+  while (x < x_end) {   // one segment: the part of a unit that lies in this stretch
+    while (x >= base + sq.tiles * sq.units) {
+      base += sq.tiles * sq.units;
+      sq = load_seq(p, ++b, kTile, R);
+    }
+    const int unit = (x - base) / sq.tiles;
+    const int v0 = x - base - unit * sq.tiles;
+    const int v1 = min(sq.tiles, v0 + x_end - x);
+    const int rts = sq.units / p.Hkv;
+    const int h = unit / rts, rt = unit - h * rts;
+    const long long crow = (static_cast<long long>(b) * p.Hkv + h) * p.cache_len;
+    const int copy_end = min(p.cache_len, max(4, (sq.n + 3) & ~3));   // cache rows worth copying: whole 16 bytes of meta
+
+    // lanes 0 to 3 fetch a tile's K codes, V codes, K meta, V meta: each has its own source, row size and place
+    const int what = lane & 3;
+    const uint32_t row_bytes = what < 2 ? D / 2 : NG * 4;
+    const uint8_t* src = (what == 0 ? p.k_codes : what == 1 ? p.v_codes : what == 2 ? p.k_meta : p.v_meta) + crow * row_bytes;
+    uint8_t* dst = ring + (what & 1) * (what < 2 ? L::kCodes : L::kMeta) + (what < 2 ? 0 : 2 * L::kCodes);
+    auto issue = [&](int v, uint32_t slot) {   // whole warp: tile v of the unit into ring slot `slot`
+      const int k0 = (v < sq.sink_tiles ? v : sq.win_tile + v - sq.sink_tiles) * kTile;
+      const uint32_t rows = static_cast<uint32_t>(min(kTile, copy_end - k0));
+      if (lane == 0) mbar_arrive_expect_tx(&bars[slot], rows * (D + NG * 8));
+      __syncwarp();
+      if (lane < 4) bulk_load(dst + slot * L::kStage, src + static_cast<long long>(k0) * row_bytes, rows * row_bytes, &bars[slot]);
+    };
+    auto drain = [&](int v) {   // a wait gave up: the copies in flight (tile v and those behind it) get their time to land
+      for (int i = 0; i < kStages && v + i * kWarps < v1; ++i) {
+        const uint32_t u = used + i;
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&bars[u % kStages], (u / kStages) & 1) && clock64() - t0 < p.wait_limit) {
+        }
+      }
+    };
+    if (ok) {
+#pragma unroll
+      for (int i = 0; i < kStages; ++i)
+        if (v0 + warp + i * kWarps < v1) issue(v0 + warp + i * kWarps, (used + i) % kStages);
+    }
+
+    // ---- the unit's query rows: MMA column m is row rt * R + m, i.e. (token, query head of the group)
+    const int n_rows = sq.r * p.group;
+    uint32_t qf[NT][NG][4][2];
+    float2 qs[NT][NG], cf[NT];
+    int cpos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int m = rt * R + nt * 8 + g;
+      const bool live = m < n_rows;
+      const int tok = live ? m / p.group : 0;
+      const int hq = h * p.group + (live ? m - tok * p.group : 0);
+      const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + hq * p.qs[1] + tok * p.qs[2] + t * 16;
+      float v[NG][16];
+      float top = 0.f, sum[NG];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        sum[gr] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 raw = live ? __ldg(reinterpret_cast<const uint4*>(qp + gr * 64) + i) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = Pack2<T>::unpack(w[e]);
+            v[gr][i * 8 + 2 * e] = f.x;
+            v[gr][i * 8 + 2 * e + 1] = f.y;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          top = fmaxf(top, fabsf(v[gr][e]));
+          sum[gr] += v[gr][e];
+        }
+        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
+        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // a power of two that brings the row's largest magnitude to [8, 16)
+      const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 30);
+      const float up = __uint_as_float(static_cast<uint32_t>(257 - ex) << 23);        // 2^(130 - ex)
+      const float down = __uint_as_float(static_cast<uint32_t>(ex - 3) << 23);        // its inverse
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const int e = (ks >> 1) * 8 + (ks & 1) * 2;
+          qf[nt][gr][ks][0] = Pack2<__half>::pack(v[gr][e] * up, v[gr][e + 4] * up);
+          qf[nt][gr][ks][1] = Pack2<__half>::pack(v[gr][e + 1] * up * 0.0625f, v[gr][e + 5] * up * 0.0625f);
+        }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {   // what columns 2t and 2t + 1 need of their rows
+        const int src = (2 * t + c) * 4;
+        const float u = __shfl_sync(0xffffffffu, up, src);
+        // 2^24, and never 0: a hidden score is -inf times this
+        const float f = fmaxf(__shfl_sync(0xffffffffu, down, src) * (p.scale_log2 * 16777216.f), 1.17549435e-38f);
+        if (c == 0) cf[nt].x = f; else cf[nt].y = f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const float q1 = __shfl_sync(0xffffffffu, sum[gr], src) * u * 5.9604644775390625e-8f;   // 2^-24
+          if (c == 0) qs[nt][gr].x = q1; else qs[nt][gr].y = q1;
+        }
+        const int mc = rt * R + nt * 8 + 2 * t + c;
+        cpos[nt][c] = mc < n_rows ? sq.n - sq.r + mc / p.group : -1;
+      }
+    }
+
+    float o[NT][NG][4][4], mx[NT][2];
+    float2 z[NT][NG], l[NT], nmref[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][gr][i][e] = 0.f;
+        z[nt][gr] = make_float2(0.f, 0.f);
+      }
+      mx[nt][0] = mx[nt][1] = -INFINITY;
+      l[nt] = nmref[nt] = make_float2(0.f, 0.f);
+    }
+    int ev = 30;   // biased exponent of the largest V scale so far
+
+    for (int v = v0 + warp; v < v1; v += kWarps) {
+      const uint32_t slot = used % kStages;
+      if (!ok || !mbar_wait(&bars[slot], (used / kStages) & 1, ctx, 701)) {   // (the CTA goes on to its barriers without this warp's keys)
+        if (ok) drain(v);
+        ok = false;
+        break;
+      }
+      const uint8_t* st = ring + slot * L::kStage;
+      const uint8_t* kc = st;
+      const uint8_t* vc = st + L::kCodes;
+      const uint8_t* km = st + 2 * L::kCodes;
+      const uint8_t* vm = km + L::kMeta;
+      const int tile = v < sq.sink_tiles ? v : sq.win_tile + v - sq.sink_tiles;
+      const int k0 = tile * kTile;
+      // every key of the tile visible to every row of the sequence?
+      const bool full = k0 + kTile - 1 <= sq.n - sq.r && (p.window == 0 || k0 > sq.n - 1 - p.window || k0 + kTile - 1 < p.sinks);
+
+      float2 s[kTile / 16][NT][2];   // [keys g, g + 8][rows 2t, 2t + 1], without the row's factor cf
+#pragma unroll
+      for (int sp = 0; sp < kTile / 16; ++sp) {
+        // MMA row (slot) 2a + e of eight is key a + 4 e: the four lanes of a column pair then read neighbouring rows
+        const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
+        float acc[NT][NG][4];
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const uint2 w0 = *reinterpret_cast<const uint2*>(kc + key0 * (D / 2) + gr * 32 + t * 8);
+          const uint2 w1 = *reinterpret_cast<const uint2*>(kc + key1 * (D / 2) + gr * 32 + t * 8);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[nt][gr][0] = acc[nt][gr][1] = acc[nt][gr][2] = acc[nt][gr][3] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const uint32_t x0 = ((ks & 2) ? w0.y : w0.x) >> ((ks & 1) * 8), x1 = ((ks & 2) ? w1.y : w1.x) >> ((ks & 1) * 8);
+            const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
+          }
+        }
+        float2 m0[NG], m1[NG];
+        load_meta<T, NG>(km + key0 * (NG * 4), m0);
+        load_meta<T, NG>(km + key1 * (NG * 4), m1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float2 y0 = __fmul2_rn(make_float2(m0[0].y, m0[0].y), qs[nt][0]), y1 = __fmul2_rn(make_float2(m1[0].y, m1[0].y), qs[nt][0]);
+          if constexpr (NG == 2) {
+            y0 = __ffma2_rn(make_float2(m0[1].y, m0[1].y), qs[nt][1], y0);
+            y1 = __ffma2_rn(make_float2(m1[1].y, m1[1].y), qs[nt][1], y1);
+          }
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            y0 = __ffma2_rn(make_float2(m0[gr].x, m0[gr].x), make_float2(acc[nt][gr][0], acc[nt][gr][1]), y0);
+            y1 = __ffma2_rn(make_float2(m1[gr].x, m1[gr].x), make_float2(acc[nt][gr][2], acc[nt][gr][3]), y1);
+          }
+          s[sp][nt][0] = y0; s[sp][nt][1] = y1;
+        }
+        if (!full) {
+          const int a = k0 + key0, d = k0 + key1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            auto sees = [&](int key, int pos) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks); };
+            if (!sees(a, cpos[nt][0])) s[sp][nt][0].x = -INFINITY;
+            if (!sees(a, cpos[nt][1])) s[sp][nt][0].y = -INFINITY;
+            if (!sees(d, cpos[nt][0])) s[sp][nt][1].x = -INFINITY;
+            if (!sees(d, cpos[nt][1])) s[sp][nt][1].y = -INFINITY;
+          }
+        }
+      }
+
+      // ---- running maximum of the scores and of the V scales: what a thread sees of either decides whether the warp has
+      //      to look closer
+      uint32_t big = 0;
+#pragma unroll
+      for (int i = 0; i < kTile / 32; ++i) {
+        const int key = i * 32 + lane;
+        bool alive = true;
+        if (!full) {
+          const int a = k0 + key;
+          alive = a < sq.n && (p.window == 0 || a > sq.n - sq.r - p.window || a < p.sinks);
+        }
+        float2 mv[NG];
+        load_meta<T, NG>(vm + key * (NG * 4), mv);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const uint32_t u = __float_as_uint(mv[gr].x);
+          if (alive && u < 0x7f800000u) big = max(big, u);
+        }
+      }
+      float top[NT][2];
+      bool grown = static_cast<int>(big >> 23) > ev;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float t0 = fmaxf(s[0][nt][0].x, s[0][nt][1].x), t1 = fmaxf(s[0][nt][0].y, s[0][nt][1].y);
+#pragma unroll
+        for (int sp = 1; sp < kTile / 16; ++sp) {
+          t0 = max3(t0, s[sp][nt][0].x, s[sp][nt][1].x);
+          t1 = max3(t1, s[sp][nt][0].y, s[sp][nt][1].y);
+        }
+        top[nt][0] = t0 * cf[nt].x;
+        top[nt][1] = t1 * cf[nt].y;
+        grown |= top[nt][0] > mx[nt][0] + kSlack || top[nt][1] > mx[nt][1] + kSlack;
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+        const int ev_new = max(ev, static_cast<int>(__reduce_max_sync(0xffffffffu, big) >> 23));
+        const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 + ev - ev_new, 0)) << 23);   // 2^(ev - ev_new)
+        ev = ev_new;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float a[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m_new = top[nt][c];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
+            m_new = fmaxf(m_new, mx[nt][c]);
+            a[c] = m_new == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - m_new);
+            mx[nt][c] = m_new;
+          }
+          const float2 a2 = make_float2(a[0], a[1]), as2 = make_float2(a[0] * shrink, a[1] * shrink);
+          nmref[nt] = make_float2(mx[nt][0] == -INFINITY ? 0.f : -mx[nt][0], mx[nt][1] == -INFINITY ? 0.f : -mx[nt][1]);
+          l[nt] = __fmul2_rn(l[nt], a2);
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            z[nt][gr] = __fmul2_rn(z[nt][gr], a2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][gr][i][e] *= (e & 1) ? as2.y : as2.x;
+          }
+        }
+      }
+      const float sfac = __uint_as_float(static_cast<uint32_t>(259 - ev) << 23);   // 2^(5 - exponent): with p <= 2^kSlack, p s sfac < 2^14
+
+#pragma unroll
+      for (int sp = 0; sp < kTile / 16; ++sp) {
+        const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
+        float2 e[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 y = __ffma2_rn(s[sp][nt][k], cf[nt], nmref[nt]);
+            e[nt][k] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+            l[nt] = __fadd2_rn(l[nt], e[nt][k]);
+          }
+        float2 m0[NG], m1[NG];
+        load_meta<T, NG>(vm + key0 * (NG * 4), m0);
+        load_meta<T, NG>(vm + key1 * (NG * 4), m1);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const float s0 = m0[gr].x * sfac, s1 = m1[gr].x * sfac, c0 = fmaf(8.f, m0[gr].x, m0[gr].y), c1 = fmaf(8.f, m1[gr].x, m1[gr].y);
+          uint32_t pf[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float2 w0 = __fmul2_rn(e[nt][0], make_float2(s0, s0)), w1 = __fmul2_rn(e[nt][1], make_float2(s1, s1));
+            if (full) {
+              z[nt][gr] = __ffma2_rn(e[nt][0], make_float2(c0, c0), z[nt][gr]);
+              z[nt][gr] = __ffma2_rn(e[nt][1], make_float2(c1, c1), z[nt][gr]);
+            } else {   // what a row does not see may hold anything: 0 * inf and 0 * NaN must not arise
+              if (e[nt][0].x > 0.f) z[nt][gr].x = fmaf(e[nt][0].x, c0, z[nt][gr].x); else w0.x = 0.f;
+              if (e[nt][0].y > 0.f) z[nt][gr].y = fmaf(e[nt][0].y, c0, z[nt][gr].y); else w0.y = 0.f;
+              if (e[nt][1].x > 0.f) z[nt][gr].x = fmaf(e[nt][1].x, c1, z[nt][gr].x); else w1.x = 0.f;
+              if (e[nt][1].y > 0.f) z[nt][gr].y = fmaf(e[nt][1].y, c1, z[nt][gr].y); else w1.y = 0.f;
+            }
+            pf[nt][0] = transpose8x8(Pack2<__half>::pack(w0.x, w0.y));
+            pf[nt][1] = transpose8x8(Pack2<__half>::pack(w1.x, w1.y));
+          }
+          // MMA columns 2t, 2t+1 (and 2t+8, 2t+9) of V^T are keys t, t + 4 (and t + 8, t + 12); row g of the four row tiles
+          // holds elements 8 g + {0, 2, 4, 6}, row g + 8 the odd ones
+          const uint8_t* vp = vc + (sp * 16 + t) * (D / 2) + gr * 32 + g * 4;
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(vp), wb = *reinterpret_cast<const uint32_t*>(vp + 4 * (D / 2));
+          const uint32_t wc = *reinterpret_cast<const uint32_t*>(vp + 8 * (D / 2)), wd = *reinterpret_cast<const uint32_t*>(vp + 12 * (D / 2));
+          const uint32_t xl = __byte_perm(wa, wb, 0x5410), xh = __byte_perm(wa, wb, 0x7632);
+          const uint32_t yl = __byte_perm(wc, wd, 0x5410), yh = __byte_perm(wc, wd, 0x7632);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x0 = ((i & 2) ? xh : xl) >> ((i & 1) * 8), y0 = ((i & 2) ? yh : yl) >> ((i & 1) * 8);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(o[nt][gr][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+              // minus 8 p: -8 * 2^-24 in row g, -8 * 2^-20 in row g + 8
+              mma_f16(o[nt][gr][i], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[nt][0], pf[nt][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();   // every lane has read the slot
+      if (v + kStages * kWarps < v1) issue(v + kStages * kWarps, slot);
+      ++used;
+    }
+
+    // ---- this warp's share of the segment into shared memory: o relative to its own maximum
+    __syncthreads();   // every warp is done with its ring
+    float* wm = reinterpret_cast<float*>(smem + L::kMergeOff) + warp * R * L::kMergePitch;
+    float2* wml = reinterpret_cast<float2*>(smem + L::kMlOff) + warp * R;
+    const float fe = __uint_as_float(static_cast<uint32_t>(ev) << 23);   // 2^24 / sfac = 2^19 * 2^(ev - 127)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int m = nt * 8 + 2 * t + c;
+        float ls = c ? l[nt].y : l[nt].x;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, d);
+        if (g == 0) wml[m] = make_float2(mx[nt][c], ls);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float zs = c ? z[nt][gr].y : z[nt][gr].x;
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) zs += __shfl_xor_sync(0xffffffffu, zs, d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float2*>(wm + m * L::kMergePitch + gr * 64 + g * 8 + 2 * i) =
+                make_float2(fmaf(o[nt][gr][i][c] * 524288.f, fe, zs), fmaf(o[nt][gr][i][2 + c] * 32768.f, fe, zs));   // 2^19, 2^15
+        }
+      }
+    __syncthreads();
+    // ---- the four warps' shares, in a fixed order
+    const bool whole = v0 == 0 && v1 == sq.tiles;
+    const float* mall = reinterpret_cast<const float*>(smem + L::kMergeOff);
+    const float2* mlall = reinterpret_cast<const float2*>(smem + L::kMlOff);
+    const int slot_out = 2 * blockIdx.x + (v0 == 0 ? 1 : 0);
+    for (int i = threadIdx.x; i < R * D / 4; i += kThreads) {
+      const int m = i / (D / 4), d = (i % (D / 4)) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, mlall[w * R + m].x);
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = mlall[w * R + m];
+        const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+        const float4 a = *reinterpret_cast<const float4*>(mall + (w * R + m) * L::kMergePitch + d);
+        sum = fmaf(f, ml.y, sum);
+        acc.x = fmaf(f, a.x, acc.x); acc.y = fmaf(f, a.y, acc.y); acc.z = fmaf(f, a.z, acc.z); acc.w = fmaf(f, a.w, acc.w);
+      }
+      if (whole) {
+        const int mr = rt * R + m;
+        if (mr < n_rows) {
+          const float inv = sum > 0.f ? 1.f / sum : sum;   // 0: the row sees nothing; NaN stays
+          const int tok = mr / p.group;
+          T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + d;
+          *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
+        }
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (static_cast<long long>(slot_out) * R + m) * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot_out) * R + m) * 2) = make_float2(top, sum);
+      }
+    }
+    fence_proxy_async_smem();   // the next bulk copies overwrite what was just read and written
+    __syncthreads();
+    x += v1 - v0;
+  }
+}
+
+// Merges the partial results of the units that lie in several stretches.  CTA (c, y): the unit that begins in stretch c
+// and goes on behind its end, if there is one, and of it the rows y, y + gridDim.y, ...; its first part is in slot 2c + 1,
+// the others in the slots 2c' of the stretches c' it covers.
+constexpr int kCombineThreads = 128;
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kCombineThreads) cache_combine_kernel(const __grid_constant__ CacheAttnParams p) {
+  constexpr int R = 8 * NT;
+  constexpr int kLanes = D / 4, kParts = kCombineThreads / kLanes;   // parts summed side by side
+  extern __shared__ float weights[];                                 // [stretches]
+  __shared__ float4 red[kParts][kLanes];
+  __shared__ float2 tops[kCombineThreads / 32];
+  pdl_launch_dependents();
+  const int c = blockIdx.x;
+  const Line ln = walk_line(p, kTile, R, kMinTiles, [&](const Line& l) { return l.per * (c + 1) - 1; });
+  const int end = ln.per * (c + 1);
+  bool mine = end < ln.total;
+  Seq sq;
+  int unit = 0, u1 = 0, rts = 1;
+  if (mine) {
+    sq = load_seq(p, ln.seq, kTile, R);
+    unit = (end - 1 - ln.base) / sq.tiles;
+    const int u0 = ln.base + unit * sq.tiles;
+    u1 = u0 + sq.tiles;
+    rts = sq.units / p.Hkv;
+    mine = u1 > end && u0 >= ln.per * c;
+  }
+  pdl_wait();
+  if (!mine) return;
+  const int b = ln.seq, h = unit / rts, rt = unit - h * rts;
+  const int parts = (u1 - 1) / ln.per - c + 1;
+  const int tid = threadIdx.x;
+  for (int m = blockIdx.y; m < R; m += gridDim.y) {
+    const int mr = rt * R + m;
+    if (mr >= sq.r * p.group) break;
+    auto slot = [&](int i) { return static_cast<long long>(2 * (c + i) + (i == 0 ? 1 : 0)) * R + m; };
+    // weights of the parts, their common maximum and sum
+    float top = -INFINITY;
+    for (int i = tid; i < parts; i += kCombineThreads) top = fmaxf(top, __ldcg(p.part_ml + slot(i) * 2));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if ((tid & 31) == 0) tops[tid >> 5].x = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kCombineThreads / 32; ++w) top = fmaxf(top, tops[w].x);
+    float sum = 0.f;
+    for (int i = tid; i < parts; i += kCombineThreads) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2));
+      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+      weights[i] = f;
+      sum = fmaf(f, ml.y, sum);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if ((tid & 31) == 0) tops[tid >> 5].y = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kCombineThreads / 32; ++w) sum += tops[w].y;
+    const int part = tid / kLanes, d4 = tid % kLanes;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = part; i < parts; i += kParts) {
+      const float f = weights[i];
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot(i) * D) + d4);
+      acc.x = fmaf(f, a.x, acc.x); acc.y = fmaf(f, a.y, acc.y); acc.z = fmaf(f, a.z, acc.z); acc.w = fmaf(f, a.w, acc.w);
+    }
+    red[part][d4] = acc;
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int w = 1; w < kParts; ++w) {
+        const float4 a = red[w][d4];
+        acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
+      }
+      const float inv = sum > 0.f ? 1.f / sum : sum;
+      const int tok = mr / p.group;
+      T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + d4 * 4;
+      *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
+    }
+    __syncthreads();   // tops, weights and red are free again
+  }
+}
+
+// The 16-bit caches: one warp per (sequence, query head, query row), the keys one after the other.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) cache_rows_kernel(const CacheAttnParams p, const T* k16, const T* v16, long long ks0, long long ks1, long long ks2,
+                                                          long long vs0, long long vs1, long long vs2) {
   constexpr int V = D / 32;   // columns per lane
   const int lane = threadIdx.x & 31;
   const long long rows = static_cast<long long>(p.B) * p.Hq * p.S;
-  const long long step = static_cast<long long>(gridDim.x) * (kThreads / 32);
-  for (long long w = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); w < rows; w += step) {
+  for (long long w = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < rows; w += static_cast<long long>(gridDim.x) * 8) {
     const int i = static_cast<int>(w % p.S);
     const int hq = static_cast<int>((w / p.S) % p.Hq);
     const int b = static_cast<int>(w / (static_cast<long long>(p.S) * p.Hq));
     const int n = max(0, min(p.kv_lens[b], p.cache_len));
     const int r = p.q_rows ? max(0, min(p.q_rows[b], p.S)) : p.S;
     if (i >= r) continue;
-    const int hkv = hq / (p.Hq / p.Hkv);
+    const int hkv = hq / p.group;
     const int at = n - r + i;
     const int low = p.window > 0 ? max(0, at - p.window + 1) : 0;
     const int few = min(p.sinks, low);
@@ -52,36 +679,17 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const CacheAttnPar
     const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + hq * p.qs[1] + i * p.qs[2] + lane * V;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      q[e] = to_f(qp[e]) * p.scale_log2;
+      q[e] = static_cast<float>(qp[e]) * p.scale_log2;
       o[e] = 0.f;
     }
     float m = -INFINITY, l = 0.f;
     for (int x = 0; x < few + at + 1 - low; ++x) {
       const int j = x < few ? x : x - few + low;
-      float k[V], v[V];
-      if constexpr (KV4) {
-        const long long row = (static_cast<long long>(b) * p.Hkv + hkv) * p.cache_len + j;
-        const int c0 = lane * V;
-        const T* km = reinterpret_cast<const T*>(p.k_meta) + (row * (D / 64) + c0 / 64) * 2;
-        const T* vm = reinterpret_cast<const T*>(p.v_meta) + (row * (D / 64) + c0 / 64) * 2;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int sh = ((c0 + e) & 1) * 4;
-          k[e] = fmaf(static_cast<float>((p.k_codes[row * (D / 2) + (c0 + e) / 2] >> sh) & 15), to_f(km[0]), to_f(km[1]));
-          v[e] = fmaf(static_cast<float>((p.v_codes[row * (D / 2) + (c0 + e) / 2] >> sh) & 15), to_f(vm[0]), to_f(vm[1]));
-        }
-      } else {
-        const T* kp = reinterpret_cast<const T*>(p.k16) + b * p.ks[0] + hkv * p.ks[1] + j * p.ks[2] + lane * V;
-        const T* vp = reinterpret_cast<const T*>(p.v16) + b * p.vs[0] + hkv * p.vs[1] + j * p.vs[2] + lane * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          k[e] = to_f(kp[e]);
-          v[e] = to_f(vp[e]);
-        }
-      }
+      const T* kp = k16 + b * ks0 + hkv * ks1 + j * ks2 + lane * V;
+      const T* vp = v16 + b * vs0 + hkv * vs1 + j * vs2 + lane * V;
       float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) s = fmaf(q[e], k[e], s);
+      for (int e = 0; e < V; ++e) s = fmaf(q[e], static_cast<float>(kp[e]), s);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
       const float m_new = fmaxf(m, s);
@@ -90,20 +698,23 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const CacheAttnPar
       m = m_new;
       l = fmaf(l, a, pr);
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = fmaf(o[e], a, pr * v[e]);
+      for (int e = 0; e < V; ++e) o[e] = fmaf(o[e], a, pr * static_cast<float>(vp[e]));
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const float inv = l > 0.f ? 1.f / l : l;
     T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + hq * p.os[1] + i * p.os[2] + lane * V;
 #pragma unroll
     for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(op + e) = Pack2<T>::pack(o[e] * inv, o[e + 1] * inv);
   }
 }
 
+constexpr int kMaxExtent = 1 << 30;
+
 int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   if (a == nullptr) return TB200_ERR_INVALID;
   if (a->dtype != TB200_BF16 && a->dtype != TB200_F16) return TB200_ERR_UNSUPPORTED;
   if (a->head_dim != 64 && a->head_dim != 128) return TB200_ERR_UNSUPPORTED;
   if (a->batch < 0 || a->rows < 0 || a->n_kv_heads < 1 || a->n_q_heads < 1 || a->n_q_heads % a->n_kv_heads || a->cache_len < 1) return TB200_ERR_INVALID;
+  if (a->batch > kMaxExtent || a->cache_len > kMaxExtent || static_cast<int64_t>(a->n_q_heads) * a->rows > kMaxExtent) return TB200_ERR_INVALID;
   if (a->window < 0 || a->sinks < 0 || !(a->sm_scale > 0.f) || !(a->sm_scale < INFINITY)) return TB200_ERR_INVALID;
   if (!a->q || !a->o || !a->kv_lens || a->q == a->o || !aligned16(a->q) || !aligned16(a->o) || !aligned4(a->kv_lens) || !aligned4(a->q_rows))
     return TB200_ERR_INVALID;
@@ -122,12 +733,77 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   return TB200_OK;
 }
 
-template <typename T, int D, bool KV4>
-int launch_simple(const CacheAttnParams& p, int num_sms, cudaStream_t stream) {
+// CTAs of the decode kernel that an SM holds: by shared memory (72 KB with 8 query rows, 90 KB with 16 at D = 128)
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+
+struct AttnPlan {
+  int nt = 1;                // MMA column blocks of a unit
+  int stretches = 0;
+  size_t part_o = 0, part_ml = 0;
+};
+AttnPlan plan_attn(const tb200_cache_attn_args* a, int num_sms) {
+  AttnPlan pl;
+  const int64_t rows = static_cast<int64_t>(a->rows) * (a->n_q_heads / a->n_kv_heads);
+  pl.nt = rows <= 8 ? 1 : 2;
+  pl.stretches = num_sms * ctas_per_sm(pl.nt);
+  pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * a->head_dim * sizeof(float), 256);
+  pl.part_ml = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * 2 * sizeof(float), 256);
+  return pl;
+}
+
+CacheAttnParams make_params(const tb200_cache_attn_args* a, const DeviceState* st) {
+  CacheAttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.B = a->batch; p.S = a->rows; p.Hq = a->n_q_heads; p.Hkv = a->n_kv_heads; p.group = a->n_q_heads / a->n_kv_heads;
+  p.cache_len = a->cache_len;
+  p.window = a->window < a->cache_len ? a->window : 0;   // a window as long as the cache hides nothing
+  p.sinks = p.window > 0 ? (a->sinks < a->cache_len ? a->sinks : a->cache_len) : 0;
+  p.scale_log2 = a->sm_scale * kLog2e;
+  p.q = static_cast<const uint8_t*>(a->q);
+  p.o = static_cast<uint8_t*>(a->o);
+  for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_stride[i]; p.os[i] = a->o_stride[i]; }
+  p.kv_lens = a->kv_lens; p.q_rows = a->q_rows;
+  p.k_codes = static_cast<const uint8_t*>(a->k_codes);
+  p.v_codes = static_cast<const uint8_t*>(a->v_codes);
+  p.k_meta = static_cast<const uint8_t*>(a->k_meta);
+  p.v_meta = static_cast<const uint8_t*>(a->v_meta);
+  p.err = st->err_word;
+  p.wait_limit = wait_limit_cycles();
+  return p;
+}
+
+template <typename T, int D, int NT>
+int launch_decode(const CacheAttnParams& p, cudaStream_t stream) {
+  using L = DecSmem<D, NT>;
+  static bool attr_set[32] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_set[dev & 31]) {
+    if (cudaFuncSetAttribute(cache_decode_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return TB200_ERR_CUDA;
+    attr_set[dev & 31] = true;
+  }
+  if (launch_chained(cache_decode_kernel<T, D, NT>, dim3(p.stretches), dim3(kThreads), L::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
+  // few units are split over many stretches each: a CTA per row of a unit; many units: one CTA for all rows
+  int combine_rows = 1;
+  while (combine_rows < 8 * NT && static_cast<long long>(p.B) * p.Hkv * combine_rows * 2 <= 256) combine_rows *= 2;
+  if (launch_chained(cache_combine_kernel<T, D, NT>, dim3(p.stretches, combine_rows), dim3(kCombineThreads), p.stretches * sizeof(float), stream, p) != cudaSuccess)
+    return TB200_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+}
+
+template <typename T>
+int run_kv4(const CacheAttnParams& p, int head_dim, int nt, cudaStream_t stream) {
+  if (head_dim == 128) return nt == 1 ? launch_decode<T, 128, 1>(p, stream) : launch_decode<T, 128, 2>(p, stream);
+  return nt == 1 ? launch_decode<T, 64, 1>(p, stream) : launch_decode<T, 64, 2>(p, stream);
+}
+
+template <typename T, int D>
+int launch_rows16(const CacheAttnParams& p, const tb200_cache_attn_args* a, int num_sms, cudaStream_t stream) {
   const long long rows = static_cast<long long>(p.B) * p.Hq * p.S;
-  long long blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
+  long long blocks = (rows + 7) / 8;
   if (blocks > num_sms * 8) blocks = num_sms * 8;
-  cache_attn_kernel<T, D, KV4><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
+  cache_rows_kernel<T, D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, static_cast<const T*>(a->k_cache), static_cast<const T*>(a->v_cache),
+      a->k_stride[0], a->k_stride[1], a->k_stride[2], a->v_stride[0], a->v_stride[1], a->v_stride[2]);
   return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
 }
 
@@ -139,27 +815,20 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   if (!st) return status;
   if (a->batch == 0 || a->rows == 0) return TB200_OK;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  CacheAttnParams p;
-  p.B = a->batch; p.S = a->rows; p.Hq = a->n_q_heads; p.Hkv = a->n_kv_heads; p.cache_len = a->cache_len;
-  p.window = a->window; p.sinks = a->window > 0 ? a->sinks : 0;
-  p.scale_log2 = a->sm_scale * kLog2e;
-  p.q = static_cast<const uint8_t*>(a->q);
-  p.o = static_cast<uint8_t*>(a->o);
-  for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_stride[i]; p.os[i] = a->o_stride[i]; p.ks[i] = a->k_stride[i]; p.vs[i] = a->v_stride[i]; }
-  p.kv_lens = a->kv_lens; p.q_rows = a->q_rows;
-  p.k16 = static_cast<const uint8_t*>(a->k_cache);
-  p.v16 = static_cast<const uint8_t*>(a->v_cache);
-  p.k_codes = static_cast<const uint8_t*>(a->k_codes);
-  p.v_codes = static_cast<const uint8_t*>(a->v_codes);
-  p.k_meta = static_cast<const uint8_t*>(a->k_meta);
-  p.v_meta = static_cast<const uint8_t*>(a->v_meta);
-  const bool d128 = a->head_dim == 128;
-  if (a->dtype == TB200_BF16) {
-    if (kv4) return d128 ? launch_simple<__nv_bfloat16, 128, true>(p, st->num_sms, stream) : launch_simple<__nv_bfloat16, 64, true>(p, st->num_sms, stream);
-    return d128 ? launch_simple<__nv_bfloat16, 128, false>(p, st->num_sms, stream) : launch_simple<__nv_bfloat16, 64, false>(p, st->num_sms, stream);
+  CacheAttnParams p = make_params(a, st);
+  if (!kv4) {
+    if (a->dtype == TB200_BF16)
+      return a->head_dim == 128 ? launch_rows16<__nv_bfloat16, 128>(p, a, st->num_sms, stream) : launch_rows16<__nv_bfloat16, 64>(p, a, st->num_sms, stream);
+    return a->head_dim == 128 ? launch_rows16<__half, 128>(p, a, st->num_sms, stream) : launch_rows16<__half, 64>(p, a, st->num_sms, stream);
   }
-  if (kv4) return d128 ? launch_simple<__half, 128, true>(p, st->num_sms, stream) : launch_simple<__half, 64, true>(p, st->num_sms, stream);
-  return d128 ? launch_simple<__half, 128, false>(p, st->num_sms, stream) : launch_simple<__half, 64, false>(p, st->num_sms, stream);
+  const AttnPlan pl = plan_attn(a, st->num_sms);
+  if (!a->workspace || a->workspace_bytes < pl.part_o + pl.part_ml) return TB200_ERR_WORKSPACE;
+  if (!aligned16(a->workspace)) return TB200_ERR_INVALID;
+  p.stretches = pl.stretches;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
+  ChainScope chain;
+  return a->dtype == TB200_BF16 ? run_kv4<__nv_bfloat16>(p, a->head_dim, pl.nt, stream) : run_kv4<__half>(p, a->head_dim, pl.nt, stream);
 }
 
 }  // namespace
@@ -172,7 +841,13 @@ extern "C" {
 int tb200_attn_window_check(const tb200_cache_attn_args* a) { return check_attn(a, false); }
 int tb200_kv4_attn_check(const tb200_cache_attn_args* a) { return check_attn(a, true); }
 size_t tb200_attn_window_workspace_bytes(const tb200_cache_attn_args*) { return 0; }
-size_t tb200_kv4_attn_workspace_bytes(const tb200_cache_attn_args*) { return 0; }
+size_t tb200_kv4_attn_workspace_bytes(const tb200_cache_attn_args* a) {
+  int status = TB200_OK;
+  DeviceState* st = device_state(&status);
+  if (!st || check_attn(a, true) != TB200_OK) return 0;
+  const AttnPlan pl = plan_attn(a, st->num_sms);
+  return pl.part_o + pl.part_ml;
+}
 int tb200_attn_window(const tb200_cache_attn_args* a, void* stream) { return run_attn(a, false, stream); }
 int tb200_kv4_attn(const tb200_cache_attn_args* a, void* stream) { return run_attn(a, true, stream); }
 
