@@ -20,6 +20,11 @@
 // (issued after P_j V_j) cannot overwrite P_j early, and an arrival on s_full also means the previous P V is done.
 // The first P V of an item overwrites O, so it waits until the output warpgroup has read the previous item's O (o_free).
 //
+// SEQ instances (launch_attn_fwd_seq) serve caches with per-sequence lengths and a sliding window: an item's key tiles are
+// those of the first positions that stay visible and those from the window of its first query to its last query; rows of
+// V that no query of the item sees are cleared in shared memory before they meet a probability of 0, because a cache may
+// hold anything there.
+//
 // One thread owns one query row.  (Two threads per row were measured slower on B200 -- 0.418 ms against 0.353 ms on
 // the Llama-3-8B B8 S2048 prefill: the row-max exchange costs more than the extra warps hide -- and so was a variant
 // with P staged in shared memory.)
@@ -86,6 +91,11 @@ struct Attn2Params {
   float* part_ml;    // (kv_splits, B, Hq, S, 2): exponent reference and row sum of each part
   int* err;
   long long wait_limit;  // cycles a bounded wait may last (tb200_set_wait_limit_cycles)
+  // SEQ: lengths per sequence, a window with first positions that stay visible, strided q and o (in elements)
+  const int32_t* kv_lens;
+  const int32_t* q_rows;
+  int cache_len, window, sinks;
+  long long o_stride[3];
 };
 
 // One unit of work.  Items are numbered so that the longest (the last queries of a causal sequence) come first and
@@ -95,10 +105,20 @@ struct Item {
   int j_begin;   // first key tile of this share
   int nt[2];     // key tiles of each query tile within the share (0: nothing to do)
   int nt_max;
+  // SEQ: positions and new rows of the sequence; the keys some query of the item sees are those up to `last` that are not
+  // in [few, low); tile j of the item is key tile j below sink_tiles, then from win_tile on
+  int past, rows, last, few, low, sink_tiles, win_tile;
 };
 
-__device__ __forceinline__ Item decode_item(const Attn2Params& p, int i) {
+template <bool SEQ> __device__ __forceinline__ int key_tile(const Item& it, int j) {   // j: tile of the share
+  const int v = it.j_begin + j;
+  if constexpr (SEQ) return v < it.sink_tiles ? v : it.win_tile + v - it.sink_tiles;
+  return v;
+}
+
+template <bool SEQ> __device__ __forceinline__ Item decode_item(const Attn2Params& p, int i) {
   Item it;
+  it.past = it.rows = it.last = it.few = it.low = it.sink_tiles = it.win_tile = 0;
   it.nt[0] = it.nt[1] = it.nt_max = 0;
   it.q0 = it.hq = it.b = it.hkv = it.sp = it.j_begin = 0;
   if (i >= p.n_items) return it;
@@ -110,6 +130,22 @@ __device__ __forceinline__ Item decode_item(const Attn2Params& p, int i) {
   it.hq = r1 - it.b * p.Hq;
   it.hkv = fdiv(it.hq, p.d_group);
   it.q0 = (p.n_blocks - 1 - blk) * 2 * BQ;
+  if constexpr (SEQ) {
+    const int n = max(0, min(__ldg(p.kv_lens + it.b), p.cache_len));
+    it.rows = p.q_rows ? max(0, min(__ldg(p.q_rows + it.b), p.S)) : p.S;
+    it.past = n - it.rows;   // negative: the first rows stand before the first position and see nothing
+    it.low = p.window > 0 ? max(0, it.past + it.q0 - p.window + 1) : 0;
+    it.few = min(p.sinks, it.low);
+    it.win_tile = it.low / BKV;
+    it.sink_tiles = min((it.few + BKV - 1) / BKV, it.win_tile);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int q0t = it.q0 + t * BQ;
+      if (q0t >= it.rows) continue;
+      it.last = it.past + min(q0t + BQ, it.rows) - 1;
+      it.nt[t] = it.sink_tiles + max(0, it.last) / BKV + 1 - it.win_tile;   // without a visible key: one masked tile makes the zeros
+    }
+  } else
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int q0t = it.q0 + t * BQ;
@@ -127,7 +163,7 @@ __device__ __forceinline__ Item decode_item(const Attn2Params& p, int i) {
   return it;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SEQ>
 __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_constant__ Attn2Params p) {
   using L = Smem2<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -197,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
     uint32_t q_loads[2] = {0, 0};    // Q tiles loaded so far, per query tile
     bool ok = true;
     for (int i = blockIdx.x; ok && i < p.n_items; i += gridDim.x) {
-      const Item it = decode_item(p, i);
+      const Item it = decode_item<SEQ>(p, i);
       // order: Q0, K0, Q1, V0, then K1 V1 K2 V2 ...: the first S of query tile 0 needs only Q0 and K0
       for (int step = 0; ok && step < 2 * it.nt_max + 2; ++step) {
         if (step == 0 || step == 2) {
@@ -208,9 +244,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
           if (lane == 0) {
             mbar_arrive_expect_tx(&q_full[t], L::kTile);
 #pragma unroll
-            for (int dc = 0; dc < D / 64; ++dc)
-              tma_load_3d(smem + L::kQOff + t * L::kTile + dc * (BQ * 128), &p.map_q, &q_full[t], dc * 64, it.q0 + t * BQ,
-                          it.b * p.Hq + it.hq);
+            for (int dc = 0; dc < D / 64; ++dc) {
+              uint8_t* dst = smem + L::kQOff + t * L::kTile + dc * (BQ * 128);
+              if constexpr (SEQ) tma_load_4d(dst, &p.map_q, &q_full[t], dc * 64, it.q0 + t * BQ, it.hq, it.b);
+              else tma_load_3d(dst, &p.map_q, &q_full[t], dc * 64, it.q0 + t * BQ, it.b * p.Hq + it.hq);
+            }
           }
           __syncwarp();
           if (t == 0) ++q_loads[0]; else ++q_loads[1];
@@ -230,9 +268,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
           mbar_arrive_expect_tx(full, L::kTile);
           uint8_t* dst = smem + (is_v ? L::kVOff : L::kKOff) + st * L::kTile;
 #pragma unroll
-          for (int dc = 0; dc < D / 64; ++dc)
-            tma_load_3d(dst + dc * (BKV * 128), is_v ? &p.map_v : &p.map_k, full, dc * 64, (it.j_begin + j) * BKV,
-                        it.b * p.Hkv + it.hkv);
+          for (int dc = 0; dc < D / 64; ++dc) {
+            if constexpr (SEQ)
+              tma_load_4d(dst + dc * (BKV * 128), is_v ? &p.map_v : &p.map_k, full, dc * 64, key_tile<SEQ>(it, j) * BKV, it.hkv, it.b);
+            else
+              tma_load_3d(dst + dc * (BKV * 128), is_v ? &p.map_v : &p.map_k, full, dc * 64, (it.j_begin + j) * BKV,
+                          it.b * p.Hkv + it.hkv);
+          }
         }
         __syncwarp();
       }
@@ -312,13 +354,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
       return true;
     };
 
-    Item cur = decode_item(p, blockIdx.x);
+    Item cur = decode_item<SEQ>(p, blockIdx.x);
     ok = start_item(cur);
     for (int i = blockIdx.x; ok && i < p.n_items; i += gridDim.x) {
-      const Item nxt = decode_item(p, i + gridDim.x);
+      const Item nxt = decode_item<SEQ>(p, i + gridDim.x);
       if (cur.nt_max == 0) ok = start_item(nxt);
       for (int j = 0; ok && j < cur.nt_max; ++j) {
         if (!mbar_wait(&v_full[vpos & 1], (vpos >> 1) & 1, ctx, 405)) { ok = false; break; }
+        if constexpr (SEQ) {  // clear the rows of V that no query of the item sees
+          const int k0 = key_tile<SEQ>(cur, j) * BKV;
+          if (k0 + BKV - 1 > cur.last || (k0 < cur.low && k0 + BKV - 1 >= cur.few)) {
+            uint8_t* vt = smem + L::kVOff + (vpos & 1) * L::kTile;
+            for (int i = lane; i < BKV * 8; i += 32) {
+              const int key = k0 + (i >> 3);
+              if (key > cur.last || (key < cur.low && key >= cur.few)) {
+#pragma unroll
+                for (int dc = 0; dc < D / 64; ++dc) *reinterpret_cast<uint4*>(vt + dc * (BKV * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
         tc_fence_after();
         if (j + 1 < cur.nt_max) {
           // Every barrier wait and every commit costs this warp about 200 cycles, and whatever stands between the
@@ -363,18 +420,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
     bool ok = true;
 
     for (int i = blockIdx.x; ok && i < p.n_items; i += gridDim.x) {
-      int my_nt, k_first, key_limit;
+      int my_nt, k_first, key_limit, win_low = 0, sink_tiles = 0, win_skip = 0;
       {  // only what the key loop needs stays live through it; the item is decoded again for the output addresses
-        const Item it = decode_item(p, i);
+        const Item it = decode_item<SEQ>(p, i);
         my_nt = t == 0 ? it.nt[0] : it.nt[1];
         k_first = it.j_begin * BKV;
         const int qi = it.q0 + t * BQ + r_in;
         key_limit = p.causal ? min(p.past + qi, p.kv_len - 1) : p.kv_len - 1;
+        if constexpr (SEQ) {
+          k_first = it.j_begin;
+          key_limit = it.past + qi;
+          win_low = p.window > 0 ? key_limit - p.window + 1 : 0;
+          sink_tiles = it.sink_tiles;
+          win_skip = it.win_tile - it.sink_tiles;
+        }
       }
       float m_use = -INFINITY, l = 0.f;
 
       for (int j = 0; j < my_nt; ++j, ++s_count) {
-        const int k0 = k_first + j * BKV;
+        int k0 = k_first + j * BKV;
+        if constexpr (SEQ) {
+          const int v = k_first + j;
+          k0 = (v < sink_tiles ? v : v + win_skip) * BKV;
+        }
         if (!mbar_wait(&s_full[t], s_count & 1, ctx, 408)) { ok = false; break; }
         tc_fence_after();
         uint32_t s[BKV];
@@ -386,6 +454,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
 #pragma unroll
           for (int c = 0; c < BKV; ++c)
             if (k0 + c > key_limit) s[c] = 0xff800000u;  // -inf
+        }
+        if constexpr (SEQ) {
+          if (k0 < win_low && k0 + BKV - 1 >= p.sinks) {  // these touch the keys before the window
+#pragma unroll
+            for (int c = 0; c < BKV; ++c)
+              if (k0 + c < win_low && k0 + c >= p.sinks) s[c] = 0xff800000u;
+          }
         }
         float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
@@ -447,9 +522,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
 
       // ---- end of the item: hand the factor each row of O is to be multiplied with to the output warpgroup (which
       //      waits for the last P V itself) and go on to the next item at once
-      const Item it = decode_item(p, i);
+      const Item it = decode_item<SEQ>(p, i);
       const int qi = it.q0 + t * BQ + r_in;
-      const bool row_ok = qi < p.S;
+      const bool row_ok = qi < (SEQ ? it.rows : p.S);
       if (my_nt > 0) {
         if (handed > 0 && !mbar_wait(&stat_empty[t], (handed - 1) & 1, ctx, 411)) { ok = false; break; }
         stat[t * BQ + r_in] = (p.kv_splits > 1) ? 1.f : ((l > 0.f) ? 1.f / l : 0.f);
@@ -487,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
     bool store_pending = false;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < p.n_items; i += gridDim.x) {
-      const Item it = decode_item(p, i);
+      const Item it = decode_item<SEQ>(p, i);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int nt = t == 0 ? it.nt[0] : it.nt[1];
@@ -518,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
               __syncwarp();
               if (lane == 0) mbar_arrive(&o_free[t]);
             }
-            if (qi < p.S) {
+            if (qi < (SEQ ? it.rows : p.S)) {
               uint4* d = reinterpret_cast<uint4*>(p.part_o + prow * D + c * 32);
 #pragma unroll
               for (int e = 0; e < 8; ++e) d[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
@@ -552,6 +627,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
         }
         fence_proxy_async_smem();
         named_barrier_sync(1, 128);
+        if constexpr (SEQ) {
+          if (q0t + BQ <= it.rows || it.rows == p.S) {
+            if (tid == 0) {
+#pragma unroll
+              for (int dc = 0; dc < D / 64; ++dc) tma_store_4d(&p.map_o, stage + dc * (BQ * 128), dc * 64, q0t, it.hq, it.b);
+              tma_store_commit();
+            }
+          } else {  // rows behind the sequence's last one stay as they are
+            T* o = static_cast<T*>(p.o2) + it.b * p.o_stride[0] + it.hq * p.o_stride[1];
+            for (int i = tid; i < (it.rows - q0t) * (D / 8); i += 128) {
+              const int r = i / (D / 8), c = i % (D / 8);
+              *reinterpret_cast<uint4*>(o + static_cast<long long>(q0t + r) * p.o_stride[2] + c * 8) =
+                  *reinterpret_cast<const uint4*>(stage + (c >> 3) * (BQ * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            }
+          }
+        } else
         if (tid == 0) {  // rows beyond S are clipped by the tensor map
 #pragma unroll
           for (int dc = 0; dc < D / 64; ++dc) tma_store_3d(&p.map_o, stage + dc * (BQ * 128), it.hq * D + dc * 64, q0t, it.b);
@@ -572,9 +663,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
 }
 
 // Merge the shares of a key-split launch: one warp per (batch, head, query) row, lanes over the D columns.
-template <typename T, int D>
+struct CombineSeq {   // SEQ: where o goes and which rows exist
+  const int32_t* q_rows;
+  long long o_stride[3];
+};
+template <typename T, int D, bool SEQ>
 __global__ void attn_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, T* __restrict__ o2,
-                                    float* __restrict__ lse2, int splits, int B, int Hq, int S) {
+                                    float* __restrict__ lse2, int splits, int B, int Hq, int S, const CombineSeq seq) {
   constexpr int V = D / 32;
   pdl_launch_dependents();
   pdl_wait();
@@ -582,6 +677,9 @@ __global__ void attn_combine_kernel(const float* __restrict__ part_o, const floa
   const int lane = threadIdx.x & 31;
   for (long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; row < rows;
        row += (static_cast<long long>(gridDim.x) * blockDim.x) >> 5) {
+    if constexpr (SEQ) {
+      if (seq.q_rows && static_cast<int>(row % S) >= __ldg(seq.q_rows + row / (static_cast<long long>(S) * Hq))) continue;
+    }
     // all the shares' loads are in flight together (at most 16 shares): one trip to L2, not one per share
     constexpr int kMaxSplits = 16;
     float2 ml[kMaxSplits];
@@ -611,36 +709,60 @@ __global__ void attn_combine_kernel(const float* __restrict__ part_o, const floa
     const int qi = static_cast<int>(row % S);
     const int hq = static_cast<int>((row / S) % Hq);
     const int b = static_cast<int>(row / (static_cast<long long>(S) * Hq));
-    uint32_t* dst = reinterpret_cast<uint32_t*>(o2 + ((static_cast<long long>(b) * S + qi) * Hq + hq) * D + lane * V);
+    T* at = o2 + ((static_cast<long long>(b) * S + qi) * Hq + hq) * D;
+    if constexpr (SEQ) at = o2 + b * seq.o_stride[0] + hq * seq.o_stride[1] + qi * seq.o_stride[2];
+    uint32_t* dst = reinterpret_cast<uint32_t*>(at + lane * V);
 #pragma unroll
     for (int i = 0; i < V; i += 2) dst[i >> 1] = Pack2<T>::pack(acc[i] * inv_l, acc[i + 1] * inv_l);
     if (lane == 0 && lse2 != nullptr) lse2[row] = m + log2f(l);
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SEQ>
 int launch_one(const Attn2Params& p, dim3 grid, int num_sms, cudaStream_t stream) {
   static bool attr_set[32] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_set[dev & 31]) {
-    if (cudaFuncSetAttribute(attn_fwd2_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem2<D>::kTotal) != cudaSuccess)
+    if (cudaFuncSetAttribute(attn_fwd2_kernel<T, D, SEQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem2<D>::kTotal) != cudaSuccess)
       return TB200_ERR_CUDA;
     attr_set[dev & 31] = true;
   }
-  if (launch_chained(attn_fwd2_kernel<T, D>, grid, dim3(kThreads, 1, 1), Smem2<D>::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
+  if (launch_chained(attn_fwd2_kernel<T, D, SEQ>, grid, dim3(kThreads, 1, 1), Smem2<D>::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
   if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
   if (p.kv_splits > 1) {
     const long long rows = static_cast<long long>(p.B) * p.Hq * p.S;
     long long blocks = (rows * 32 + 255) / 256;
     if (blocks > num_sms * 8) blocks = num_sms * 8;
-    if (launch_chained(attn_combine_kernel<T, D>, dim3(static_cast<unsigned>(blocks), 1, 1), dim3(256, 1, 1), 0, stream, p.part_o, p.part_ml,
-                       static_cast<T*>(p.o2), p.lse2, p.kv_splits, p.B, p.Hq, p.S) != cudaSuccess)
+    CombineSeq seq;
+    seq.q_rows = p.q_rows;
+    for (int i = 0; i < 3; ++i) seq.o_stride[i] = p.o_stride[i];
+    if (launch_chained(attn_combine_kernel<T, D, SEQ>, dim3(static_cast<unsigned>(blocks), 1, 1), dim3(256, 1, 1), 0, stream, p.part_o, p.part_ml,
+                       static_cast<T*>(p.o2), p.lse2, p.kv_splits, p.B, p.Hq, p.S, seq) != cudaSuccess)
       return TB200_ERR_CUDA;
     if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
   }
   return TB200_OK;
 }
+
+// The items of a launch and the launch itself, once the tensors are described.
+template <bool SEQ>
+int finish_launch(Attn2Params& p, int dtype, int D, const DeviceState* st, cudaStream_t stream) {
+  p.n_blocks = (p.S + 2 * BQ - 1) / (2 * BQ);
+  const long long items = static_cast<long long>(p.n_blocks) * p.kv_splits * p.Hq * p.B;
+  if (items > 0x7fffffffLL) return TB200_ERR_INVALID;
+  p.n_items = static_cast<int>(items);
+  p.d_per_blk = make_fastdiv(static_cast<uint32_t>(p.B) * p.Hq * p.kv_splits);
+  p.d_splits = make_fastdiv(static_cast<uint32_t>(p.kv_splits));
+  p.d_hq = make_fastdiv(static_cast<uint32_t>(p.Hq));
+  p.d_group = make_fastdiv(static_cast<uint32_t>(p.Hq / p.Hkv));
+  const dim3 grid(static_cast<unsigned>(p.n_items < st->num_sms ? p.n_items : st->num_sms), 1, 1);  // persistent: one CTA per SM
+  if (dtype == TB200_BF16) {
+    return D == 128 ? launch_one<__nv_bfloat16, 128, SEQ>(p, grid, st->num_sms, stream) : launch_one<__nv_bfloat16, 64, SEQ>(p, grid, st->num_sms, stream);
+  }
+  return D == 128 ? launch_one<__half, 128, SEQ>(p, grid, st->num_sms, stream) : launch_one<__half, 64, SEQ>(p, grid, st->num_sms, stream);
+}
+
 
 }  // namespace
 
@@ -692,19 +814,41 @@ int launch_attn_fwd_pingpong(const AttnLaunch& a, cudaStream_t stream) {
     const uint32_t box[3] = {64, BQ, 1};
     if ((status = make_tensor_map(&p.map_o, a.o2, 3, dims, strides, box)) != TB200_OK) return status;
   }
-  p.n_blocks = (a.S + 2 * BQ - 1) / (2 * BQ);
-  const long long items = static_cast<long long>(p.n_blocks) * p.kv_splits * a.Hq * a.B;
-  if (items > 0x7fffffffLL) return TB200_ERR_INVALID;
-  p.n_items = static_cast<int>(items);
-  p.d_per_blk = make_fastdiv(static_cast<uint32_t>(a.B) * a.Hq * p.kv_splits);
-  p.d_splits = make_fastdiv(static_cast<uint32_t>(p.kv_splits));
-  p.d_hq = make_fastdiv(static_cast<uint32_t>(a.Hq));
-  p.d_group = make_fastdiv(static_cast<uint32_t>(a.Hq / a.Hkv));
-  const dim3 grid(static_cast<unsigned>(p.n_items < st->num_sms ? p.n_items : st->num_sms), 1, 1);  // persistent: one CTA per SM
-  if (a.dtype == TB200_BF16) {
-    return a.D == 128 ? launch_one<__nv_bfloat16, 128>(p, grid, st->num_sms, stream) : launch_one<__nv_bfloat16, 64>(p, grid, st->num_sms, stream);
-  }
-  return a.D == 128 ? launch_one<__half, 128>(p, grid, st->num_sms, stream) : launch_one<__half, 64>(p, grid, st->num_sms, stream);
+  return finish_launch<false>(p, a.dtype, a.D, st, stream);
+}
+
+// The same kernel over caches with per-sequence lengths; arguments are validated by the caller.
+int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
+  int status = TB200_OK;
+  DeviceState* st = device_state(&status);
+  if (!st) return status;
+  Attn2Params p;
+  memset(&p, 0, sizeof(p));
+  p.B = a.B; p.S = a.S; p.Hq = a.Hq; p.Hkv = a.Hkv; p.kv_len = a.cache_len; p.causal = 1;
+  p.cache_len = a.cache_len; p.window = a.window; p.sinks = a.sinks;
+  p.kv_lens = a.kv_lens; p.q_rows = a.q_rows;
+  p.scale_log2 = a.sm_scale * kLog2e;
+  p.o2 = a.o;
+  for (int i = 0; i < 3; ++i) p.o_stride[i] = a.o_stride[i];
+  p.kv_splits = a.kv_splits > 1 ? a.kv_splits : 1;
+  p.part_o = a.part_o;
+  p.part_ml = a.part_ml;
+  p.err = st->err_word;
+  p.wait_limit = wait_limit_cycles();
+  auto map4 = [&](CUtensorMap* map, const void* base, int rows, int heads, const int64_t (&st3)[3]) {   // strides: batch, head, row
+    const uint64_t d = static_cast<uint64_t>(a.D);
+    const uint64_t dims[4] = {d, static_cast<uint64_t>(rows), static_cast<uint64_t>(heads), static_cast<uint64_t>(a.B)};
+    const uint64_t strides[3] = {rows > 1 ? static_cast<uint64_t>(st3[2]) * 2 : d * 2, heads > 1 ? static_cast<uint64_t>(st3[1]) * 2 : d * 2,
+                                 a.B > 1 ? static_cast<uint64_t>(st3[0]) * 2 : d * 2};
+    const uint32_t box[4] = {64, BQ, 1, 1};
+    return make_tensor_map(map, base, 4, dims, strides, box);
+  };
+  static_assert(BQ == BKV, "one box size for queries and keys");
+  if ((status = map4(&p.map_q, a.q, a.S, a.Hq, a.q_stride)) != TB200_OK) return status;
+  if ((status = map4(&p.map_k, a.k_cache, a.cache_len, a.Hkv, a.k_stride)) != TB200_OK) return status;
+  if ((status = map4(&p.map_v, a.v_cache, a.cache_len, a.Hkv, a.v_stride)) != TB200_OK) return status;
+  if ((status = map4(&p.map_o, a.o, a.S, a.Hq, a.o_stride)) != TB200_OK) return status;
+  return finish_launch<true>(p, a.dtype, a.D, st, stream);
 }
 
 }  // namespace tb200

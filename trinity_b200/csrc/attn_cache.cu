@@ -657,56 +657,6 @@ __global__ void __launch_bounds__(kCombineThreads) cache_combine_kernel(const __
   }
 }
 
-// The 16-bit caches: one warp per (sequence, query head, query row), the keys one after the other.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) cache_rows_kernel(const CacheAttnParams p, const T* k16, const T* v16, long long ks0, long long ks1, long long ks2,
-                                                          long long vs0, long long vs1, long long vs2) {
-  constexpr int V = D / 32;   // columns per lane
-  const int lane = threadIdx.x & 31;
-  const long long rows = static_cast<long long>(p.B) * p.Hq * p.S;
-  for (long long w = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); w < rows; w += static_cast<long long>(gridDim.x) * 8) {
-    const int i = static_cast<int>(w % p.S);
-    const int hq = static_cast<int>((w / p.S) % p.Hq);
-    const int b = static_cast<int>(w / (static_cast<long long>(p.S) * p.Hq));
-    const int n = max(0, min(p.kv_lens[b], p.cache_len));
-    const int r = p.q_rows ? max(0, min(p.q_rows[b], p.S)) : p.S;
-    if (i >= r) continue;
-    const int hkv = hq / p.group;
-    const int at = n - r + i;
-    const int low = p.window > 0 ? max(0, at - p.window + 1) : 0;
-    const int few = min(p.sinks, low);
-    float q[V], o[V];
-    const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + hq * p.qs[1] + i * p.qs[2] + lane * V;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      q[e] = static_cast<float>(qp[e]) * p.scale_log2;
-      o[e] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int x = 0; x < few + at + 1 - low; ++x) {
-      const int j = x < few ? x : x - few + low;
-      const T* kp = k16 + b * ks0 + hkv * ks1 + j * ks2 + lane * V;
-      const T* vp = v16 + b * vs0 + hkv * vs1 + j * vs2 + lane * V;
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) s = fmaf(q[e], static_cast<float>(kp[e]), s);
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      const float m_new = fmaxf(m, s);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float a = fast_exp2(m - m_use), pr = fast_exp2(s - m_use);
-      m = m_new;
-      l = fmaf(l, a, pr);
-#pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = fmaf(o[e], a, pr * static_cast<float>(vp[e]));
-    }
-    const float inv = l > 0.f ? 1.f / l : l;
-    T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + hq * p.os[1] + i * p.os[2] + lane * V;
-#pragma unroll
-    for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(op + e) = Pack2<T>::pack(o[e] * inv, o[e + 1] * inv);
-  }
-}
-
 constexpr int kMaxExtent = 1 << 30;
 
 int check_attn(const tb200_cache_attn_args* a, bool kv4) {
@@ -736,14 +686,32 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
 // CTAs of the decode kernel that an SM holds: by shared memory (72 KB with 8 query rows, 90 KB with 16 at D = 128)
 constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
+// New rows per sequence up to which a call on a 4-bit cache runs cache_decode_kernel.
+constexpr int kDecodeTokens = 32;
+
 struct AttnPlan {
-  int nt = 1;                // MMA column blocks of a unit
+  bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
+  int nt = 1;                // decode: MMA column blocks of a unit
   int stretches = 0;
-  size_t part_o = 0, part_ml = 0;
+  int kv_splits = 1;         // prompt
+  size_t part_o = 0, part_ml = 0, cache16 = 0;   // bytes; cache16: of one of the two caches
+  size_t total() const { return part_o + part_ml + 2 * cache16; }
 };
-AttnPlan plan_attn(const tb200_cache_attn_args* a, int num_sms) {
+AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   AttnPlan pl;
   const int64_t rows = static_cast<int64_t>(a->rows) * (a->n_q_heads / a->n_kv_heads);
+  pl.prompt = !kv4 || a->rows > kDecodeTokens;
+  if (pl.prompt) {
+    const int64_t seen = a->window > 0 ? static_cast<int64_t>(a->window) + a->rows + a->sinks : a->cache_len;
+    pl.kv_splits = attn_kv_splits(a->batch, a->rows, a->n_q_heads, static_cast<int>(seen < a->cache_len ? seen : a->cache_len), num_sms);
+    if (pl.kv_splits > 1) {
+      const size_t prows = static_cast<size_t>(pl.kv_splits) * a->batch * a->n_q_heads * a->rows;
+      pl.part_o = align_up(prows * a->head_dim * sizeof(float), 256);
+      pl.part_ml = align_up(prows * 2 * sizeof(float), 256);
+    }
+    if (kv4) pl.cache16 = align_up(static_cast<size_t>(a->batch) * a->n_kv_heads * a->cache_len * a->head_dim * 2, 256);
+    return pl;
+  }
   pl.nt = rows <= 8 ? 1 : 2;
   pl.stretches = num_sms * ctas_per_sm(pl.nt);
   pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * a->head_dim * sizeof(float), 256);
@@ -797,14 +765,30 @@ int run_kv4(const CacheAttnParams& p, int head_dim, int nt, cudaStream_t stream)
   return nt == 1 ? launch_decode<T, 64, 1>(p, stream) : launch_decode<T, 64, 2>(p, stream);
 }
 
-template <typename T, int D>
-int launch_rows16(const CacheAttnParams& p, const tb200_cache_attn_args* a, int num_sms, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(p.B) * p.Hq * p.S;
-  long long blocks = (rows + 7) / 8;
-  if (blocks > num_sms * 8) blocks = num_sms * 8;
-  cache_rows_kernel<T, D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, static_cast<const T*>(a->k_cache), static_cast<const T*>(a->v_cache),
-      a->k_stride[0], a->k_stride[1], a->k_stride[2], a->v_stride[0], a->v_stride[1], a->v_stride[2]);
-  return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, const CacheAttnParams& p, int num_sms, cudaStream_t stream) {
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  AttnSeqLaunch s;
+  s.dtype = a->dtype;
+  s.B = a->batch; s.S = a->rows; s.Hq = a->n_q_heads; s.Hkv = a->n_kv_heads; s.D = a->head_dim; s.cache_len = a->cache_len;
+  s.window = p.window; s.sinks = p.sinks;
+  s.sm_scale = a->sm_scale;
+  s.q = a->q; s.o = a->o;
+  s.kv_lens = a->kv_lens; s.q_rows = a->q_rows;
+  s.kv_splits = pl.kv_splits;
+  s.part_o = reinterpret_cast<float*>(ws);
+  s.part_ml = reinterpret_cast<float*>(ws + pl.part_o);
+  s.k_cache = a->k_cache; s.v_cache = a->v_cache;
+  for (int i = 0; i < 3; ++i) { s.q_stride[i] = a->q_stride[i]; s.o_stride[i] = a->o_stride[i]; s.k_stride[i] = a->k_stride[i]; s.v_stride[i] = a->v_stride[i]; }
+  if (kv4) {
+    uint8_t* k16 = ws + pl.part_o + pl.part_ml;
+    const int status = launch_kv4_read_seen(*a, p.window, p.sinks, k16, k16 + pl.cache16, num_sms, stream);
+    if (status != TB200_OK) return status;
+    s.k_cache = k16; s.v_cache = k16 + pl.cache16;
+    s.k_stride[2] = s.v_stride[2] = a->head_dim;
+    s.k_stride[1] = s.v_stride[1] = static_cast<int64_t>(a->cache_len) * a->head_dim;
+    s.k_stride[0] = s.v_stride[0] = s.k_stride[1] * a->n_kv_heads;
+  }
+  return launch_attn_fwd_seq(s, stream);
 }
 
 int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
@@ -816,19 +800,22 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   if (a->batch == 0 || a->rows == 0) return TB200_OK;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   CacheAttnParams p = make_params(a, st);
-  if (!kv4) {
-    if (a->dtype == TB200_BF16)
-      return a->head_dim == 128 ? launch_rows16<__nv_bfloat16, 128>(p, a, st->num_sms, stream) : launch_rows16<__nv_bfloat16, 64>(p, a, st->num_sms, stream);
-    return a->head_dim == 128 ? launch_rows16<__half, 128>(p, a, st->num_sms, stream) : launch_rows16<__half, 64>(p, a, st->num_sms, stream);
-  }
-  const AttnPlan pl = plan_attn(a, st->num_sms);
-  if (!a->workspace || a->workspace_bytes < pl.part_o + pl.part_ml) return TB200_ERR_WORKSPACE;
+  const AttnPlan pl = plan_attn(a, kv4, st->num_sms);
+  if (pl.total() > 0 && (!a->workspace || a->workspace_bytes < pl.total())) return TB200_ERR_WORKSPACE;
   if (!aligned16(a->workspace)) return TB200_ERR_INVALID;
+  ChainScope chain;
+  if (pl.prompt) return run_prompt(a, kv4, pl, p, st->num_sms, stream);
   p.stretches = pl.stretches;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
-  ChainScope chain;
   return a->dtype == TB200_BF16 ? run_kv4<__nv_bfloat16>(p, a->head_dim, pl.nt, stream) : run_kv4<__half>(p, a->head_dim, pl.nt, stream);
+}
+
+size_t workspace_bytes(const tb200_cache_attn_args* a, bool kv4) {
+  int status = TB200_OK;
+  DeviceState* st = device_state(&status);
+  if (!st || check_attn(a, kv4) != TB200_OK || a->batch == 0 || a->rows == 0) return 0;
+  return plan_attn(a, kv4, st->num_sms).total();
 }
 
 }  // namespace
@@ -840,14 +827,8 @@ extern "C" {
 
 int tb200_attn_window_check(const tb200_cache_attn_args* a) { return check_attn(a, false); }
 int tb200_kv4_attn_check(const tb200_cache_attn_args* a) { return check_attn(a, true); }
-size_t tb200_attn_window_workspace_bytes(const tb200_cache_attn_args*) { return 0; }
-size_t tb200_kv4_attn_workspace_bytes(const tb200_cache_attn_args* a) {
-  int status = TB200_OK;
-  DeviceState* st = device_state(&status);
-  if (!st || check_attn(a, true) != TB200_OK) return 0;
-  const AttnPlan pl = plan_attn(a, st->num_sms);
-  return pl.part_o + pl.part_ml;
-}
+size_t tb200_attn_window_workspace_bytes(const tb200_cache_attn_args* a) { return workspace_bytes(a, false); }
+size_t tb200_kv4_attn_workspace_bytes(const tb200_cache_attn_args* a) { return workspace_bytes(a, true); }
 int tb200_attn_window(const tb200_cache_attn_args* a, void* stream) { return run_attn(a, false, stream); }
 int tb200_kv4_attn(const tb200_cache_attn_args* a, void* stream) { return run_attn(a, true, stream); }
 

@@ -182,6 +182,24 @@ int launch_attn_fwd(const AttnLaunch& a, cudaStream_t stream);
 // attn2.cu: two query tiles per CTA; chosen by launch_attn_fwd when there is no noise tensor
 int launch_attn_fwd_pingpong(const AttnLaunch& a, cudaStream_t stream);
 int attn_kv_splits(int B, int S, int Hq, int kv_len, int num_sms);
+// attn2.cu over caches with per-sequence lengths, an optional window with first positions that stay visible (window 0:
+// none), and q, caches and o addressed by element strides of their (batch, head, row) axes
+struct AttnSeqLaunch {
+  int dtype = TB200_BF16;
+  int B = 0, S = 0, Hq = 0, Hkv = 0, D = 0, cache_len = 0, window = 0, sinks = 0;
+  float sm_scale = 1.f;
+  const void* q = nullptr;
+  const void* k_cache = nullptr;
+  const void* v_cache = nullptr;
+  void* o = nullptr;
+  int64_t q_stride[3] = {}, k_stride[3] = {}, v_stride[3] = {}, o_stride[3] = {};
+  const int32_t* kv_lens = nullptr;
+  const int32_t* q_rows = nullptr;
+  int kv_splits = 1;
+  float* part_o = nullptr;          // (kv_splits,B,Hq,S,D) fp32
+  float* part_ml = nullptr;         // (kv_splits,B,Hq,S,2) fp32
+};
+int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream);
 // attn_kf.cu: the same kernel with the KeyFormer statistic (noise tiles by TMA; kv_len a multiple of 8)
 int launch_attn_fwd_keyformer(const AttnLaunch& a, cudaStream_t stream);
 
@@ -240,6 +258,8 @@ int launch_kv_compact(const tb200_kv_compact_args& a, cudaStream_t stream);
 // Element strides of the (batch, head, row) axes with extents ext: steps of 16 bytes, and with `written` rows that do
 // not overlap.  Axes of one element are not looked at.
 int check_strides(const int64_t (&stride)[3], const int64_t (&ext)[3], int head_dim, bool written);
-int launch_kv4_rows(const tb200_kv4_rows_args& a, bool append, int num_sms, cudaStream_t stream);
+// The positions of a 4-bit cache that some query row of its sequence sees, as contiguous 16-bit caches
+// (B, Hkv, cache_len, D); the other positions of k16 and v16 are left as they are.
+int launch_kv4_read_seen(const tb200_cache_attn_args& a, int window, int sinks, void* k16, void* v16, int num_sms, cudaStream_t stream);
 
 }  // namespace tb200

@@ -14,6 +14,7 @@ namespace tb200 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kPerThread = 4;   // rows of a reading thread: eight loads in flight
 
 struct RowsParams {
   const int32_t* start;
@@ -24,6 +25,8 @@ struct RowsParams {
   long long stride[2][3];   // elements: batch, head, row
   uint8_t* codes[2];
   uint8_t* meta[2];
+  const int32_t* q_rows;    // SEEN
+  int q_rows_max, window, sinks;
 };
 
 template <typename T> struct Bits;   // a 16-bit value and its raw bits
@@ -100,32 +103,54 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const RowsParams p
   }
 }
 
-template <typename T, int D>
+// SEEN: only the positions that some query row of the sequence sees (a prompt's attention reads the 16-bit rows next).
+template <typename T, int D, bool SEEN>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const RowsParams p) {
   constexpr int kLanes = D / 8;
-  constexpr int kRows = kThreads / kLanes;
+  constexpr int kRows = kThreads / kLanes;   // rows side by side
+  if constexpr (SEEN) pdl_launch_dependents();
   const int tid = threadIdx.x;
   const int r_in = tid / kLanes, c8 = tid % kLanes;
   for (long long u = blockIdx.x; u < p.units; u += gridDim.x) {
     const long long bh = u / p.row_blocks;
     const int rb = static_cast<int>(u - bh * p.row_blocks);
     const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<long long>(b) * p.heads);
-    const int row = rb * kRows + r_in;
     const int n = p.n_rows ? min(p.n_rows[b], p.rows) : p.rows;
-    const long long pos = static_cast<long long>(p.start ? p.start[b] : p.start_all) + row;
-    if (row >= n || pos < 0 || pos >= p.cache_len) continue;
-    const long long crow = bh * p.cache_len + pos;
+    const int start = p.start ? p.start[b] : p.start_all;
+    int low = 0, few = 0;
+    if constexpr (SEEN) {
+      const int r = p.q_rows ? max(0, min(p.q_rows[b], p.q_rows_max)) : p.q_rows_max;
+      low = p.window > 0 ? n - r - p.window + 1 : 0;
+      few = r > 0 ? p.sinks : 0;
+      if (r == 0) low = n;
+    }
+    uint32_t word[2][kPerThread], m[2][kPerThread];
+    bool live[kPerThread];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(p.codes[which] + crow * (D / 2) + c8 * 4);
-      const uint32_t m = *reinterpret_cast<const uint32_t*>(p.meta[which] + (crow * (D / 64) + c8 / 8) * 4);
-      *reinterpret_cast<uint4*>(p.x[which] + 2 * (b * p.stride[which][0] + h * p.stride[which][1] + row * p.stride[which][2] + c8 * 8)) =
-          Kv4Decode<T>::decode8(word, m);
+    for (int k = 0; k < kPerThread; ++k) {
+      const int row = (rb * kPerThread + k) * kRows + r_in;
+      const long long pos = static_cast<long long>(start) + row;
+      live[k] = row < n && pos >= 0 && pos < p.cache_len;
+      if constexpr (SEEN) live[k] = live[k] && (row >= low || row < few);
+      const long long crow = bh * p.cache_len + pos;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        word[w][k] = live[k] ? __ldg(reinterpret_cast<const uint32_t*>(p.codes[w] + crow * (D / 2) + c8 * 4)) : 0u;
+        m[w][k] = live[k] ? __ldg(reinterpret_cast<const uint32_t*>(p.meta[w] + (crow * (D / 64) + c8 / 8) * 4)) : 0u;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kPerThread; ++k) {
+      if (!live[k]) continue;
+      const long long row = (rb * kPerThread + k) * kRows + r_in;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        *reinterpret_cast<uint4*>(p.x[w] + 2 * (b * p.stride[w][0] + h * p.stride[w][1] + row * p.stride[w][2] + c8 * 8)) =
+            Kv4Decode<T>::decode8(word[w][k], m[w][k]);
     }
   }
 }
 
-// Strides of (batch, head, row) in elements: whole 16-byte steps, and rows that do not overlap where they are written.
 }  // namespace
 
 int check_strides(const int64_t (&st)[3], const int64_t (&ext)[3], int head_dim, bool written) {
@@ -164,14 +189,13 @@ int check_rows(const tb200_kv4_rows_args* a) {
   return TB200_OK;
 }
 
-template <typename T, int D>
-int launch_rows(const tb200_kv4_rows_args& a, bool append, int num_sms, cudaStream_t stream) {
+enum RowsWork { kAppend, kRead, kReadSeen };
+
+RowsParams rows_params(const tb200_kv4_rows_args& a) {
   RowsParams p;
+  memset(&p, 0, sizeof(p));
   p.start = a.start; p.n_rows = a.n_rows; p.start_all = a.start_all;
   p.rows = a.rows; p.heads = a.n_kv_heads; p.cache_len = a.cache_len;
-  constexpr int kRows = kThreads / (D / 8);
-  p.row_blocks = (a.rows + kRows - 1) / kRows;
-  p.units = static_cast<long long>(a.batch) * a.n_kv_heads * p.row_blocks;
   p.x[0] = static_cast<uint8_t*>(a.k);
   p.x[1] = static_cast<uint8_t*>(a.v);
   for (int i = 0; i < 3; ++i) { p.stride[0][i] = a.k_stride[i]; p.stride[1][i] = a.v_stride[i]; }
@@ -179,20 +203,49 @@ int launch_rows(const tb200_kv4_rows_args& a, bool append, int num_sms, cudaStre
   p.codes[1] = static_cast<uint8_t*>(a.v_codes);
   p.meta[0] = static_cast<uint8_t*>(a.k_meta);
   p.meta[1] = static_cast<uint8_t*>(a.v_meta);
+  return p;
+}
+
+template <typename T, int D>
+int launch_rows(RowsParams p, int batch, RowsWork work, int num_sms, cudaStream_t stream) {
+  const int unit_rows = kThreads / (D / 8) * (work == kAppend ? 1 : kPerThread);
+  p.row_blocks = (p.rows + unit_rows - 1) / unit_rows;
+  p.units = static_cast<long long>(batch) * p.heads * p.row_blocks;
   const long long most = static_cast<long long>(num_sms) * 8;
-  const unsigned grid = static_cast<unsigned>(p.units < most ? p.units : most);
-  if (append) kv4_append_kernel<T, D><<<grid, kThreads, 0, stream>>>(p);
-  else kv4_read_kernel<T, D><<<grid, kThreads, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+  const dim3 grid(static_cast<unsigned>(p.units < most ? p.units : most));
+  cudaError_t e;
+  if (work == kAppend) e = launch_chained(kv4_append_kernel<T, D>, grid, dim3(kThreads), 0, stream, p);
+  else if (work == kRead) e = launch_chained(kv4_read_kernel<T, D, false>, grid, dim3(kThreads), 0, stream, p);
+  else e = launch_chained(kv4_read_kernel<T, D, true>, grid, dim3(kThreads), 0, stream, p);
+  return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+}
+
+int launch_rows(const RowsParams& p, int dtype, int head_dim, int batch, RowsWork work, int num_sms, cudaStream_t stream) {
+  if (batch == 0 || p.rows == 0 || p.cache_len == 0) return TB200_OK;
+  if (dtype == TB200_BF16)
+    return head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(p, batch, work, num_sms, stream) : launch_rows<__nv_bfloat16, 64>(p, batch, work, num_sms, stream);
+  return head_dim == 128 ? launch_rows<__half, 128>(p, batch, work, num_sms, stream) : launch_rows<__half, 64>(p, batch, work, num_sms, stream);
 }
 
 }  // namespace
 
-int launch_kv4_rows(const tb200_kv4_rows_args& a, bool append, int num_sms, cudaStream_t stream) {
-  if (a.batch == 0 || a.rows == 0 || a.cache_len == 0) return TB200_OK;
-  if (a.dtype == TB200_BF16)
-    return a.head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(a, append, num_sms, stream) : launch_rows<__nv_bfloat16, 64>(a, append, num_sms, stream);
-  return a.head_dim == 128 ? launch_rows<__half, 128>(a, append, num_sms, stream) : launch_rows<__half, 64>(a, append, num_sms, stream);
+int launch_kv4_read_seen(const tb200_cache_attn_args& a, int window, int sinks, void* k16, void* v16, int num_sms, cudaStream_t stream) {
+  RowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.n_rows = a.kv_lens; p.rows = a.cache_len; p.heads = a.n_kv_heads; p.cache_len = a.cache_len;
+  p.x[0] = static_cast<uint8_t*>(k16);
+  p.x[1] = static_cast<uint8_t*>(v16);
+  for (int w = 0; w < 2; ++w) {
+    p.stride[w][2] = a.head_dim;
+    p.stride[w][1] = static_cast<long long>(a.cache_len) * a.head_dim;
+    p.stride[w][0] = p.stride[w][1] * a.n_kv_heads;
+  }
+  p.codes[0] = static_cast<uint8_t*>(const_cast<void*>(a.k_codes));
+  p.codes[1] = static_cast<uint8_t*>(const_cast<void*>(a.v_codes));
+  p.meta[0] = static_cast<uint8_t*>(const_cast<void*>(a.k_meta));
+  p.meta[1] = static_cast<uint8_t*>(const_cast<void*>(a.v_meta));
+  p.q_rows = a.q_rows; p.q_rows_max = a.rows; p.window = window; p.sinks = sinks;
+  return launch_rows(p, a.dtype, a.head_dim, a.batch, kReadSeen, num_sms, stream);
 }
 
 }  // namespace tb200
@@ -207,7 +260,7 @@ extern "C" int tb200_kv4_append(const tb200_kv4_rows_args* a, void* stream) {
   int status = TB200_OK;
   DeviceState* st = device_state(&status);
   if (!st) return status;
-  return launch_kv4_rows(*a, true, st->num_sms, static_cast<cudaStream_t>(stream));
+  return launch_rows(rows_params(*a), a->dtype, a->head_dim, a->batch, kAppend, st->num_sms, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tb200_kv4_read(const tb200_kv4_rows_args* a, void* stream) {
@@ -219,5 +272,5 @@ extern "C" int tb200_kv4_read(const tb200_kv4_rows_args* a, void* stream) {
   int status = TB200_OK;
   DeviceState* st = device_state(&status);
   if (!st) return status;
-  return launch_kv4_rows(*a, false, st->num_sms, static_cast<cudaStream_t>(stream));
+  return launch_rows(rows_params(*a), a->dtype, a->head_dim, a->batch, kRead, st->num_sms, static_cast<cudaStream_t>(stream));
 }
