@@ -14,7 +14,7 @@ namespace tb200 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 4;   // rows of a reading thread: eight loads in flight
+constexpr int kPerThread = 4;   // rows of a thread: eight loads in flight
 
 struct RowsParams {
   const int32_t* start;
@@ -39,65 +39,111 @@ template <> struct Bits<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t rn(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 };
 
-// Codes of eight values of a group (x - lo and s exact in 64 bits where a quotient lies next to a border).
+// Two 16-bit values at once: minimum (a NaN wins), and their sign flipped.
+template <typename T> __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t min2_nan<__half>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t min2_nan<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Below this scale its rounding to the type is so coarse that a quotient may pass 15.5.
+template <typename T> struct SmallScale;
+template <> struct SmallScale<__half> { static constexpr float value = 1.9073486328125e-06f; };        // 2^-19: steps of 2^-24
+template <> struct SmallScale<__nv_bfloat16> { static constexpr float value = 1.17549435e-38f; };      // 2^-126
+
+// Codes of eight values of a group.  The quotient is formed in fp32 with an approximate reciprocal (off by less than 1e-5)
+// and rounded by adding 1.5 * 2^23, which leaves the code in the sum's low bits; where one of the eight quotients lies
+// within 1e-4 of a border between two codes, all are formed again in 64 bits.
 template <typename T>
-__device__ __forceinline__ uint32_t encode8(const uint4& raw, float lo, float s) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+__device__ __forceinline__ uint32_t encode8(const uint32_t (&w)[4], float lo, float s) {
+  constexpr float kMagic = 12582912.f;
+  const float inv = __fdividef(1.f, s);
+  const float2 nlo = make_float2(-lo, -lo), inv2 = make_float2(inv, inv), magic = make_float2(kMagic, kMagic), nmagic = make_float2(-kMagic, -kMagic);
   uint32_t word = 0;
+  float worst = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = Bits<T>::f((w[i >> 1] >> ((i & 1) * 16)) & 0xffffu);
-    float c = 0.f;
-    if (s > 0.f) c = static_cast<float>(fmin(fmax(rint((static_cast<double>(x) - static_cast<double>(lo)) / static_cast<double>(s)), 0.0), 15.0));
-    word |= static_cast<uint32_t>(c) << (4 * i);
+  for (int i = 3; i >= 0; --i) {
+    const float2 q = __fmul2_rn(__fadd2_rn(Pack2<T>::unpack(w[i]), nlo), inv2);
+    const float2 r = __fadd2_rn(q, magic);
+    const float2 d = __fadd2_rn(__fadd2_rn(r, nmagic), make_float2(-q.x, -q.y));
+    worst = fmaxf(worst, fmaxf(fabsf(d.x), fabsf(d.y)));
+    word = word * 16 + __float_as_uint(r.y);
+    word = word * 16 + __float_as_uint(r.x);
+  }
+  // every sum carries the bits of 1.5 * 2^23 along: taken out once for all eight
+  constexpr uint32_t kBits = 0x4b400000u;
+  constexpr uint32_t kCarry = kBits * 0x11111111u;
+  word -= kCarry;
+  if (!(worst < 0.4999f) || !(s >= SmallScale<T>::value)) {
+    word = 0;
+    if (s > 0.f) {
+#pragma unroll 1
+      for (int i = 7; i >= 0; --i) {
+        const float2 x2 = Pack2<T>::unpack(i < 2 ? w[0] : i < 4 ? w[1] : i < 6 ? w[2] : w[3]);
+        const double x = (i & 1) ? x2.y : x2.x;
+        const double q = (x - static_cast<double>(lo)) / static_cast<double>(s);
+        word = word * 16 + static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0));
+      }
+    }
   }
   return word;
 }
 
+// A unit is kPerThread * kThreads / (D / 8) rows of one (sequence, head), k and v.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv4_append_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kThreads) kv4_append_kernel(const __grid_constant__ RowsParams p) {
   constexpr int kLanes = D / 8;                 // lanes per row
-  constexpr int kRows = kThreads / kLanes;      // rows of a unit
+  constexpr int kRows = kThreads / kLanes;      // rows side by side
   const int tid = threadIdx.x;
   const int r_in = tid / kLanes, c8 = tid % kLanes;
   for (long long u = blockIdx.x; u < p.units; u += gridDim.x) {
     const long long bh = u / p.row_blocks;
     const int rb = static_cast<int>(u - bh * p.row_blocks);
     const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<long long>(b) * p.heads);
-    const int row = rb * kRows + r_in;
     const int n = p.n_rows ? min(p.n_rows[b], p.rows) : p.rows;
-    const long long pos = static_cast<long long>(p.start ? p.start[b] : p.start_all) + row;
-    const bool live = row < n && pos >= 0 && pos < p.cache_len;
+    const int start = p.start ? p.start[b] : p.start_all;
+    if (rb * kPerThread * kRows >= n) continue;   // the whole CTA
+    uint4 raw[kPerThread][2];
+    bool live[kPerThread];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-      if (live)
-        raw = *reinterpret_cast<const uint4*>(p.x[which] + 2 * (b * p.stride[which][0] + h * p.stride[which][1] + row * p.stride[which][2] + c8 * 8));
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-      float lo = INFINITY, hi = -INFINITY;
-      bool odd = false;   // an infinity or a NaN
+    for (int k = 0; k < kPerThread; ++k) {
+      const int row = (rb * kPerThread + k) * kRows + r_in;
+      const long long pos = static_cast<long long>(start) + row;
+      live[k] = row < n && pos >= 0 && pos < p.cache_len;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = Bits<T>::f((w[i >> 1] >> ((i & 1) * 16)) & 0xffffu);
-        odd |= !(fabsf(x) < INFINITY);
-        lo = fminf(lo, x);
-        hi = fmaxf(hi, x);
+      for (int x = 0; x < 2; ++x) {
+        raw[k][x] = make_uint4(0u, 0u, 0u, 0u);
+        if (live[k])
+          raw[k][x] = __ldcs(reinterpret_cast<const uint4*>(p.x[x] + 2 * (b * p.stride[x][0] + h * p.stride[x][1] + row * p.stride[x][2] + c8 * 8)));
       }
+    }
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        odd |= __shfl_xor_sync(0xffffffffu, static_cast<int>(odd), o) != 0;
-      }
-      const float range = __fsub_rn(hi, lo);
-      odd |= !(range < INFINITY);
-      const uint32_t sb = odd ? 0x7fffu : Bits<T>::rn(__fdiv_rn(range, 15.f));
-      const uint32_t lb = odd ? 0x7fffu : Bits<T>::rn(lo);
-      if (live) {
-        const long long crow = bh * p.cache_len + pos;
-        const uint32_t word = encode8<T>(raw, lo, odd ? 0.f : Bits<T>::f(sb));
-        *reinterpret_cast<uint32_t*>(p.codes[which] + crow * (D / 2) + c8 * 4) = word;
-        if ((c8 & 7) == 0) *reinterpret_cast<uint32_t*>(p.meta[which] + (crow * (D / 64) + c8 / 8) * 4) = sb | (lb << 16);
+    for (int k = 0; k < kPerThread; ++k) {
+      const long long crow = bh * p.cache_len + start + (rb * kPerThread + k) * kRows + r_in;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t w[4] = {raw[k][x].x, raw[k][x].y, raw[k][x].z, raw[k][x].w};
+        // minimum, and minus the maximum as the minimum of the negated values, side by side in one register
+        uint32_t lo2 = min2_nan<T>(min2_nan<T>(w[0], w[1]), min2_nan<T>(w[2], w[3]));
+        uint32_t hi2 = min2_nan<T>(min2_nan<T>(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u), min2_nan<T>(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
+        uint32_t both = min2_nan<T>(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, o));
+        const float2 f = Pack2<T>::unpack(both);
+        const float lo = f.x, range = __fsub_rn(-f.y, f.x);
+        const bool odd = !(range < INFINITY);    // an infinity or a NaN among the 64, or a range past fp32
+        const uint32_t sb = odd ? 0x7fffu : Bits<T>::rn(__fdiv_rn(range, 15.f));
+        const uint32_t lb = odd ? 0x7fffu : (both & 0xffffu);
+        const uint32_t word = encode8<T>(w, lo, odd ? 0.f : Bits<T>::f(sb));
+        if (live[k]) {
+          *reinterpret_cast<uint32_t*>(p.codes[x] + crow * (D / 2) + c8 * 4) = word;
+          if ((c8 & 7) == 0) *reinterpret_cast<uint32_t*>(p.meta[x] + (crow * (D / 64) + c8 / 8) * 4) = sb | (lb << 16);
+        }
       }
     }
   }
@@ -105,7 +151,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const RowsParams p
 
 // SEEN: only the positions that some query row of the sequence sees (a prompt's attention reads the 16-bit rows next).
 template <typename T, int D, bool SEEN>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constant__ RowsParams p) {
   constexpr int kLanes = D / 8;
   constexpr int kRows = kThreads / kLanes;   // rows side by side
   if constexpr (SEEN) pdl_launch_dependents();
@@ -208,7 +254,7 @@ RowsParams rows_params(const tb200_kv4_rows_args& a) {
 
 template <typename T, int D>
 int launch_rows(RowsParams p, int batch, RowsWork work, int num_sms, cudaStream_t stream) {
-  const int unit_rows = kThreads / (D / 8) * (work == kAppend ? 1 : kPerThread);
+  const int unit_rows = kThreads / (D / 8) * kPerThread;
   p.row_blocks = (p.rows + unit_rows - 1) / unit_rows;
   p.units = static_cast<long long>(batch) * p.heads * p.row_blocks;
   const long long most = static_cast<long long>(num_sms) * 8;

@@ -7,6 +7,7 @@ been cached, so they can be captured in a CUDA graph after one warm-up call.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Dict, NamedTuple, Optional, Union
 
 import torch
@@ -37,6 +38,11 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _raw_stream(index: int) -> int:
+    """The current stream of device `index`, without a Stream object (which costs about 3 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 class Workspace:
     """Scratch buffers the operators hand to the C ABI, one per (device, tag, stream).
 
@@ -58,7 +64,7 @@ class Workspace:
         if nbytes == 0:
             return None
         index = device.index if device.index is not None else torch.cuda.current_device()
-        key = (index, tag, torch.cuda.current_stream(device).cuda_stream)
+        key = (index, tag, _raw_stream(index))
         buf = cls._bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             if torch.cuda.is_current_stream_capturing():
@@ -321,54 +327,94 @@ def kv4_cache(batch: int, kv_heads: int, cache_len: int, head_dim: int, dtype: t
     return Kv4Cache(*codes, *meta)
 
 
-def _rows4(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device):
-    """Pointer and element strides (batch, head, row) of a ``(B, heads, rows, D)`` tensor whose last axis is contiguous."""
+# The argument blocks, packed in one call: a ctypes structure filled field by field costs more than the launch of a small kernel.
+_KV4_ROWS = struct.Struct("@8i2P2P3q3q4P")
+_CACHE_ATTN = struct.Struct("@9if2P3q3q2P2P3q3q4PPN")
+
+
+def _pack(layout: struct.Struct, *fields) -> bytes:
+    try:
+        return layout.pack(*fields)
+    except struct.error as e:
+        raise ValueError(f"an argument is no whole number or out of range: {e}") from None
+
+
+def _refuse_rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int):
     if not t.is_cuda:
         raise ValueError("trinity_b200 operators take CUDA tensors (there is no CPU path)")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the call's first tensor on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the call's first tensor on cuda:{index}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"the last axis of {name} must be contiguous")
-    return t.data_ptr(), (C.c_int64 * 3)(*t.stride()[:3])
+    raise ValueError(f"the last axis of {name} must be contiguous")
 
 
-def _ints(t: Optional[torch.Tensor], name: str, batch: int, device: torch.device) -> Optional[int]:
+def _rows4(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int):
+    """Strides of a ``(B, heads, rows, D)`` tensor whose last axis is contiguous, in elements."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or t.stride(3) != 1:
+        _refuse_rows(t, name, shape, dtype, index)
+    return t.stride()
+
+
+def _ints(t: Optional[torch.Tensor], name: str, batch: int, index: int) -> int:
     if t is None:
-        return None
-    if t.dtype != torch.int32 or tuple(t.shape) != (batch,):
+        return 0
+    if t.dtype is not torch.int32 or t.shape != (batch,):
         raise TypeError(f"{name} must be int32 of shape ({batch},)")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the call's first tensor on {device}")
-    return _ptr(t)
+    if t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor on cuda:{index}")
+    return t.data_ptr()
 
 
-def _kv4_parts(cache: Kv4Cache, device: torch.device):
-    """(batch, kv heads, cache length, head_dim, type) of a 4-bit cache and its pointers."""
-    b, h, length, half = cache.k_codes.shape
-    d, dt = 2 * half, cache.k_meta.dtype
-    for name in ("k_codes", "v_codes", "k_meta", "v_meta"):
-        t = getattr(cache, name)
-        shape, want = ((b, h, length, half), torch.uint8) if name.endswith("codes") else ((b, h, length, d // 64, 2), dt)
-        if tuple(t.shape) != shape or t.dtype != want:
-            raise ValueError(f"{name} must be {want} of shape {shape}, not {t.dtype} of shape {tuple(t.shape)}")
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the call's first tensor on {device}")
-    return (b, h, length, d, dt), {n: _ptr(getattr(cache, n)) for n in Kv4Cache._fields}
+def _kv4_parts(cache: Kv4Cache, index: int):
+    """(batch, kv heads, cache length, head_dim, type) of a 4-bit cache."""
+    kc, vc, km, vm = cache
+    shape = kc.shape
+    if len(shape) != 4:
+        raise ValueError(f"k_codes must have shape (B, Hkv, L, D / 2), not {tuple(shape)}")
+    b, h, length, half = shape
+    meta, dt = (b, h, length, half // 32, 2), km.dtype
+    if (kc.dtype is not torch.uint8 or vc.dtype is not torch.uint8 or vm.dtype is not dt or vc.shape != shape or km.shape != meta or vm.shape != meta
+            or half % 32):
+        raise ValueError(f"codes must be uint8 (B, Hkv, L, D / 2), meta 16-bit (B, Hkv, L, D / 64, 2), alike for k and v; not "
+                         + ", ".join(f"{t.dtype} {tuple(t.shape)}" for t in cache))
+    for t in cache:
+        if t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"the parts of a 4-bit cache must be contiguous tensors on cuda:{index}")
+    return b, h, length, 2 * half, dt
 
 
-def _kv4_rows_args(cache: Kv4Cache, k, v, start, rows, device):
-    (b, h, length, d, dt), ptrs = _kv4_parts(cache, device)
-    count = int(k.shape[2]) if k.dim() == 4 else -1
-    kp, ks = _rows4(k, "k", (b, h, count, d), dt, device)
-    vp, vs = _rows4(v, "v", (b, h, count, d), dt, device)
+def _device_index(t: torch.Tensor) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("trinity_b200 operators take CUDA tensors (there is no CPU path)")
+    return index
+
+
+def _on_device(index: int, call, *args):
+    """call(*args) with device `index` the current one."""
+    if index == torch.cuda.current_device():
+        return call(*args)
+    with torch.cuda.device(index):
+        return call(*args)
+
+
+def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int) -> None:
+    b, h, length, d, dt = _kv4_parts(cache, index)
+    count = k.shape[2] if k.dim() == 4 else -1
+    shape = (b, h, count, d)
+    ks, vs = _rows4(k, "k", shape, dt, index), _rows4(v, "v", shape, dt, index)
     one = isinstance(start, int)
-    return L.Kv4RowsArgs(dtype=_dt(k), batch=b, n_kv_heads=h, rows=count, head_dim=d, cache_len=length, start_all=start if one else 0,
-                         start=None if one else _ints(start, "start", b, device), n_rows=_ints(rows, "rows", b, device),
-                         k=kp, v=vp, k_stride=ks, v_stride=vs, **ptrs)
+    kc, vc, km, vm = cache
+    args = L.Kv4RowsArgs.from_buffer_copy(_pack(
+        _KV4_ROWS,
+        _dt(k), b, h, count, d, length, start if one else 0, 0, 0 if one else _ints(start, "start", b, index), _ints(rows, "rows", b, index),
+        k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr()))
+    status = getattr(L.load(), name)(C.byref(args), _raw_stream(index))
+    if status:
+        L.check(status, name)
 
 
 def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor], rows: Optional[torch.Tensor] = None) -> None:
@@ -378,58 +424,53 @@ def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: Union[i
     ``(x @ wk).view(B, S, Hkv, D).transpose(1, 2)``, needs no copy.  ``start``: an int for all sequences or int32 ``(B,)``;
     ``rows`` int32 ``(B,)``: how many of the ``S`` rows of each sequence are meant (default all).  Other rows, and rows
     whose position lies outside the cache, are not written."""
-    with torch.cuda.device(_cuda_device(k)):
-        args = _kv4_rows_args(cache, k, v, start, rows, k.device)
-        L.check(L.load().tb200_kv4_append(C.byref(args), _stream()), "tb200_kv4_append")
+    index = _device_index(k)
+    _on_device(index, _kv4_rows, "tb200_kv4_append", cache, k, v, start, rows, index)
 
 
 def kv4_read(cache: Kv4Cache, start: Union[int, torch.Tensor], count: int, rows: Optional[torch.Tensor] = None,
              k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
     """Rows ``[start[b], start[b] + count)`` of a 4-bit cache as 16-bit rows ``(B, Hkv, count, D)``: ``lo + c * s`` rounded
-    once (at most the type's largest number).  ``rows`` int32 ``(B,)`` limits how many are read of each sequence; the others, and positions outside the cache,
-    are left as they are in ``k_out, v_out`` (zero when these are not given).  Returns ``(k_out, v_out)``."""
-    dev = _cuda_device(cache.k_codes)
-    with torch.cuda.device(dev):
+    once (at most the type's largest number).  ``rows`` int32 ``(B,)`` limits how many are read of each sequence; the
+    others, and positions outside the cache, are left as they are in ``k_out, v_out`` (zero when these are not given).
+    Returns ``(k_out, v_out)``."""
+    index = _device_index(cache.k_codes)
+    if k_out is None or v_out is None:
         b, h, _, half = cache.k_codes.shape
-        make = lambda: torch.zeros(b, h, count, 2 * half, dtype=cache.k_meta.dtype, device=dev)
+        make = lambda: torch.zeros(b, h, count, 2 * half, dtype=cache.k_meta.dtype, device=cache.k_codes.device)
         k_out = make() if k_out is None else k_out
         v_out = make() if v_out is None else v_out
-        if k_out.dim() != 4 or k_out.shape[2] != count:
-            raise ValueError(f"k_out must have shape {(b, h, count, 2 * half)}, not {tuple(k_out.shape)}")
-        args = _kv4_rows_args(cache, k_out, v_out, start, rows, dev)
-        L.check(L.load().tb200_kv4_read(C.byref(args), _stream()), "tb200_kv4_read")
+    if k_out.dim() != 4 or k_out.shape[2] != count:
+        raise ValueError(f"k_out must have shape (B, Hkv, {count}, D), not {tuple(k_out.shape)}")
+    _on_device(index, _kv4_rows, "tb200_kv4_read", cache, k_out, v_out, start, rows, index)
     return k_out, v_out
 
 
-def _cuda_device(t: torch.Tensor) -> torch.device:
-    if not t.is_cuda:
-        raise ValueError("trinity_b200 operators take CUDA tensors (there is no CPU path)")
-    return t.device
-
-
-def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, **cache):
+def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index: int):
     lib = L.load()
     b, h, length, d, dt = dims
-    dev = q.device
     if q.dim() != 4:
         raise ValueError(f"q must have shape (B, Hq, S, D), not {tuple(q.shape)}")
-    hq, s = int(q.shape[1]), int(q.shape[2])
     if kv_lens is None:
         raise TypeError("kv_lens must be an int32 tensor")
+    hq, s = q.shape[1], q.shape[2]
     if out is None:
-        out = torch.empty(b, s, hq, d, dtype=dt, device=dev).transpose(1, 2)
+        out = torch.empty(b, s, hq, d, dtype=dt, device=q.device).transpose(1, 2)
         if q_rows is not None:
             out.zero_()
-    qp, qs = _rows4(q, "q", (b, hq, s, d), dt, dev)
-    op, os_ = _rows4(out, "out", (b, hq, s, d), dt, dev)
-    args = L.CacheAttnArgs(dtype=_dt(q), batch=b, rows=s, n_q_heads=hq, n_kv_heads=h, head_dim=d, cache_len=length, window=window, sinks=sinks,
-                           sm_scale=sm_scale, q=qp, o=op, q_stride=qs, o_stride=os_, kv_lens=_ints(kv_lens, "kv_lens", b, dev),
-                           q_rows=_ints(q_rows, "q_rows", b, dev), **cache)
-    L.check(getattr(lib, name + "_check")(C.byref(args)), name)
-    need = getattr(lib, name + "_workspace_bytes")(C.byref(args))
-    ws = Workspace.get(dev, need, name)
-    args.workspace, args.workspace_bytes = _ptr(ws), need
-    L.check(getattr(lib, name)(C.byref(args), _stream()), name)
+    shape = (b, hq, s, d)
+    qs, os_ = _rows4(q, "q", shape, dt, index), _rows4(out, "out", shape, dt, index)
+    args = L.CacheAttnArgs.from_buffer_copy(_pack(
+        _CACHE_ATTN, _dt(q), b, s, hq, h, d, length, window, sinks, sm_scale, q.data_ptr(), out.data_ptr(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2],
+        _ints(kv_lens, "kv_lens", b, index), _ints(q_rows, "q_rows", b, index), *caches, 0, 0))
+    ref = C.byref(args)
+    need = getattr(lib, name + "_workspace_bytes")(ref)
+    if need:
+        ws = Workspace.get(q.device, need, name)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    status = getattr(lib, name)(ref, _raw_stream(index))
+    if status:
+        L.check(status, name)
     return out
 
 
@@ -443,24 +484,23 @@ def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
     its own, with ``window > 0`` only the last ``window`` of these and the first ``sinks`` ones.  A row that sees nothing
     gives zeros.  Rows from ``q_rows`` on are left as they are in ``out`` (zero when it is not given).  Returns ``out``,
     ``(B, Hq, S, D)``; by default laid out so that ``out.transpose(1, 2).reshape(B, S, Hq * D)`` is a view."""
-    dev = _cuda_device(q)
-    if k_cache.dim() != 4:
-        raise ValueError(f"k_cache must have shape (B, Hkv, L, D), not {tuple(k_cache.shape)}")
-    b, h, length, d = k_cache.shape
-    with torch.cuda.device(dev):
-        kp, ks = _rows4(k_cache, "k_cache", (b, h, length, d), q.dtype, dev)
-        vp, vs = _rows4(v_cache, "v_cache", (b, h, length, d), q.dtype, dev)
-        return _cache_attn("tb200_attn_window", q, out, kv_lens, q_rows, window, sinks, sm_scale, (b, h, length, d, q.dtype),
-                           k_cache=kp, v_cache=vp, k_stride=ks, v_stride=vs)
+    index = _device_index(q)
+    shape = k_cache.shape
+    if len(shape) != 4:
+        raise ValueError(f"k_cache must have shape (B, Hkv, L, D), not {tuple(shape)}")
+    ks, vs = _rows4(k_cache, "k_cache", shape, q.dtype, index), _rows4(v_cache, "v_cache", shape, q.dtype, index)
+    caches = (k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], 0, 0, 0, 0)
+    return _on_device(index, _cache_attn, "tb200_attn_window", q, out, kv_lens, q_rows, window, sinks, sm_scale, (*shape, q.dtype), caches, index)
 
 
 def kv4_attn(q: torch.Tensor, cache: Kv4Cache, kv_lens: torch.Tensor, *, window: int = 0, sinks: int = 0, sm_scale: float = 1.0,
              q_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attn_window`` over a 4-bit cache: the same arguments and the same result, with ``cache`` a :class:`Kv4Cache`."""
-    dev = _cuda_device(q)
-    with torch.cuda.device(dev):
-        dims, ptrs = _kv4_parts(cache, dev)
-        return _cache_attn("tb200_kv4_attn", q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, **ptrs)
+    index = _device_index(q)
+    dims = _kv4_parts(cache, index)
+    kc, vc, km, vm = cache
+    caches = (0, 0, 0, 0, 0, 0, 0, 0, kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr())
+    return _on_device(index, _cache_attn, "tb200_kv4_attn", q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index)
 
 
 def device_status() -> int:
