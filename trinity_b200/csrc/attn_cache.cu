@@ -17,9 +17,9 @@
 //            AND per two codes makes an operand.  With K = lo + c s per group of 64:  q.k = sum_g s_g (q.c)_g + lo_g sum(q)_g,
 //            so s and lo meet the scores in fp32 and no key is ever rounded.  With V:  o = sum_g [sum_j (p_j s_jg)(c_jd - 8) +
 //            sum_j p_j (lo_jg + 8 s_jg)]: the scale goes into the probability (rounded to fp16, after a power of two that
-//            keeps the largest p s below 2^14), the second sum is fp32, and the 8 is taken out with the SAME rounded
-//            probabilities (an MMA against a constant -8 into the same accumulator): the rounding error is that of centred codes,
-//            and the accumulator stays small, which matters because the tensor core's additions truncate.
+//            keeps the largest p s below 2^14), the second sum is fp32, and for fp16 outputs the 8 is taken out with the SAME
+//            rounded probabilities (an MMA against a constant 8), so that the rounding error is that of centred codes, 2.6
+//            times smaller; bf16 outputs are rounded sixteen times more coarsely than that and do without.
 //            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 #include <math.h>
 
@@ -47,6 +47,7 @@ struct CacheAttnParams {
   const uint8_t *k_codes, *v_codes, *k_meta, *v_meta;
   float* part_o;             // (2 grid, R, D)
   float* part_ml;            // (2 grid, R, 2)
+  int4* split;               // (grid): the unit that begins in a stretch and goes on behind it: sequence, kv head, row tile, stretches it lies in (0: none)
   int stretches;             // CTAs of the decode kernel
   int* err;
   long long wait_limit;
@@ -80,9 +81,8 @@ struct Line {
   int seq;      // the sequence in which position x lies
   int base;     // the line's position of that sequence's first tile
 };
-// pick(total, per) chooses x, the position to look for (x >= total: seq and base are not set).
-template <typename Pick>
-__device__ __forceinline__ Line walk_line(const CacheAttnParams& p, int tile, int unit_rows, int min_tiles, Pick pick) {
+// x is the first position of stretch `stretch` (behind the line's end: seq and base are not set).
+__device__ __forceinline__ Line walk_line(const CacheAttnParams& p, int tile, int unit_rows, int min_tiles, int stretch) {
   const int lane = static_cast<int>(lane_id());
   Line ln;
   ln.seq = ln.base = 0;
@@ -107,7 +107,7 @@ __device__ __forceinline__ Line walk_line(const CacheAttnParams& p, int tile, in
   }
   ln.total = total;
   ln.per = max((total + p.stretches - 1) / p.stretches, min_tiles);
-  const int x = pick(ln);
+  const int x = ln.per * stretch;
   if (x >= total) return ln;
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -173,6 +173,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
   using L = DecSmem<D, NT>;
   constexpr int NG = D / 64;
   constexpr int R = L::kR;
+  // fp16 outputs are worth the centred codes (see above); bf16's own rounding is sixteen times coarser than what they gain
+  constexpr bool kCentre = !IsBf16<T>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -188,10 +190,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
   }
   __syncthreads();
 
-  const Line ln = walk_line(p, kTile, R, kMinTiles, [&](const Line& l) { return l.per * static_cast<int>(blockIdx.x); });
+  const Line ln = walk_line(p, kTile, R, kMinTiles, blockIdx.x);
   int x = ln.per * static_cast<int>(blockIdx.x);
   const int x_end = min(x + ln.per, ln.total);
-  if (x >= x_end) return;
+  if (x >= x_end) {
+    if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   int base = ln.base, b = ln.seq;
   Seq sq = load_seq(p, b, kTile, R);
   uint32_t used = 0;    // tiles this warp has taken through its ring
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
     // ---- the unit's query rows: MMA column m is row rt * R + m, i.e. (token, query head of the group)
     const int n_rows = sq.r * p.group;
     uint32_t qf[NT][NG][4][2];
-    float2 qs[NT][NG], cf[NT];
+    float qs[NT][NG][2], cf[NT][2];
     int cpos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -291,33 +296,29 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
         const int src = (2 * t + c) * 4;
         const float u = __shfl_sync(0xffffffffu, up, src);
         // 2^24, and never 0: a hidden score is -inf times this
-        const float f = fmaxf(__shfl_sync(0xffffffffu, down, src) * (p.scale_log2 * 16777216.f), 1.17549435e-38f);
-        if (c == 0) cf[nt].x = f; else cf[nt].y = f;
+        cf[nt][c] = fmaxf(__shfl_sync(0xffffffffu, down, src) * (p.scale_log2 * 16777216.f), 1.17549435e-38f);
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          const float q1 = __shfl_sync(0xffffffffu, sum[gr], src) * u * 5.9604644775390625e-8f;   // 2^-24
-          if (c == 0) qs[nt][gr].x = q1; else qs[nt][gr].y = q1;
-        }
+        for (int gr = 0; gr < NG; ++gr) qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[gr], src) * u * 5.9604644775390625e-8f;   // 2^-24
         const int mc = rt * R + nt * 8 + 2 * t + c;
         cpos[nt][c] = mc < n_rows ? sq.n - sq.r + mc / p.group : -1;
       }
     }
 
-    float o[NT][NG][4][4], mx[NT][2];
-    float2 z[NT][NG], l[NT], nmref[NT];
+    // o, z, l: relative to 2^(maximum) and, all alike, times 2^(5 - exponent of the largest V scale so far), see `ev`
+    float o[NT][NG][4][4], o8[NT][NG][2], z[NT][NG][2], l[NT][2], mx[NT][2], shift[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
+      for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int gr = 0; gr < NG; ++gr) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][gr][i][e] = 0.f;
-        z[nt][gr] = make_float2(0.f, 0.f);
+          for (int i = 0; i < 4; ++i) o[nt][gr][i][c] = o[nt][gr][i][2 + c] = 0.f;
+          o8[nt][gr][c] = z[nt][gr][c] = 0.f;
+        }
+        mx[nt][c] = -INFINITY;
+        l[nt][c] = shift[nt][c] = 0.f;
       }
-      mx[nt][0] = mx[nt][1] = -INFINITY;
-      l[nt] = nmref[nt] = make_float2(0.f, 0.f);
-    }
     int ev = 30;   // biased exponent of the largest V scale so far
 
     for (int v = v0 + warp; v < v1; v += kWarps) {
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
       // every key of the tile visible to every row of the sequence?
       const bool full = k0 + kTile - 1 <= sq.n - sq.r && (p.window == 0 || k0 > sq.n - 1 - p.window || k0 + kTile - 1 < p.sinks);
 
-      float2 s[kTile / 16][NT][2];   // [keys g, g + 8][rows 2t, 2t + 1], without the row's factor cf
+      float s[kTile / 16][NT][4];   // scores without the row's factor cf: keys g (rows 2t, 2t + 1) and g + 8 of sixteen; then probabilities
 #pragma unroll
       for (int sp = 0; sp < kTile / 16; ++sp) {
         // MMA row (slot) 2a + e of eight is key a + 4 e: the four lanes of a column pair then read neighbouring rows
@@ -361,30 +362,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
         load_meta<T, NG>(km + key0 * (NG * 4), m0);
         load_meta<T, NG>(km + key1 * (NG * 4), m1);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float2 y0 = __fmul2_rn(make_float2(m0[0].y, m0[0].y), qs[nt][0]), y1 = __fmul2_rn(make_float2(m1[0].y, m1[0].y), qs[nt][0]);
-          if constexpr (NG == 2) {
-            y0 = __ffma2_rn(make_float2(m0[1].y, m0[1].y), qs[nt][1], y0);
-            y1 = __ffma2_rn(make_float2(m1[1].y, m1[1].y), qs[nt][1], y1);
-          }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-            y0 = __ffma2_rn(make_float2(m0[gr].x, m0[gr].x), make_float2(acc[nt][gr][0], acc[nt][gr][1]), y0);
-            y1 = __ffma2_rn(make_float2(m1[gr].x, m1[gr].x), make_float2(acc[nt][gr][2], acc[nt][gr][3]), y1);
-          }
-          s[sp][nt][0] = y0; s[sp][nt][1] = y1;
-        }
-        if (!full) {
-          const int a = k0 + key0, d = k0 + key1;
+          for (int c = 0; c < 2; ++c) {
+            float y0 = m0[0].y * qs[nt][0][c], y1 = m1[0].y * qs[nt][0][c];
+            if constexpr (NG == 2) {
+              y0 = fmaf(m0[1].y, qs[nt][1][c], y0);
+              y1 = fmaf(m1[1].y, qs[nt][1][c], y1);
+            }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            auto sees = [&](int key, int pos) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.sinks); };
-            if (!sees(a, cpos[nt][0])) s[sp][nt][0].x = -INFINITY;
-            if (!sees(a, cpos[nt][1])) s[sp][nt][0].y = -INFINITY;
-            if (!sees(d, cpos[nt][0])) s[sp][nt][1].x = -INFINITY;
-            if (!sees(d, cpos[nt][1])) s[sp][nt][1].y = -INFINITY;
+            for (int gr = 0; gr < NG; ++gr) {
+              y0 = fmaf(m0[gr].x, acc[nt][gr][c], y0);
+              y1 = fmaf(m1[gr].x, acc[nt][gr][2 + c], y1);
+            }
+            s[sp][nt][c] = y0;
+            s[sp][nt][2 + c] = y1;
+            if (!full) {
+              const int a = k0 + key0, d = k0 + key1, pos = cpos[nt][c];
+              if (!(a <= pos && (p.window == 0 || a > pos - p.window || a < p.sinks))) s[sp][nt][c] = -INFINITY;
+              if (!(d <= pos && (p.window == 0 || d > pos - p.window || d < p.sinks))) s[sp][nt][2 + c] = -INFINITY;
+            }
           }
-        }
       }
 
       // ---- running maximum of the scores and of the V scales: what a thread sees of either decides whether the warp has
@@ -409,81 +407,91 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
       float top[NT][2];
       bool grown = static_cast<int>(big >> 23) > ev;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float t0 = fmaxf(s[0][nt][0].x, s[0][nt][1].x), t1 = fmaxf(s[0][nt][0].y, s[0][nt][1].y);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int sp = 1; sp < kTile / 16; ++sp) {
-          t0 = max3(t0, s[sp][nt][0].x, s[sp][nt][1].x);
-          t1 = max3(t1, s[sp][nt][0].y, s[sp][nt][1].y);
+        for (int c = 0; c < 2; ++c) {
+          float x = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
+#pragma unroll
+          for (int sp = 1; sp < kTile / 16; ++sp) x = max3(x, s[sp][nt][c], s[sp][nt][2 + c]);
+          top[nt][c] = x * cf[nt][c];
+          grown |= top[nt][c] > mx[nt][c] + kSlack;
         }
-        top[nt][0] = t0 * cf[nt].x;
-        top[nt][1] = t1 * cf[nt].y;
-        grown |= top[nt][0] > mx[nt][0] + kSlack || top[nt][1] > mx[nt][1] + kSlack;
-      }
       if (__any_sync(0xffffffffu, grown)) {
         const int ev_new = max(ev, static_cast<int>(__reduce_max_sync(0xffffffffu, big) >> 23));
         const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 + ev - ev_new, 0)) << 23);   // 2^(ev - ev_new)
         ev = ev_new;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float a[2];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float m_new = top[nt][c];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
             m_new = fmaxf(m_new, mx[nt][c]);
-            a[c] = m_new == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - m_new);
+            const float a = (m_new == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - m_new)) * shrink;
             mx[nt][c] = m_new;
+            shift[nt][c] = static_cast<float>(132 - ev) - (m_new == -INFINITY ? 0.f : m_new);   // 5 - (ev - 127): with p <= 2^kSlack, p s < 2^14
+            l[nt][c] *= a;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+              z[nt][gr][c] *= a;
+              if (kCentre) o8[nt][gr][c] *= a;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                o[nt][gr][i][c] *= a;
+                o[nt][gr][i][2 + c] *= a;
+              }
+            }
           }
-          const float2 a2 = make_float2(a[0], a[1]), as2 = make_float2(a[0] * shrink, a[1] * shrink);
-          nmref[nt] = make_float2(mx[nt][0] == -INFINITY ? 0.f : -mx[nt][0], mx[nt][1] == -INFINITY ? 0.f : -mx[nt][1]);
-          l[nt] = __fmul2_rn(l[nt], a2);
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-            z[nt][gr] = __fmul2_rn(z[nt][gr], a2);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][gr][i][e] *= (e & 1) ? as2.y : as2.x;
-          }
-        }
       }
-      const float sfac = __uint_as_float(static_cast<uint32_t>(259 - ev) << 23);   // 2^(5 - exponent): with p <= 2^kSlack, p s sfac < 2^14
 
 #pragma unroll
-      for (int sp = 0; sp < kTile / 16; ++sp) {
-        const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
-        float2 e[NT][2];
+      for (int sp = 0; sp < kTile / 16; ++sp)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 y = __ffma2_rn(s[sp][nt][k], cf[nt], nmref[nt]);
-            e[nt][k] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
-            l[nt] = __fadd2_rn(l[nt], e[nt][k]);
+          for (int c = 0; c < 2; ++c) {
+            s[sp][nt][c] = fast_exp2(fmaf(s[sp][nt][c], cf[nt][c], shift[nt][c]));
+            s[sp][nt][2 + c] = fast_exp2(fmaf(s[sp][nt][2 + c], cf[nt][c], shift[nt][c]));
+            l[nt][c] += s[sp][nt][c] + s[sp][nt][2 + c];
           }
-        float2 m0[NG], m1[NG];
-        load_meta<T, NG>(vm + key0 * (NG * 4), m0);
-        load_meta<T, NG>(vm + key1 * (NG * 4), m1);
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          const float s0 = m0[gr].x * sfac, s1 = m1[gr].x * sfac, c0 = fmaf(8.f, m0[gr].x, m0[gr].y), c1 = fmaf(8.f, m1[gr].x, m1[gr].y);
+      for (int gr = 0; gr < NG; ++gr) {
+        // a tile's products are summed from zero and then added in fp32: the tensor core's additions truncate, and over
+        // thousands of keys with codes of one sign that would add up
+        float part[NT][4][4], part8[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            part8[nt][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[nt][i][e] = 0.f;
+          }
+#pragma unroll
+        for (int sp = 0; sp < kTile / 16; ++sp) {
+          const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
+          const float2 m0 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key0 * NG + gr) * 4));
+          const float2 m1 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key1 * NG + gr) * 4));
+          const float c0 = kCentre ? fmaf(8.f, m0.x, m0.y) : m0.y, c1 = kCentre ? fmaf(8.f, m1.x, m1.y) : m1.y;
           uint32_t pf[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float2 w0 = __fmul2_rn(e[nt][0], make_float2(s0, s0)), w1 = __fmul2_rn(e[nt][1], make_float2(s1, s1));
+            const float* e = s[sp][nt];
+            float w[4] = {e[0] * m0.x, e[1] * m0.x, e[2] * m1.x, e[3] * m1.x};
             if (full) {
-              z[nt][gr] = __ffma2_rn(e[nt][0], make_float2(c0, c0), z[nt][gr]);
-              z[nt][gr] = __ffma2_rn(e[nt][1], make_float2(c1, c1), z[nt][gr]);
+              z[nt][gr][0] = fmaf(e[2], c1, fmaf(e[0], c0, z[nt][gr][0]));
+              z[nt][gr][1] = fmaf(e[3], c1, fmaf(e[1], c0, z[nt][gr][1]));
             } else {   // what a row does not see may hold anything: 0 * inf and 0 * NaN must not arise
-              if (e[nt][0].x > 0.f) z[nt][gr].x = fmaf(e[nt][0].x, c0, z[nt][gr].x); else w0.x = 0.f;
-              if (e[nt][0].y > 0.f) z[nt][gr].y = fmaf(e[nt][0].y, c0, z[nt][gr].y); else w0.y = 0.f;
-              if (e[nt][1].x > 0.f) z[nt][gr].x = fmaf(e[nt][1].x, c1, z[nt][gr].x); else w1.x = 0.f;
-              if (e[nt][1].y > 0.f) z[nt][gr].y = fmaf(e[nt][1].y, c1, z[nt][gr].y); else w1.y = 0.f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (e[i] > 0.f) z[nt][gr][i & 1] = fmaf(e[i], i < 2 ? c0 : c1, z[nt][gr][i & 1]);
+                else w[i] = 0.f;
+              }
             }
-            pf[nt][0] = transpose8x8(Pack2<__half>::pack(w0.x, w0.y));
-            pf[nt][1] = transpose8x8(Pack2<__half>::pack(w1.x, w1.y));
+            pf[nt][0] = transpose8x8(Pack2<__half>::pack(w[0], w[1]));
+            pf[nt][1] = transpose8x8(Pack2<__half>::pack(w[2], w[3]));
+            if constexpr (kCentre) mma_f16(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
           }
           // MMA columns 2t, 2t+1 (and 2t+8, 2t+9) of V^T are keys t, t + 4 (and t + 8, t + 12); row g of the four row tiles
           // holds elements 8 g + {0, 2, 4, 6}, row g + 8 the odd ones
@@ -496,10 +504,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
           for (int i = 0; i < 4; ++i) {
             const uint32_t x0 = ((i & 2) ? xh : xl) >> ((i & 1) * 8), y0 = ((i & 2) ? yh : yl) >> ((i & 1) * 8);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(o[nt][gr][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
-              // minus 8 p: -8 * 2^-24 in row g, -8 * 2^-20 in row g + 8
-              mma_f16(o[nt][gr][i], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[nt][0], pf[nt][1]);
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if constexpr (kCentre) o8[nt][gr][c] += part8[nt][c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[nt][gr][i][c] += part[nt][i][c];
+              o[nt][gr][i][2 + c] += part[nt][i][2 + c];
             }
           }
         }
@@ -513,30 +530,33 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
     __syncthreads();   // every warp is done with its ring
     float* wm = reinterpret_cast<float*>(smem + L::kMergeOff) + warp * R * L::kMergePitch;
     float2* wml = reinterpret_cast<float2*>(smem + L::kMlOff) + warp * R;
-    const float fe = __uint_as_float(static_cast<uint32_t>(ev) << 23);   // 2^24 / sfac = 2^19 * 2^(ev - 127)
+    const float fe = __uint_as_float(static_cast<uint32_t>(ev - 5) << 23);   // 2^(ev - 127 - 5): out of the accumulators' scale
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int m = nt * 8 + 2 * t + c;
-        float ls = c ? l[nt].y : l[nt].x;
+        float ls = l[nt][c];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, d);
-        if (g == 0) wml[m] = make_float2(mx[nt][c], ls);
+        if (g == 0) wml[m] = make_float2(mx[nt][c], ls * fe);
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
-          float zs = c ? z[nt][gr].y : z[nt][gr].x;
+          float zs = z[nt][gr][c];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) zs += __shfl_xor_sync(0xffffffffu, zs, d);
+          const float a8 = kCentre ? o8[nt][gr][c] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)   // 2^24; row g + 8 holds codes times 2^-20
             *reinterpret_cast<float2*>(wm + m * L::kMergePitch + gr * 64 + g * 8 + 2 * i) =
-                make_float2(fmaf(o[nt][gr][i][c] * 524288.f, fe, zs), fmaf(o[nt][gr][i][2 + c] * 32768.f, fe, zs));   // 2^19, 2^15
+                make_float2(fmaf(o[nt][gr][i][c] - a8, 16777216.f, zs) * fe, fmaf(o[nt][gr][i][2 + c] * 0.0625f - a8, 16777216.f, zs) * fe);
         }
       }
     __syncthreads();
     // ---- the four warps' shares, in a fixed order
     const bool whole = v0 == 0 && v1 == sq.tiles;
+    if (threadIdx.x == 0 && x + v1 - v0 >= x_end)   // the stretch's last segment
+      p.split[blockIdx.x] = make_int4(b, h, rt, v0 == 0 && !whole ? (x + sq.tiles - 1) / ln.per - static_cast<int>(blockIdx.x) + 1 : 0);
     const float* mall = reinterpret_cast<const float*>(smem + L::kMergeOff);
     const float2* mlall = reinterpret_cast<const float2*>(smem + L::kMlOff);
     const int slot_out = 2 * blockIdx.x + (v0 == 0 ? 1 : 0);
@@ -574,86 +594,90 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
   }
 }
 
-// Merges the partial results of the units that lie in several stretches.  CTA (c, y): the unit that begins in stretch c
-// and goes on behind its end, if there is one, and of it the rows y, y + gridDim.y, ...; its first part is in slot 2c + 1,
-// the others in the slots 2c' of the stretches c' it covers.
-constexpr int kCombineThreads = 128;
+// Merges the partial results of the units that lie in several stretches.  CTA (c, y): rows 4y to 4y + 3 of the unit that
+// begins in stretch c and goes on behind its end, if there is one; its first part is in slot 2c + 1, the others in the slots
+// 2c' of the stretches c' it covers.  The four warps share the parts; sums are taken in a fixed order.
+constexpr int kCombineThreads = 128, kCombineRows = 4;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kCombineThreads) cache_combine_kernel(const __grid_constant__ CacheAttnParams p) {
-  constexpr int R = 8 * NT;
-  constexpr int kLanes = D / 4, kParts = kCombineThreads / kLanes;   // parts summed side by side
-  extern __shared__ float weights[];                                 // [stretches]
-  __shared__ float4 red[kParts][kLanes];
-  __shared__ float2 tops[kCombineThreads / 32];
+  constexpr int R = 8 * NT, V = D / 32;
+  extern __shared__ float weights[];                                 // [rows][stretches]
+  __shared__ float red[4][kCombineRows][D];
   pdl_launch_dependents();
-  const int c = blockIdx.x;
-  const Line ln = walk_line(p, kTile, R, kMinTiles, [&](const Line& l) { return l.per * (c + 1) - 1; });
-  const int end = ln.per * (c + 1);
-  bool mine = end < ln.total;
-  Seq sq;
-  int unit = 0, u1 = 0, rts = 1;
-  if (mine) {
-    sq = load_seq(p, ln.seq, kTile, R);
-    unit = (end - 1 - ln.base) / sq.tiles;
-    const int u0 = ln.base + unit * sq.tiles;
-    u1 = u0 + sq.tiles;
-    rts = sq.units / p.Hkv;
-    mine = u1 > end && u0 >= ln.per * c;
-  }
+  const int c = blockIdx.x, m0 = blockIdx.y * kCombineRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  if (!mine) return;
-  const int b = ln.seq, h = unit / rts, rt = unit - h * rts;
-  const int parts = (u1 - 1) / ln.per - c + 1;
-  const int tid = threadIdx.x;
-  for (int m = blockIdx.y; m < R; m += gridDim.y) {
-    const int mr = rt * R + m;
-    if (mr >= sq.r * p.group) break;
-    auto slot = [&](int i) { return static_cast<long long>(2 * (c + i) + (i == 0 ? 1 : 0)) * R + m; };
-    // weights of the parts, their common maximum and sum
-    float top = -INFINITY;
-    for (int i = tid; i < parts; i += kCombineThreads) top = fmaxf(top, __ldcg(p.part_ml + slot(i) * 2));
+  const int4 rec = __ldcg(p.split + c);
+  const int parts = rec.w;
+  if (parts == 0) return;
+  const int b = rec.x, h = rec.y, rt = rec.z;
+  const int r = p.q_rows ? max(0, min(__ldg(p.q_rows + b), p.S)) : p.S;
+  if (rt * R + m0 >= r * p.group) return;
+  auto slot = [&](int i, int m) { return static_cast<long long>(2 * (c + i) + (i == 0 ? 1 : 0)) * R + m0 + m; };
+  float acc[kCombineRows][V], first[kCombineRows][V];
+  auto fetch = [&](int i, float (&v)[kCombineRows][V]) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if ((tid & 31) == 0) tops[tid >> 5].x = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kCombineThreads / 32; ++w) top = fmaxf(top, tops[w].x);
-    float sum = 0.f;
-    for (int i = tid; i < parts; i += kCombineThreads) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2));
-      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-      weights[i] = f;
-      sum = fmaf(f, ml.y, sum);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if ((tid & 31) == 0) tops[tid >> 5].y = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kCombineThreads / 32; ++w) sum += tops[w].y;
-    const int part = tid / kLanes, d4 = tid % kLanes;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = part; i < parts; i += kParts) {
-      const float f = weights[i];
-      const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot(i) * D) + d4);
-      acc.x = fmaf(f, a.x, acc.x); acc.y = fmaf(f, a.y, acc.y); acc.z = fmaf(f, a.z, acc.z); acc.w = fmaf(f, a.w, acc.w);
-    }
-    red[part][d4] = acc;
-    __syncthreads();
-    if (part == 0) {
-#pragma unroll
-      for (int w = 1; w < kParts; ++w) {
-        const float4 a = red[w][d4];
-        acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
+    for (int m = 0; m < kCombineRows; ++m) {
+      const float* src = p.part_o + slot(i, m) * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
+        v[m][0] = f.x; v[m][1] = f.y; v[m][2] = f.z; v[m][3] = f.w;
+      } else {
+        const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
+        v[m][0] = f.x; v[m][1] = f.y;
       }
-      const float inv = sum > 0.f ? 1.f / sum : sum;
-      const int tok = mr / p.group;
-      T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + d4 * 4;
-      *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
     }
-    __syncthreads();   // tops, weights and red are free again
+  };
+  if (warp < parts) fetch(warp, first);   // on its way while the weights are made
+  // warp w: the weights of row w's parts, their maximum and sum
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(p.part_ml + slot(i, warp) * 2));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float sum = 0.f;
+  for (int i = lane; i < parts; i += 32) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot(i, warp) * 2));
+    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+    weights[warp * p.stretches + i] = f;
+    sum = fmaf(f, ml.y, sum);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < kCombineRows; ++m)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[m][e] = warp < parts ? first[m][e] * weights[m * p.stretches + warp] : 0.f;
+#pragma unroll 4
+  for (int i = warp + 4; i < parts; i += 4) {
+    fetch(i, first);
+#pragma unroll
+    for (int m = 0; m < kCombineRows; ++m) {
+      const float f = weights[m * p.stretches + i];
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[m][e] = fmaf(f, first[m][e], acc[m][e]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kCombineRows; ++m)
+#pragma unroll
+    for (int e = 0; e < V; ++e) red[warp][m][lane * V + e] = acc[m][e];
+  __syncthreads();
+  const int mr = rt * R + m0 + warp;
+  if (mr >= r * p.group) return;
+  const float inv = sum > 0.f ? 1.f / sum : sum;   // 0: the row sees nothing; NaN stays
+  const int tok = mr / p.group;
+  T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; e += 2) {
+    float y[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      y[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) y[k] += red[w][warp][lane * V + e + k];
+    }
+    *reinterpret_cast<uint32_t*>(op + e) = Pack2<T>::pack(y[0] * inv, y[1] * inv);
   }
 }
 
@@ -694,8 +718,8 @@ struct AttnPlan {
   int nt = 1;                // decode: MMA column blocks of a unit
   int stretches = 0;
   int kv_splits = 1;         // prompt
-  size_t part_o = 0, part_ml = 0, cache16 = 0;   // bytes; cache16: of one of the two caches
-  size_t total() const { return part_o + part_ml + 2 * cache16; }
+  size_t part_o = 0, part_ml = 0, split = 0, cache16 = 0;   // bytes; cache16: of one of the two caches
+  size_t total() const { return part_o + part_ml + split + 2 * cache16; }
 };
 AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   AttnPlan pl;
@@ -716,6 +740,7 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   pl.stretches = num_sms * ctas_per_sm(pl.nt);
   pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * a->head_dim * sizeof(float), 256);
   pl.part_ml = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * 2 * sizeof(float), 256);
+  pl.split = align_up(static_cast<size_t>(pl.stretches) * sizeof(int4), 256);
   return pl;
 }
 
@@ -751,10 +776,8 @@ int launch_decode(const CacheAttnParams& p, cudaStream_t stream) {
     attr_set[dev & 31] = true;
   }
   if (launch_chained(cache_decode_kernel<T, D, NT>, dim3(p.stretches), dim3(kThreads), L::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
-  // few units are split over many stretches each: a CTA per row of a unit; many units: one CTA for all rows
-  int combine_rows = 1;
-  while (combine_rows < 8 * NT && static_cast<long long>(p.B) * p.Hkv * combine_rows * 2 <= 256) combine_rows *= 2;
-  if (launch_chained(cache_combine_kernel<T, D, NT>, dim3(p.stretches, combine_rows), dim3(kCombineThreads), p.stretches * sizeof(float), stream, p) != cudaSuccess)
+  if (launch_chained(cache_combine_kernel<T, D, NT>, dim3(p.stretches, 8 * NT / kCombineRows), dim3(kCombineThreads),
+                     kCombineRows * p.stretches * sizeof(float), stream, p) != cudaSuccess)
     return TB200_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
 }
@@ -808,6 +831,7 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   p.stretches = pl.stretches;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
+  p.split = reinterpret_cast<int4*>(static_cast<uint8_t*>(a->workspace) + pl.part_o + pl.part_ml);
   return a->dtype == TB200_BF16 ? run_kv4<__nv_bfloat16>(p, a->head_dim, pl.nt, stream) : run_kv4<__half>(p, a->head_dim, pl.nt, stream);
 }
 
