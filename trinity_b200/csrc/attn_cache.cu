@@ -1,16 +1,10 @@
 // Attention over a cache that already holds the new rows: tb200_attn_window (16-bit caches) and tb200_kv4_attn (4-bit
 // caches), per-sequence lengths, an optional sliding window with a few first positions that stay visible.
 //
-// cache_decode_kernel: few query rows per sequence.  Bound: HBM (the visible cache rows are read once per key/value
+// cache_decode_kernel: few query rows per sequence on a 4-bit cache (units, line and stretches: cache_line.cuh; a warp has
+// its own ring of bulk copies, no CTA-wide barrier inside a segment).  Bound: HBM (the visible cache rows are read once per key/value
 // head), and the instructions that turn 4-bit codes into matrix operands.
 //
-//   unit     (sequence, kv head, R query rows): the rows of a unit are (new token, query head of the group) pairs, so
-//            that a cache row is read once for all query heads that share it.  R = 8 or 16 columns of an MMA.
-//   work     the key tiles of all units form one line, dealt out in equal stretches over the CTAs (each computes the
-//            line's layout from kv_lens itself): long and short sequences load the SMs evenly, with no host knowledge
-//            of the lengths.  A unit that lies within one CTA's stretch is finished there; the others leave a partial
-//            result (accumulator, maximum, sum) per stretch, which cache_combine_kernel merges in the order of the keys.
-//   warp     takes every fourth tile of a stretch: its own ring of bulk copies, no CTA-wide barrier inside a stretch.
 //   math     transposed: S^T = K Q^T (keys are the rows of the MMA, query rows its 8 columns), O^T = V^T P^T.
 //   4 bits   a code c needs no conversion: the bits c in the low mantissa of an otherwise zero fp16 are the number
 //            c * 2^-24, one nibble higher c * 2^-20, and the tensor core takes such (subnormal) numbers exactly.  One
@@ -23,115 +17,19 @@
 //            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 #include <math.h>
 
-#include "common.cuh"
-#include "internal.h"
-#include "kv4.cuh"
+#include "cache_line.cuh"
 
 namespace tb200 {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-
-struct CacheAttnParams {
-  int B, S, Hq, Hkv, group, cache_len, window, sinks;
-  int row_tiles;             // units per (sequence, kv head) at most
-  float scale_log2;
-  const uint8_t* q;
-  uint8_t* o;
-  long long qs[3], os[3];
-  const int32_t* kv_lens;
-  const int32_t* q_rows;
-  const uint8_t *k_codes, *v_codes, *k_meta, *v_meta;
-  float* part_o;             // (2 grid, R, D)
-  float* part_ml;            // (2 grid, R, 2)
-  int4* split;               // (grid): the unit that begins in a stretch and goes on behind it: sequence, kv head, row tile, stretches it lies in (0: none)
-  int stretches;             // CTAs of the decode kernel
-  int* err;
-  long long wait_limit;
-};
-
-// What a sequence asks for.
-struct Seq {
-  int n, r;                  // positions, new rows
-  int few;                   // first positions that stay visible, below the window
-  int sink_tiles, win_tile;  // tiles [0, sink_tiles) and from win_tile on
-  int tiles;                 // tiles of a unit
-  int units;                 // units of the sequence: kv heads x row tiles
-};
-__device__ __forceinline__ Seq load_seq(const CacheAttnParams& p, int b, int tile, int unit_rows) {
-  Seq s;
-  s.n = max(0, min(__ldg(p.kv_lens + b), p.cache_len));
-  s.r = p.q_rows ? max(0, min(__ldg(p.q_rows + b), p.S)) : p.S;
-  const int low = p.window > 0 ? max(0, s.n - s.r - p.window + 1) : 0;
-  s.few = min(p.sinks, low);
-  s.win_tile = low / tile;
-  s.sink_tiles = min((s.few + tile - 1) / tile, s.win_tile);
-  s.tiles = max(1, s.sink_tiles + (s.n + tile - 1) / tile - s.win_tile);   // a sequence without keys: one masked tile writes the zeros
-  s.units = s.r > 0 ? p.Hkv * ((s.r * p.group + unit_rows - 1) / unit_rows) : 0;
-  return s;
-}
-
-// The line of all tiles: its length, and how it is dealt out.  Every lane of a warp calls these and gets the same.
-struct Line {
-  int total;    // tiles of all units
-  int per;      // tiles of a stretch
-  int seq;      // the sequence in which position x lies
-  int base;     // the line's position of that sequence's first tile
-};
-// x is the first position of stretch `stretch` (behind the line's end: seq and base are not set).
-__device__ __forceinline__ Line walk_line(const CacheAttnParams& p, int tile, int unit_rows, int min_tiles, int stretch) {
-  const int lane = static_cast<int>(lane_id());
-  Line ln;
-  ln.seq = ln.base = 0;
-  int sum = 0, own = 0, total = 0;
-  auto scan = [&](int b0) {   // inclusive sums over 32 sequences
-    const int b = b0 + lane;
-    own = 0;
-    if (b < p.B) {
-      const Seq s = load_seq(p, b, tile, unit_rows);
-      own = s.tiles * s.units;
-    }
-    sum = own;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += up;
-    }
-  };
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    scan(b0);
-    total += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  ln.total = total;
-  ln.per = max((total + p.stretches - 1) / p.stretches, min_tiles);
-  const int x = ln.per * stretch;
-  if (x >= total) return ln;
-  int before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    if (p.B > 32) scan(b0);   // else the sums are still there
-    const unsigned hit = __ballot_sync(0xffffffffu, before + sum > x);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      ln.seq = b0 + l;
-      ln.base = before + __shfl_sync(0xffffffffu, sum - own, l);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  return ln;
-}
-
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // d = a b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -150,7 +48,6 @@ template <typename T, int NG> __device__ __forceinline__ void load_meta(const ui
 
 constexpr int kTile = 64;     // keys of a tile
 constexpr int kStages = 2;
-constexpr float kSlack = 8.f; // the exponent reference of a row moves only when its maximum has grown by more than 2^kSlack
 constexpr int kMinTiles = kWarps;
 
 template <int D, int NT> struct DecSmem {
@@ -160,11 +57,9 @@ template <int D, int NT> struct DecSmem {
   static constexpr int kStage = 2 * (kCodes + kMeta);      // K codes, V codes, K meta, V meta
   static constexpr int kRing = kStages * kStage;           // per warp
   static constexpr int kMergePitch = D + 4;                // floats per row: 4 keep the rows' banks apart
-  // the merge buffers take the place of the rings, which are empty by then
-  static constexpr int kMergeOff = 0;                      // float [warps][R][pitch]
-  static constexpr int kMlOff = kMergeOff + kWarps * kR * kMergePitch * 4;   // float2 [warps][R]
   static constexpr int kBarOff = kWarps * kRing;
-  static_assert(kMlOff + kWarps * kR * 8 <= kBarOff, "the merge buffers must fit where the rings were");
+  // the merge buffers take the place of the rings, which are empty by then
+  static_assert(MergeSmem<D, NT>::kBytes <= kBarOff, "the merge buffers must fit where the rings were");
   static constexpr int kTotal = kBarOff + kWarps * kStages * 8 + 16;
 };
 
@@ -190,28 +85,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
   }
   __syncthreads();
 
-  const Line ln = walk_line(p, kTile, R, kMinTiles, blockIdx.x);
-  int x = ln.per * static_cast<int>(blockIdx.x);
-  const int x_end = min(x + ln.per, ln.total);
-  if (x >= x_end) {
-    if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
-    return;
-  }
-  int base = ln.base, b = ln.seq;
-  Seq sq = load_seq(p, b, kTile, R);
+  Walk wk;
+  if (!wk.begin(p, kTile, R, kMinTiles)) return;
   uint32_t used = 0;    // tiles this warp has taken through its ring
   bool ok = true;
 
-  while (x < x_end) {   // one segment: the part of a unit that lies in this stretch
-    while (x >= base + sq.tiles * sq.units) {
-      base += sq.tiles * sq.units;
-      sq = load_seq(p, ++b, kTile, R);
-    }
-    const int unit = (x - base) / sq.tiles;
-    const int v0 = x - base - unit * sq.tiles;
-    const int v1 = min(sq.tiles, v0 + x_end - x);
-    const int rts = sq.units / p.Hkv;
-    const int h = unit / rts, rt = unit - h * rts;
+  for (; wk.x < wk.x_end;) {
+    const Segment sg = wk.segment(p, kTile, R);
+    const Seq& sq = wk.sq;
+    const int b = sg.b, h = sg.h, rt = sg.rt, v0 = sg.v0, v1 = sg.v1, n_rows = sg.n_rows;
     const long long crow = (static_cast<long long>(b) * p.Hkv + h) * p.cache_len;
     const int copy_end = min(p.cache_len, max(4, (sq.n + 3) & ~3));   // cache rows worth copying: whole 16 bytes of meta
 
@@ -221,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
     const uint8_t* src = (what == 0 ? p.k_codes : what == 1 ? p.v_codes : what == 2 ? p.k_meta : p.v_meta) + crow * row_bytes;
     uint8_t* dst = ring + (what & 1) * (what < 2 ? L::kCodes : L::kMeta) + (what < 2 ? 0 : 2 * L::kCodes);
     auto issue = [&](int v, uint32_t slot) {   // whole warp: tile v of the unit into ring slot `slot`
-      const int k0 = (v < sq.sink_tiles ? v : sq.win_tile + v - sq.sink_tiles) * kTile;
+      const int k0 = wk.tile_of(v) * kTile;
       const uint32_t rows = static_cast<uint32_t>(min(kTile, copy_end - k0));
       if (lane == 0) mbar_arrive_expect_tx(&bars[slot], rows * (D + NG * 8));
       __syncwarp();
@@ -242,7 +124,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
     }
 
     // ---- the unit's query rows: MMA column m is row rt * R + m, i.e. (token, query head of the group)
-    const int n_rows = sq.r * p.group;
     uint32_t qf[NT][NG][4][2];
     float qs[NT][NG][2], cf[NT][2];
     int cpos[NT][2];
@@ -333,8 +214,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
       const uint8_t* vc = st + L::kCodes;
       const uint8_t* km = st + 2 * L::kCodes;
       const uint8_t* vm = km + L::kMeta;
-      const int tile = v < sq.sink_tiles ? v : sq.win_tile + v - sq.sink_tiles;
-      const int k0 = tile * kTile;
+      const int k0 = wk.tile_of(v) * kTile;
       // every key of the tile visible to every row of the sequence?
       const bool full = k0 + kTile - 1 <= sq.n - sq.r && (p.window == 0 || k0 > sq.n - 1 - p.window || k0 + kTile - 1 < p.sinks);
 
@@ -349,13 +229,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
           const uint2 w0 = *reinterpret_cast<const uint2*>(kc + key0 * (D / 2) + gr * 32 + t * 8);
           const uint2 w1 = *reinterpret_cast<const uint2*>(kc + key1 * (D / 2) + gr * 32 + t * 8);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[nt][gr][0] = acc[nt][gr][1] = acc[nt][gr][2] = acc[nt][gr][3] = 0.f;
-#pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             const uint32_t x0 = ((ks & 2) ? w0.y : w0.x) >> ((ks & 1) * 8), x1 = ((ks & 2) ? w1.y : w1.x) >> ((ks & 1) * 8);
             const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (ks == 0) mma_f16_first(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
+              else mma_f16(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
+            }
           }
         }
         float2 m0[NG], m1[NG];
@@ -461,14 +342,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
         // thousands of keys with codes of one sign that would add up
         float part[NT][4][4], part8[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            part8[nt][e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[nt][i][e] = 0.f;
-          }
-#pragma unroll
         for (int sp = 0; sp < kTile / 16; ++sp) {
           const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
           const float2 m0 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key0 * NG + gr) * 4));
@@ -491,7 +364,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
             }
             pf[nt][0] = transpose8x8(Pack2<__half>::pack(w[0], w[1]));
             pf[nt][1] = transpose8x8(Pack2<__half>::pack(w[2], w[3]));
-            if constexpr (kCentre) mma_f16(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
+            if constexpr (kCentre) {
+              if (sp == 0) mma_f16_first(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
+              else mma_f16(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
+            }
           }
           // MMA columns 2t, 2t+1 (and 2t+8, 2t+9) of V^T are keys t, t + 4 (and t + 8, t + 12); row g of the four row tiles
           // holds elements 8 g + {0, 2, 4, 6}, row g + 8 the odd ones
@@ -504,8 +380,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
           for (int i = 0; i < 4; ++i) {
             const uint32_t x0 = ((i & 2) ? xh : xl) >> ((i & 1) * 8), y0 = ((i & 2) ? yh : yl) >> ((i & 1) * 8);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_f16(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (sp == 0) mma_f16_first(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+              else mma_f16(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+            }
           }
         }
 #pragma unroll
@@ -528,8 +406,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
 
     // ---- this warp's share of the segment into shared memory: o relative to its own maximum
     __syncthreads();   // every warp is done with its ring
-    float* wm = reinterpret_cast<float*>(smem + L::kMergeOff) + warp * R * L::kMergePitch;
-    float2* wml = reinterpret_cast<float2*>(smem + L::kMlOff) + warp * R;
+    using M = MergeSmem<D, NT>;
+    float* wm = reinterpret_cast<float*>(smem) + warp * R * M::kPitch;
+    float2* wml = reinterpret_cast<float2*>(smem + M::kMlOff) + warp * R;
     const float fe = __uint_as_float(static_cast<uint32_t>(ev - 5) << 23);   // 2^(ev - 127 - 5): out of the accumulators' scale
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -548,49 +427,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
           const float a8 = kCentre ? o8[nt][gr][c] : 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i)   // 2^24; row g + 8 holds codes times 2^-20
-            *reinterpret_cast<float2*>(wm + m * L::kMergePitch + gr * 64 + g * 8 + 2 * i) =
+            *reinterpret_cast<float2*>(wm + m * M::kPitch + gr * 64 + g * 8 + 2 * i) =
                 make_float2(fmaf(o[nt][gr][i][c] - a8, 16777216.f, zs) * fe, fmaf(o[nt][gr][i][2 + c] * 0.0625f - a8, 16777216.f, zs) * fe);
         }
       }
     __syncthreads();
-    // ---- the four warps' shares, in a fixed order
-    const bool whole = v0 == 0 && v1 == sq.tiles;
-    if (threadIdx.x == 0 && x + v1 - v0 >= x_end)   // the stretch's last segment
-      p.split[blockIdx.x] = make_int4(b, h, rt, v0 == 0 && !whole ? (x + sq.tiles - 1) / ln.per - static_cast<int>(blockIdx.x) + 1 : 0);
-    const float* mall = reinterpret_cast<const float*>(smem + L::kMergeOff);
-    const float2* mlall = reinterpret_cast<const float2*>(smem + L::kMlOff);
-    const int slot_out = 2 * blockIdx.x + (v0 == 0 ? 1 : 0);
-    for (int i = threadIdx.x; i < R * D / 4; i += kThreads) {
-      const int m = i / (D / 4), d = (i % (D / 4)) * 4;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, mlall[w * R + m].x);
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float2 ml = mlall[w * R + m];
-        const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-        const float4 a = *reinterpret_cast<const float4*>(mall + (w * R + m) * L::kMergePitch + d);
-        sum = fmaf(f, ml.y, sum);
-        acc.x = fmaf(f, a.x, acc.x); acc.y = fmaf(f, a.y, acc.y); acc.z = fmaf(f, a.z, acc.z); acc.w = fmaf(f, a.w, acc.w);
-      }
-      if (whole) {
-        const int mr = rt * R + m;
-        if (mr < n_rows) {
-          const float inv = sum > 0.f ? 1.f / sum : sum;   // 0: the row sees nothing; NaN stays
-          const int tok = mr / p.group;
-          T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + d;
-          *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
-        }
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (static_cast<long long>(slot_out) * R + m) * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot_out) * R + m) * 2) = make_float2(top, sum);
-      }
-    }
+    merge_segment<T, D, NT>(p, smem, wk, sg);
     fence_proxy_async_smem();   // the next bulk copies overwrite what was just read and written
     __syncthreads();
-    x += v1 - v0;
+    wk.x += v1 - v0;
   }
 }
 
@@ -689,7 +534,7 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   if (a->head_dim != 64 && a->head_dim != 128) return TB200_ERR_UNSUPPORTED;
   if (a->batch < 0 || a->rows < 0 || a->n_kv_heads < 1 || a->n_q_heads < 1 || a->n_q_heads % a->n_kv_heads || a->cache_len < 1) return TB200_ERR_INVALID;
   if (a->batch > kMaxExtent || a->cache_len > kMaxExtent || static_cast<int64_t>(a->n_q_heads) * a->rows > kMaxExtent) return TB200_ERR_INVALID;
-  if (a->window < 0 || a->sinks < 0 || !(a->sm_scale > 0.f) || !(a->sm_scale < INFINITY)) return TB200_ERR_INVALID;
+  if (a->window < 0 || a->sinks < 0 || !(a->sm_scale >= 1e-30f) || !(a->sm_scale < INFINITY)) return TB200_ERR_INVALID;
   if (!a->q || !a->o || !a->kv_lens || a->q == a->o || !aligned16(a->q) || !aligned16(a->o) || !aligned4(a->kv_lens) || !aligned4(a->q_rows))
     return TB200_ERR_INVALID;
   const int64_t ext[3] = {a->batch, a->n_q_heads, a->rows};
@@ -710,8 +555,8 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
 // CTAs of the decode kernel that an SM holds: by shared memory (72 KB with 8 query rows, 90 KB with 16 at D = 128)
 constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
-// New rows per sequence up to which a call on a 4-bit cache runs cache_decode_kernel.
-constexpr int kDecodeTokens = 32;
+// New rows per sequence up to which a call runs a decode kernel.
+constexpr int kDecodeTokens4 = 32, kDecodeTokens16 = 32;
 
 struct AttnPlan {
   bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
@@ -724,7 +569,7 @@ struct AttnPlan {
 AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   AttnPlan pl;
   const int64_t rows = static_cast<int64_t>(a->rows) * (a->n_q_heads / a->n_kv_heads);
-  pl.prompt = !kv4 || a->rows > kDecodeTokens;
+  pl.prompt = a->rows > (kv4 ? kDecodeTokens4 : kDecodeTokens16);
   if (pl.prompt) {
     const int64_t seen = a->window > 0 ? static_cast<int64_t>(a->window) + a->rows + a->sinks : a->cache_len;
     pl.kv_splits = attn_kv_splits(a->batch, a->rows, a->n_q_heads, static_cast<int>(seen < a->cache_len ? seen : a->cache_len), num_sms);
@@ -737,7 +582,7 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
     return pl;
   }
   pl.nt = rows <= 8 ? 1 : 2;
-  pl.stretches = num_sms * ctas_per_sm(pl.nt);
+  pl.stretches = kv4 ? num_sms * ctas_per_sm(pl.nt) : cache16_stretches(pl.nt, num_sms);
   pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * a->head_dim * sizeof(float), 256);
   pl.part_ml = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * 2 * sizeof(float), 256);
   pl.split = align_up(static_cast<size_t>(pl.stretches) * sizeof(int4), 256);
@@ -776,10 +621,20 @@ int launch_decode(const CacheAttnParams& p, cudaStream_t stream) {
     attr_set[dev & 31] = true;
   }
   if (launch_chained(cache_decode_kernel<T, D, NT>, dim3(p.stretches), dim3(kThreads), L::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+}
+
+template <typename T, int D, int NT>
+int launch_combine(const CacheAttnParams& p, cudaStream_t stream) {
   if (launch_chained(cache_combine_kernel<T, D, NT>, dim3(p.stretches, 8 * NT / kCombineRows), dim3(kCombineThreads),
                      kCombineRows * p.stretches * sizeof(float), stream, p) != cudaSuccess)
     return TB200_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+}
+template <typename T>
+int launch_combine(const CacheAttnParams& p, int head_dim, int nt, cudaStream_t stream) {
+  if (head_dim == 128) return nt == 1 ? launch_combine<T, 128, 1>(p, stream) : launch_combine<T, 128, 2>(p, stream);
+  return nt == 1 ? launch_combine<T, 64, 1>(p, stream) : launch_combine<T, 64, 2>(p, stream);
 }
 
 template <typename T>
@@ -832,7 +687,14 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
   p.split = reinterpret_cast<int4*>(static_cast<uint8_t*>(a->workspace) + pl.part_o + pl.part_ml);
-  return a->dtype == TB200_BF16 ? run_kv4<__nv_bfloat16>(p, a->head_dim, pl.nt, stream) : run_kv4<__half>(p, a->head_dim, pl.nt, stream);
+  // positions on the line of tiles are 32-bit numbers
+  const int64_t rows = static_cast<int64_t>(a->rows) * p.group;
+  if ((rows / (8 * pl.nt) + 1) * a->n_kv_heads * a->batch * static_cast<double>(a->cache_len / 16 + 2) >= 2147483648.0) return TB200_ERR_UNSUPPORTED;
+  if (!kv4) status = launch_cache16(p, *a, pl.nt, stream);
+  else if (a->dtype == TB200_BF16) status = run_kv4<__nv_bfloat16>(p, a->head_dim, pl.nt, stream);
+  else status = run_kv4<__half>(p, a->head_dim, pl.nt, stream);
+  if (status != TB200_OK) return status;
+  return launch_cache_combine(p, a->dtype, a->head_dim, pl.nt, stream);
 }
 
 size_t workspace_bytes(const tb200_cache_attn_args* a, bool kv4) {
@@ -843,6 +705,11 @@ size_t workspace_bytes(const tb200_cache_attn_args* a, bool kv4) {
 }
 
 }  // namespace
+
+int launch_cache_combine(const CacheAttnParams& p, int dtype, int head_dim, int nt, cudaStream_t stream) {
+  return dtype == TB200_BF16 ? launch_combine<__nv_bfloat16>(p, head_dim, nt, stream) : launch_combine<__half>(p, head_dim, nt, stream);
+}
+
 }  // namespace tb200
 
 using namespace tb200;

@@ -1,0 +1,219 @@
+// What the decode kernels over caches (attn_cache.cu: 4 bits, attn_win.cu: 16 bits) share: the line of key tiles and how it
+// is dealt out over the CTAs, and the merging of partial results.
+//
+//   unit     (sequence, kv head, R query rows): the rows of a unit are (new token, query head of the group) pairs, so
+//            that a cache row is read once for all query heads that share it.
+//   line     the key tiles of all units, one after the other, dealt out in equal stretches over the CTAs (each computes
+//            the line's layout from kv_lens itself): long and short sequences load the SMs evenly, with no host knowledge
+//            of the lengths.  A unit that lies within one CTA's stretch is finished there; the others leave a partial
+//            result (accumulator, maximum, sum) per stretch, which cache_combine_kernel merges in the order of the keys.
+//   warp     takes every fourth tile of a stretch.
+#pragma once
+
+#include <math.h>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace tb200 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 8.f;   // the exponent reference of a row moves only when its maximum has grown by more than 2^kSlack
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+
+struct CacheAttnParams {
+  int B, S, Hq, Hkv, group, cache_len, window, sinks;
+  int row_tiles;             // units per (sequence, kv head) at most
+  float scale_log2;
+  const uint8_t* q;
+  uint8_t* o;
+  long long qs[3], os[3];
+  const int32_t* kv_lens;
+  const int32_t* q_rows;
+  const uint8_t *k_codes, *v_codes, *k_meta, *v_meta;
+  float* part_o;             // (2 grid, R, D)
+  float* part_ml;            // (2 grid, R, 2)
+  int4* split;               // (grid): the unit that begins in a stretch and goes on behind it: sequence, kv head, row tile, stretches it lies in (0: none)
+  int stretches;             // CTAs of the decode kernel
+  int* err;
+  long long wait_limit;
+};
+
+// What a sequence asks for.
+struct Seq {
+  int n, r;                  // positions, new rows
+  int few;                   // first positions that stay visible, below the window
+  int sink_tiles, win_tile;  // tiles [0, sink_tiles) and from win_tile on
+  int tiles;                 // tiles of a unit
+  int units;                 // units of the sequence: kv heads x row tiles
+};
+__device__ __forceinline__ Seq load_seq(const CacheAttnParams& p, int b, int tile, int unit_rows) {
+  Seq s;
+  s.n = max(0, min(__ldg(p.kv_lens + b), p.cache_len));
+  s.r = p.q_rows ? max(0, min(__ldg(p.q_rows + b), p.S)) : p.S;
+  const int low = p.window > 0 ? max(0, s.n - s.r - p.window + 1) : 0;
+  s.few = min(p.sinks, low);
+  s.win_tile = low / tile;
+  s.sink_tiles = min((s.few + tile - 1) / tile, s.win_tile);
+  s.tiles = max(1, s.sink_tiles + (s.n + tile - 1) / tile - s.win_tile);   // a sequence without keys: one masked tile writes the zeros
+  s.units = s.r > 0 ? p.Hkv * ((s.r * p.group + unit_rows - 1) / unit_rows) : 0;
+  return s;
+}
+
+// The line of all tiles: its length, and how it is dealt out.  Every lane of a warp calls these and gets the same.
+struct Line {
+  int total;    // tiles of all units
+  int per;      // tiles of a stretch
+  int seq;      // the sequence in which position x lies
+  int base;     // the line's position of that sequence's first tile
+};
+// x is the first position of stretch `stretch` (behind the line's end: seq and base are not set).
+__device__ __forceinline__ Line walk_line(const CacheAttnParams& p, int tile, int unit_rows, int min_tiles, int stretch) {
+  const int lane = static_cast<int>(lane_id());
+  Line ln;
+  ln.seq = ln.base = 0;
+  int sum = 0, own = 0, total = 0;
+  auto scan = [&](int b0) {   // inclusive sums over 32 sequences
+    const int b = b0 + lane;
+    own = 0;
+    if (b < p.B) {
+      const Seq s = load_seq(p, b, tile, unit_rows);
+      own = s.tiles * s.units;
+    }
+    sum = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+  };
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    scan(b0);
+    total += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  ln.total = total;
+  ln.per = max((total + p.stretches - 1) / p.stretches, min_tiles);
+  const int x = ln.per * stretch;
+  if (x >= total) return ln;
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    if (p.B > 32) scan(b0);   // else the sums are still there
+    const unsigned hit = __ballot_sync(0xffffffffu, before + sum > x);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      ln.seq = b0 + l;
+      ln.base = before + __shfl_sync(0xffffffffu, sum - own, l);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return ln;
+}
+
+// One segment: the part of a unit that lies in this CTA's stretch.
+struct Segment {
+  int b, h, rt;              // sequence, kv head, row tile
+  int v0, v1;                // tiles of the unit
+  int n_rows;                // query rows of the (sequence, kv head)
+};
+// The CTA's walk along its stretch.
+struct Walk {
+  Line ln;
+  Seq sq;
+  int x, x_end;              // positions on the line: of the current segment, of the stretch's end
+  int base, b;               // the line's position of the sequence's first tile; the sequence
+  __device__ __forceinline__ bool begin(const CacheAttnParams& p, int tile, int unit_rows, int min_tiles) {   // false: nothing to do
+    ln = walk_line(p, tile, unit_rows, min_tiles, blockIdx.x);
+    x = ln.per * static_cast<int>(blockIdx.x);
+    x_end = min(x + ln.per, ln.total);
+    if (x >= x_end) {
+      if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return false;
+    }
+    base = ln.base;
+    b = ln.seq;
+    sq = load_seq(p, b, tile, unit_rows);
+    return true;
+  }
+  __device__ __forceinline__ Segment segment(const CacheAttnParams& p, int tile, int unit_rows) {
+    while (x >= base + sq.tiles * sq.units) {
+      base += sq.tiles * sq.units;
+      sq = load_seq(p, ++b, tile, unit_rows);
+    }
+    Segment s;
+    const int unit = (x - base) / sq.tiles;
+    s.v0 = x - base - unit * sq.tiles;
+    s.v1 = min(sq.tiles, s.v0 + x_end - x);
+    const int rts = sq.units / p.Hkv;
+    s.b = b;
+    s.h = unit / rts;
+    s.rt = unit - s.h * rts;
+    s.n_rows = sq.r * p.group;
+    return s;
+  }
+  __device__ __forceinline__ int tile_of(int v) const { return v < sq.sink_tiles ? v : sq.win_tile + v - sq.sink_tiles; }
+};
+
+// Shared memory in which the warps leave their shares of a segment.
+template <int D, int NT> struct MergeSmem {
+  static constexpr int kR = 8 * NT;
+  static constexpr int kPitch = D + 4;                       // floats per row: 4 keep the rows' banks apart
+  static constexpr int kMlOff = kWarps * kR * kPitch * 4;    // float2 [warps][R] behind float [warps][R][pitch]
+  static constexpr int kBytes = kMlOff + kWarps * kR * 8;
+};
+// The four warps' shares in a fixed order: into o where the unit lies in this stretch altogether, else into the stretch's
+// partial results.  Called by the whole CTA, with the shares written and a barrier behind them.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void merge_segment(const CacheAttnParams& p, const uint8_t* smem, const Walk& wk, const Segment& sg) {
+  using M = MergeSmem<D, NT>;
+  constexpr int R = M::kR;
+  const bool whole = sg.v0 == 0 && sg.v1 == wk.sq.tiles;
+  if (threadIdx.x == 0 && wk.x + sg.v1 - sg.v0 >= wk.x_end)   // the stretch's last segment
+    p.split[blockIdx.x] = make_int4(sg.b, sg.h, sg.rt, sg.v0 == 0 && !whole ? (wk.x + wk.sq.tiles - 1) / wk.ln.per - static_cast<int>(blockIdx.x) + 1 : 0);
+  const float* mall = reinterpret_cast<const float*>(smem);
+  const float2* mlall = reinterpret_cast<const float2*>(smem + M::kMlOff);
+  const int slot_out = 2 * blockIdx.x + (sg.v0 == 0 ? 1 : 0);
+  for (int i = threadIdx.x; i < R * D / 4; i += kThreads) {
+    const int m = i / (D / 4), d = (i % (D / 4)) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, mlall[w * R + m].x);
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 ml = mlall[w * R + m];
+      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+      const float4 a = *reinterpret_cast<const float4*>(mall + (w * R + m) * M::kPitch + d);
+      sum = fmaf(f, ml.y, sum);
+      acc.x = fmaf(f, a.x, acc.x); acc.y = fmaf(f, a.y, acc.y); acc.z = fmaf(f, a.z, acc.z); acc.w = fmaf(f, a.w, acc.w);
+    }
+    if (whole) {
+      const int mr = sg.rt * R + m;
+      if (mr < sg.n_rows) {
+        const float inv = sum > 0.f ? 1.f / sum : sum;   // 0: the row sees nothing; NaN stays
+        const int tok = mr / p.group;
+        T* op = reinterpret_cast<T*>(p.o) + sg.b * p.os[0] + (sg.h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + d;
+        *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
+      }
+    } else {
+      *reinterpret_cast<float4*>(p.part_o + (static_cast<long long>(slot_out) * R + m) * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot_out) * R + m) * 2) = make_float2(top, sum);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// attn_cache.cu
+int launch_cache_combine(const CacheAttnParams& p, int dtype, int head_dim, int nt, cudaStream_t stream);
+// attn_win.cu: the decode kernel over 16-bit caches, in a ChainScope; p.stretches as cache16_stretches says
+int launch_cache16(const CacheAttnParams& p, const tb200_cache_attn_args& a, int nt, cudaStream_t stream);
+int cache16_stretches(int nt, int num_sms);
+
+}  // namespace tb200
