@@ -20,10 +20,13 @@
 // (issued after P_j V_j) cannot overwrite P_j early, and an arrival on s_full also means the previous P V is done.
 // The first P V of an item overwrites O, so it waits until the output warpgroup has read the previous item's O (o_free).
 //
-// SEQ instances (launch_attn_fwd_seq) serve caches with per-sequence lengths and a sliding window: an item's key tiles are
-// those of the first positions that stay visible and those from the window of its first query to its last query; rows of
-// V that no query of the item sees are cleared in shared memory before they meet a probability of 0, because a cache may
-// hold anything there.
+// SEQ instances (launch_attn_fwd_seq) serve caches with per-sequence lengths and a sliding window.  An item's keys are laid
+// out on a line of their own: the first positions that stay visible (rounded up to sixteen), then at once the positions
+// from the window of the item's first query to its last query.  Tiles are cut from that line, so that neither a window that
+// begins inside a tile nor a handful of first positions costs a tile; the tile in which the two meet is fetched in boxes of
+// sixteen keys.  (With tiles at multiples of 128 and a tile for the first positions, 4000 queries under a window of 1000:
+// 105 us.)  Rows of V that no query of the item sees are cleared in shared memory before they meet a probability of 0,
+// because a cache may hold anything there.
 //
 // One thread owns one query row.  (Two threads per row were measured slower on B200 -- 0.418 ms against 0.353 ms on
 // the Llama-3-8B B8 S2048 prefill: the row-max exchange costs more than the extra warps hide -- and so was a variant
@@ -79,6 +82,7 @@ __device__ __forceinline__ int fdiv(int n, const FastDiv& f) {
 
 struct Attn2Params {
   CUtensorMap map_q, map_k, map_v, map_o;
+  CUtensorMap map_k16, map_v16;  // SEQ: the same caches in boxes of 16 keys
   int B, S, Hq, Hkv, past, kv_len, causal;
   int n_blocks;      // blocks of 256 queries
   int n_items;       // n_blocks * kv_splits * Hq * B
@@ -105,20 +109,14 @@ struct Item {
   int j_begin;   // first key tile of this share
   int nt[2];     // key tiles of each query tile within the share (0: nothing to do)
   int nt_max;
-  // SEQ: positions and new rows of the sequence; the keys some query of the item sees are those up to `last` that are not
-  // in [few, low); tile j of the item is key tile j below sink_tiles, then from win_tile on
-  int past, rows, last, few, low, sink_tiles, win_tile;
+  // SEQ: the sequence's new rows and the position of the first; the item's line: place x is key x below `few`, no key from
+  // there to `head` (a multiple of 16, or 0: nothing is left out), from there key x + gap, up to place `last`
+  int past, rows, few, head, gap, last;
 };
-
-template <bool SEQ> __device__ __forceinline__ int key_tile(const Item& it, int j) {   // j: tile of the share
-  const int v = it.j_begin + j;
-  if constexpr (SEQ) return v < it.sink_tiles ? v : it.win_tile + v - it.sink_tiles;
-  return v;
-}
 
 template <bool SEQ> __device__ __forceinline__ Item decode_item(const Attn2Params& p, int i) {
   Item it;
-  it.past = it.rows = it.last = it.few = it.low = it.sink_tiles = it.win_tile = 0;
+  it.past = it.rows = it.few = it.head = it.gap = it.last = 0;
   it.nt[0] = it.nt[1] = it.nt_max = 0;
   it.q0 = it.hq = it.b = it.hkv = it.sp = it.j_begin = 0;
   if (i >= p.n_items) return it;
@@ -134,16 +132,17 @@ template <bool SEQ> __device__ __forceinline__ Item decode_item(const Attn2Param
     const int n = max(0, min(__ldg(p.kv_lens + it.b), p.cache_len));
     it.rows = p.q_rows ? max(0, min(__ldg(p.q_rows + it.b), p.S)) : p.S;
     it.past = n - it.rows;   // negative: the first rows stand before the first position and see nothing
-    it.low = p.window > 0 ? max(0, it.past + it.q0 - p.window + 1) : 0;
-    it.few = min(p.sinks, it.low);
-    it.win_tile = it.low / BKV;
-    it.sink_tiles = min((it.few + BKV - 1) / BKV, it.win_tile);
+    const int low = p.window > 0 ? max(0, it.past + it.q0 - p.window + 1) : 0;
+    const bool apart = low > p.sinks;   // else the line is simply the sequence
+    it.few = p.sinks;
+    it.head = apart ? (p.sinks + 15) & ~15 : 0;
+    it.gap = apart ? low - it.head : 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int q0t = it.q0 + t * BQ;
       if (q0t >= it.rows) continue;
-      it.last = it.past + min(q0t + BQ, it.rows) - 1;
-      it.nt[t] = it.sink_tiles + max(0, it.last) / BKV + 1 - it.win_tile;   // without a visible key: one masked tile makes the zeros
+      it.last = it.past + min(q0t + BQ, it.rows) - 1 - it.gap;
+      it.nt[t] = max(0, it.last) / BKV + 1;   // without a visible key (last < 0): one masked tile makes the zeros
     }
   } else
 #pragma unroll
@@ -269,9 +268,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
           uint8_t* dst = smem + (is_v ? L::kVOff : L::kKOff) + st * L::kTile;
 #pragma unroll
           for (int dc = 0; dc < D / 64; ++dc) {
-            if constexpr (SEQ)
-              tma_load_4d(dst + dc * (BKV * 128), is_v ? &p.map_v : &p.map_k, full, dc * 64, key_tile<SEQ>(it, j) * BKV, it.hkv, it.b);
-            else
+            if constexpr (SEQ) {
+              const int x0 = (it.j_begin + j) * BKV;
+              if (x0 < it.head && x0 + BKV > it.head) {   // both kinds of keys
+#pragma unroll 1
+                for (int x = x0; x < x0 + BKV; x += 16)
+                  tma_load_4d(dst + dc * (BKV * 128) + (x - x0) * 128, is_v ? &p.map_v16 : &p.map_k16, full, dc * 64, x < it.head ? x : x + it.gap, it.hkv, it.b);
+              } else {
+                tma_load_4d(dst + dc * (BKV * 128), is_v ? &p.map_v : &p.map_k, full, dc * 64, x0 < it.head ? x0 : x0 + it.gap, it.hkv, it.b);
+              }
+            } else
               tma_load_3d(dst + dc * (BKV * 128), is_v ? &p.map_v : &p.map_k, full, dc * 64, (it.j_begin + j) * BKV,
                           it.b * p.Hkv + it.hkv);
           }
@@ -362,12 +368,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
       for (int j = 0; ok && j < cur.nt_max; ++j) {
         if (!mbar_wait(&v_full[vpos & 1], (vpos >> 1) & 1, ctx, 405)) { ok = false; break; }
         if constexpr (SEQ) {  // clear the rows of V that no query of the item sees
-          const int k0 = key_tile<SEQ>(cur, j) * BKV;
-          if (k0 + BKV - 1 > cur.last || (k0 < cur.low && k0 + BKV - 1 >= cur.few)) {
+          const int x0 = (cur.j_begin + j) * BKV;
+          if (x0 + BKV - 1 > cur.last || (x0 < cur.head && cur.few < cur.head)) {
             uint8_t* vt = smem + L::kVOff + (vpos & 1) * L::kTile;
             for (int i = lane; i < BKV * 8; i += 32) {
-              const int key = k0 + (i >> 3);
-              if (key > cur.last || (key < cur.low && key >= cur.few)) {
+              const int x = x0 + (i >> 3);
+              if (x > cur.last || (x < cur.head && x >= cur.few)) {
 #pragma unroll
                 for (int dc = 0; dc < D / 64; ++dc) *reinterpret_cast<uint4*>(vt + dc * (BKV * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
               }
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
     bool ok = true;
 
     for (int i = blockIdx.x; ok && i < p.n_items; i += gridDim.x) {
-      int my_nt, k_first, key_limit, win_low = 0, sink_tiles = 0, win_skip = 0;
+      int my_nt, k_first, key_limit, win_low = 0, few = 0;   // SEQ: all of them places on the item's line
       {  // only what the key loop needs stays live through it; the item is decoded again for the output addresses
         const Item it = decode_item<SEQ>(p, i);
         my_nt = t == 0 ? it.nt[0] : it.nt[1];
@@ -428,21 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
         const int qi = it.q0 + t * BQ + r_in;
         key_limit = p.causal ? min(p.past + qi, p.kv_len - 1) : p.kv_len - 1;
         if constexpr (SEQ) {
-          k_first = it.j_begin;
-          key_limit = it.past + qi;
-          win_low = p.window > 0 ? key_limit - p.window + 1 : 0;
-          sink_tiles = it.sink_tiles;
-          win_skip = it.win_tile - it.sink_tiles;
+          key_limit = it.past + qi - it.gap;
+          win_low = p.window > 0 ? max(it.head, key_limit - p.window + 1) : 0;
+          few = it.few;
         }
       }
       float m_use = -INFINITY, l = 0.f;
 
       for (int j = 0; j < my_nt; ++j, ++s_count) {
-        int k0 = k_first + j * BKV;
-        if constexpr (SEQ) {
-          const int v = k_first + j;
-          k0 = (v < sink_tiles ? v : v + win_skip) * BKV;
-        }
+        const int k0 = k_first + j * BKV;
         if (!mbar_wait(&s_full[t], s_count & 1, ctx, 408)) { ok = false; break; }
         tc_fence_after();
         uint32_t s[BKV];
@@ -456,10 +456,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
             if (k0 + c > key_limit) s[c] = 0xff800000u;  // -inf
         }
         if constexpr (SEQ) {
-          if (k0 < win_low && k0 + BKV - 1 >= p.sinks) {  // these touch the keys before the window
+          if (k0 < win_low && k0 + BKV - 1 >= few) {  // these touch the keys before the window
 #pragma unroll
             for (int c = 0; c < BKV; ++c)
-              if (k0 + c < win_low && k0 + c >= p.sinks) s[c] = 0xff800000u;
+              if (k0 + c < win_low && k0 + c >= few) s[c] = 0xff800000u;
           }
         }
         float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
@@ -835,19 +835,23 @@ int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
   p.part_ml = a.part_ml;
   p.err = st->err_word;
   p.wait_limit = wait_limit_cycles();
-  auto map4 = [&](CUtensorMap* map, const void* base, int rows, int heads, const int64_t (&st3)[3]) {   // strides: batch, head, row
+  auto map4 = [&](CUtensorMap* map, const void* base, int rows, int heads, const int64_t (&st3)[3], uint32_t box_rows) {   // strides: batch, head, row
     const uint64_t d = static_cast<uint64_t>(a.D);
     const uint64_t dims[4] = {d, static_cast<uint64_t>(rows), static_cast<uint64_t>(heads), static_cast<uint64_t>(a.B)};
     const uint64_t strides[3] = {rows > 1 ? static_cast<uint64_t>(st3[2]) * 2 : d * 2, heads > 1 ? static_cast<uint64_t>(st3[1]) * 2 : d * 2,
                                  a.B > 1 ? static_cast<uint64_t>(st3[0]) * 2 : d * 2};
-    const uint32_t box[4] = {64, BQ, 1, 1};
+    const uint32_t box[4] = {64, box_rows, 1, 1};
     return make_tensor_map(map, base, 4, dims, strides, box);
   };
   static_assert(BQ == BKV, "one box size for queries and keys");
-  if ((status = map4(&p.map_q, a.q, a.S, a.Hq, a.q_stride)) != TB200_OK) return status;
-  if ((status = map4(&p.map_k, a.k_cache, a.cache_len, a.Hkv, a.k_stride)) != TB200_OK) return status;
-  if ((status = map4(&p.map_v, a.v_cache, a.cache_len, a.Hkv, a.v_stride)) != TB200_OK) return status;
-  if ((status = map4(&p.map_o, a.o, a.S, a.Hq, a.o_stride)) != TB200_OK) return status;
+  if ((status = map4(&p.map_q, a.q, a.S, a.Hq, a.q_stride, BQ)) != TB200_OK) return status;
+  if ((status = map4(&p.map_k, a.k_cache, a.cache_len, a.Hkv, a.k_stride, BQ)) != TB200_OK) return status;
+  if ((status = map4(&p.map_v, a.v_cache, a.cache_len, a.Hkv, a.v_stride, BQ)) != TB200_OK) return status;
+  if (a.sinks > 0) {
+    if ((status = map4(&p.map_k16, a.k_cache, a.cache_len, a.Hkv, a.k_stride, 16)) != TB200_OK) return status;
+    if ((status = map4(&p.map_v16, a.v_cache, a.cache_len, a.Hkv, a.v_stride, 16)) != TB200_OK) return status;
+  }
+  if ((status = map4(&p.map_o, a.o, a.S, a.Hq, a.o_stride, BQ)) != TB200_OK) return status;
   return finish_launch<true>(p, a.dtype, a.D, st, stream);
 }
 
