@@ -318,8 +318,8 @@ int tb200_kv_compact(const tb200_kv_compact_args* args, void* stream);
  * (batch, kv head, position).
  *
  * A group is 64 consecutive values x of a row.  lo = min x, s = (max x - min x) / 15, computed in
- * fp32 and rounded to the cache's 16-bit type; c = the whole number nearest to (x - lo) / s in [0, 15]
- * (halves to even; 0 where s is 0).  The group stands for lo + c * s.  A group that holds an infinity
+ * fp32 and rounded to the cache's 16-bit type; c = the whole number nearest to the fp32 quotient
+ * (x - lo) / s, at most 15 (halves to even; 0 where s is 0).  The group stands for lo + c * s.  A group that holds an infinity
  * or a NaN, or whose max - min is not finite in fp32, stands for NaN throughout.
  *   codes  (B, Hkv, cache_len, D/2) bytes: element 2i in the low, 2i+1 in the high four bits of byte i
  *   meta   (B, Hkv, cache_len, D/64, 2) of the cache's type: s, lo

@@ -56,22 +56,23 @@ template <typename T> struct SmallScale;
 template <> struct SmallScale<__half> { static constexpr float value = 1.9073486328125e-06f; };        // 2^-19: steps of 2^-24
 template <> struct SmallScale<__nv_bfloat16> { static constexpr float value = 1.17549435e-38f; };      // 2^-126
 
-// Codes of eight values of a group.  The quotient is formed in fp32 with an approximate reciprocal (off by less than 1e-5)
-// and rounded by adding 1.5 * 2^23, which leaves the code in the sum's low bits; where one of the eight quotients lies
-// within 1e-4 of a border between two codes, all are formed again in 64 bits.
+// Codes of eight values of a group: round((x - lo) / s), halves to even.  bf16 values lie on few places, so a quotient is
+// exactly k + 1/2 in about one group of eight out of twenty, and it has to come out as just that: the approximate quotient
+// q0 = t inv is followed by one Newton step, q = q0 + (t - q0 s) inv with the remainder exact in a fused multiply-add
+// (P. Markstein, IBM J. Res. Dev. 34, 1990), which is the correctly rounded quotient.  Adding 1.5 * 2^23 rounds q to a
+// whole number and leaves the code in the sum's low bits.
+// (Approximate quotients re-examined in 64 bits wherever one lay next to a border took twice as long.)
 template <typename T>
 __device__ __forceinline__ uint32_t encode8(const uint32_t (&w)[4], float lo, float s) {
   constexpr float kMagic = 12582912.f;
   const float inv = __fdividef(1.f, s);
-  const float2 nlo = make_float2(-lo, -lo), inv2 = make_float2(inv, inv), magic = make_float2(kMagic, kMagic), nmagic = make_float2(-kMagic, -kMagic);
+  const float2 nlo = make_float2(-lo, -lo), inv2 = make_float2(inv, inv), ns = make_float2(-s, -s), magic = make_float2(kMagic, kMagic);
   uint32_t word = 0;
-  float worst = 0.f;
 #pragma unroll
   for (int i = 3; i >= 0; --i) {
-    const float2 q = __fmul2_rn(__fadd2_rn(Pack2<T>::unpack(w[i]), nlo), inv2);
-    const float2 r = __fadd2_rn(q, magic);
-    const float2 d = __fadd2_rn(__fadd2_rn(r, nmagic), make_float2(-q.x, -q.y));
-    worst = fmaxf(worst, fmaxf(fabsf(d.x), fabsf(d.y)));
+    const float2 t = __fadd2_rn(Pack2<T>::unpack(w[i]), nlo);
+    const float2 q0 = __fmul2_rn(t, inv2);
+    const float2 r = __fadd2_rn(__ffma2_rn(__ffma2_rn(q0, ns, t), inv2, q0), magic);
     word = word * 16 + __float_as_uint(r.y);
     word = word * 16 + __float_as_uint(r.x);
   }
@@ -79,15 +80,13 @@ __device__ __forceinline__ uint32_t encode8(const uint32_t (&w)[4], float lo, fl
   constexpr uint32_t kBits = 0x4b400000u;
   constexpr uint32_t kCarry = kBits * 0x11111111u;
   word -= kCarry;
-  if (!(worst < 0.4999f) || !(s >= SmallScale<T>::value)) {
+  if (!(s >= SmallScale<T>::value)) {   // 0, NaN, or so coarse that a quotient may pass 15.5
     word = 0;
     if (s > 0.f) {
 #pragma unroll 1
       for (int i = 7; i >= 0; --i) {
         const float2 x2 = Pack2<T>::unpack(i < 2 ? w[0] : i < 4 ? w[1] : i < 6 ? w[2] : w[3]);
-        const double x = (i & 1) ? x2.y : x2.x;
-        const double q = (x - static_cast<double>(lo)) / static_cast<double>(s);
-        word = word * 16 + static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0));
+        word = word * 16 + static_cast<uint32_t>(fminf(rintf(__fdiv_rn(((i & 1) ? x2.y : x2.x) - lo, s)), 15.f));
       }
     }
   }
@@ -124,6 +123,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const __grid_const
     }
 #pragma unroll
     for (int k = 0; k < kPerThread; ++k) {
+      if (!__any_sync(0xffffffffu, live[k])) continue;   // a warp's rows of which none is meant
       const long long crow = bh * p.cache_len + start + (rb * kPerThread + k) * kRows + r_in;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
