@@ -3,8 +3,7 @@
 // held as the codes c = round((x - lo) / s) and the pair (s, lo) in the cache's 16-bit type, and stands for lo + c s.
 // 64 values take 32 + 4 bytes: 4.5 bits per value.
 //
-// Bound: HBM.  One row of D = 128 moves 256 + 72 bytes.  Eight lanes share a group (eight values, one 16-byte access
-// each), so that minimum and maximum are three shuffles.
+// Bound: HBM (one row of D = 128 moves 256 + 72 bytes); appending also by the instructions per value.
 #include "common.cuh"
 #include "internal.h"
 #include "kv4.cuh"
@@ -14,13 +13,14 @@ namespace tb200 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 4;   // rows of a thread: eight loads in flight
+constexpr int kPerThread = 2;   // rows of a thread: eight 16-byte loads in flight
 
 struct RowsParams {
   const int32_t* start;
   const int32_t* n_rows;
-  int start_all, rows, heads, cache_len, row_blocks;
-  long long units;          // batch * heads * row_blocks
+  int start_all, rows, heads, cache_len;
+  long long n_bh;           // batch * heads
+  long long units;          // of rows, times n_bh
   uint8_t* x[2];            // k, v
   long long stride[2][3];   // elements: batch, head, row
   uint8_t* codes[2];
@@ -93,56 +93,86 @@ __device__ __forceinline__ uint32_t encode8(const uint32_t (&w)[4], float lo, fl
   return word;
 }
 
-// A unit is kPerThread * kThreads / (D / 8) rows of one (sequence, head), k and v.
+// Four lanes share a group: lane l holds the eight values from 8 l on and the eight from 32 + 8 l on, so that every access of
+// the four is one stretch of 64 bytes and what is done once per group costs half of what eight lanes spend on it.
+// A unit is kUnitRows rows of one (sequence, head), k and v; units next to one another are of different sequences, so that
+// short sequences leave no CTA without work.
+template <int D> struct RowsShape {
+  static constexpr int kLanes = D / 16;                // lanes per row
+  static constexpr int kRows = kThreads / kLanes;      // rows side by side
+  static constexpr int kUnitRows = kRows * kPerThread;
+};
+struct Unit {
+  long long bh;
+  int b, h, row0, n, start;
+};
+__device__ __forceinline__ Unit find_unit(const RowsParams& p, long long u, int unit_rows) {
+  Unit x;
+  const long long rb = u / p.n_bh;
+  x.bh = u - rb * p.n_bh;
+  x.b = static_cast<int>(x.bh / p.heads);
+  x.h = static_cast<int>(x.bh - static_cast<long long>(x.b) * p.heads);
+  x.row0 = static_cast<int>(rb) * unit_rows;
+  x.n = p.n_rows ? min(p.n_rows[x.b], p.rows) : p.rows;
+  x.start = p.start ? p.start[x.b] : p.start_all;
+  return x;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const __grid_constant__ RowsParams p) {
-  constexpr int kLanes = D / 8;                 // lanes per row
-  constexpr int kRows = kThreads / kLanes;      // rows side by side
-  const int tid = threadIdx.x;
-  const int r_in = tid / kLanes, c8 = tid % kLanes;
+  using S = RowsShape<D>;
+  const int r_in = threadIdx.x / S::kLanes, lane = threadIdx.x % S::kLanes;
+  const int chunk = (lane >> 2) * 8 + (lane & 3);   // of eight values; the other one is four further on
   for (long long u = blockIdx.x; u < p.units; u += gridDim.x) {
-    const long long bh = u / p.row_blocks;
-    const int rb = static_cast<int>(u - bh * p.row_blocks);
-    const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<long long>(b) * p.heads);
-    const int n = p.n_rows ? min(p.n_rows[b], p.rows) : p.rows;
-    const int start = p.start ? p.start[b] : p.start_all;
-    if (rb * kPerThread * kRows >= n) continue;   // the whole CTA
-    uint4 raw[kPerThread][2];
+    const Unit x = find_unit(p, u, S::kUnitRows);
+    if (x.row0 >= x.n) continue;   // the whole CTA
+    uint4 raw[kPerThread][2][2];
     bool live[kPerThread];
 #pragma unroll
     for (int k = 0; k < kPerThread; ++k) {
-      const int row = (rb * kPerThread + k) * kRows + r_in;
-      const long long pos = static_cast<long long>(start) + row;
-      live[k] = row < n && pos >= 0 && pos < p.cache_len;
+      const int row = x.row0 + k * S::kRows + r_in;
+      const long long pos = static_cast<long long>(x.start) + row;
+      live[k] = row < x.n && pos >= 0 && pos < p.cache_len;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        raw[k][x] = make_uint4(0u, 0u, 0u, 0u);
-        if (live[k])
-          raw[k][x] = __ldcs(reinterpret_cast<const uint4*>(p.x[x] + 2 * (b * p.stride[x][0] + h * p.stride[x][1] + row * p.stride[x][2] + c8 * 8)));
+      for (int w = 0; w < 2; ++w) {
+        raw[k][w][0] = raw[k][w][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (live[k]) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.x[w] + 2 * (x.b * p.stride[w][0] + x.h * p.stride[w][1] + row * p.stride[w][2])) + chunk;
+          raw[k][w][0] = __ldcs(src);
+          raw[k][w][1] = __ldcs(src + 4);
+        }
       }
     }
 #pragma unroll
     for (int k = 0; k < kPerThread; ++k) {
       if (!__any_sync(0xffffffffu, live[k])) continue;   // a warp's rows of which none is meant
-      const long long crow = bh * p.cache_len + start + (rb * kPerThread + k) * kRows + r_in;
+      const long long crow = x.bh * p.cache_len + x.start + x.row0 + k * S::kRows + r_in;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t w[4] = {raw[k][x].x, raw[k][x].y, raw[k][x].z, raw[k][x].w};
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t v[2][4] = {{raw[k][w][0].x, raw[k][w][0].y, raw[k][w][0].z, raw[k][w][0].w},
+                                  {raw[k][w][1].x, raw[k][w][1].y, raw[k][w][1].z, raw[k][w][1].w}};
         // minimum, and minus the maximum as the minimum of the negated values, side by side in one register
-        uint32_t lo2 = min2_nan<T>(min2_nan<T>(w[0], w[1]), min2_nan<T>(w[2], w[3]));
-        uint32_t hi2 = min2_nan<T>(min2_nan<T>(w[0] ^ 0x80008000u, w[1] ^ 0x80008000u), min2_nan<T>(w[2] ^ 0x80008000u, w[3] ^ 0x80008000u));
-        uint32_t both = min2_nan<T>(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
+        uint32_t lo2 = v[0][0], hi2 = v[0][0] ^ 0x80008000u;
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, o));
+        for (int i = 1; i < 8; ++i) {
+          lo2 = min2_nan<T>(lo2, v[i >> 2][i & 3]);
+          hi2 = min2_nan<T>(hi2, v[i >> 2][i & 3] ^ 0x80008000u);
+        }
+        uint32_t both = min2_nan<T>(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
+        both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, 1));
+        both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, 2));
         const float2 f = Pack2<T>::unpack(both);
         const float lo = f.x, range = __fsub_rn(-f.y, f.x);
         const bool odd = !(range < INFINITY);    // an infinity or a NaN among the 64, or a range past fp32
         const uint32_t sb = odd ? 0x7fffu : Bits<T>::rn(__fdiv_rn(range, 15.f));
         const uint32_t lb = odd ? 0x7fffu : (both & 0xffffu);
-        const uint32_t word = encode8<T>(w, lo, odd ? 0.f : Bits<T>::f(sb));
+        const float s = odd ? 0.f : Bits<T>::f(sb);
+        const uint32_t word0 = encode8<T>(v[0], lo, s), word1 = encode8<T>(v[1], lo, s);
         if (live[k]) {
-          *reinterpret_cast<uint32_t*>(p.codes[x] + crow * (D / 2) + c8 * 4) = word;
-          if ((c8 & 7) == 0) *reinterpret_cast<uint32_t*>(p.meta[x] + (crow * (D / 64) + c8 / 8) * 4) = sb | (lb << 16);
+          uint32_t* c = reinterpret_cast<uint32_t*>(p.codes[w] + crow * (D / 2)) + chunk;
+          c[0] = word0;
+          c[4] = word1;
+          if ((lane & 3) == 0) *reinterpret_cast<uint32_t*>(p.meta[w] + (crow * (D / 64) + (lane >> 2)) * 4) = sb | (lb << 16);
         }
       }
     }
@@ -152,47 +182,47 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const __grid_const
 // SEEN: only the positions that some query row of the sequence sees (a prompt's attention reads the 16-bit rows next).
 template <typename T, int D, bool SEEN>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constant__ RowsParams p) {
-  constexpr int kLanes = D / 8;
-  constexpr int kRows = kThreads / kLanes;   // rows side by side
+  using S = RowsShape<D>;
   if constexpr (SEEN) pdl_launch_dependents();
-  const int tid = threadIdx.x;
-  const int r_in = tid / kLanes, c8 = tid % kLanes;
+  const int r_in = threadIdx.x / S::kLanes, lane = threadIdx.x % S::kLanes;
+  const int chunk = (lane >> 2) * 8 + (lane & 3);
   for (long long u = blockIdx.x; u < p.units; u += gridDim.x) {
-    const long long bh = u / p.row_blocks;
-    const int rb = static_cast<int>(u - bh * p.row_blocks);
-    const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<long long>(b) * p.heads);
-    const int n = p.n_rows ? min(p.n_rows[b], p.rows) : p.rows;
-    const int start = p.start ? p.start[b] : p.start_all;
+    const Unit x = find_unit(p, u, S::kUnitRows);
+    if (x.row0 >= x.n) continue;
     int low = 0, few = 0;
     if constexpr (SEEN) {
-      const int r = p.q_rows ? max(0, min(p.q_rows[b], p.q_rows_max)) : p.q_rows_max;
-      low = p.window > 0 ? n - r - p.window + 1 : 0;
+      const int r = p.q_rows ? max(0, min(p.q_rows[x.b], p.q_rows_max)) : p.q_rows_max;
+      low = r == 0 ? x.n : p.window > 0 ? x.n - r - p.window + 1 : 0;
       few = r > 0 ? p.sinks : 0;
-      if (r == 0) low = n;
     }
-    uint32_t word[2][kPerThread], m[2][kPerThread];
+    uint32_t word[kPerThread][2][2], m[kPerThread][2];
     bool live[kPerThread];
 #pragma unroll
     for (int k = 0; k < kPerThread; ++k) {
-      const int row = (rb * kPerThread + k) * kRows + r_in;
-      const long long pos = static_cast<long long>(start) + row;
-      live[k] = row < n && pos >= 0 && pos < p.cache_len;
+      const int row = x.row0 + k * S::kRows + r_in;
+      const long long pos = static_cast<long long>(x.start) + row;
+      live[k] = row < x.n && pos >= 0 && pos < p.cache_len;
       if constexpr (SEEN) live[k] = live[k] && (row >= low || row < few);
-      const long long crow = bh * p.cache_len + pos;
+      if (!live[k]) continue;
+      const long long crow = x.bh * p.cache_len + pos;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        word[w][k] = live[k] ? __ldg(reinterpret_cast<const uint32_t*>(p.codes[w] + crow * (D / 2) + c8 * 4)) : 0u;
-        m[w][k] = live[k] ? __ldg(reinterpret_cast<const uint32_t*>(p.meta[w] + (crow * (D / 64) + c8 / 8) * 4)) : 0u;
+        const uint32_t* c = reinterpret_cast<const uint32_t*>(p.codes[w] + crow * (D / 2)) + chunk;
+        word[k][w][0] = __ldcs(c);
+        word[k][w][1] = __ldcs(c + 4);
+        m[k][w] = __ldcs(reinterpret_cast<const uint32_t*>(p.meta[w] + (crow * (D / 64) + (lane >> 2)) * 4));
       }
     }
 #pragma unroll
     for (int k = 0; k < kPerThread; ++k) {
       if (!live[k]) continue;
-      const long long row = (rb * kPerThread + k) * kRows + r_in;
+      const long long row = x.row0 + k * S::kRows + r_in;
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
-        *reinterpret_cast<uint4*>(p.x[w] + 2 * (b * p.stride[w][0] + h * p.stride[w][1] + row * p.stride[w][2] + c8 * 8)) =
-            Kv4Decode<T>::decode8(word[w][k], m[w][k]);
+      for (int w = 0; w < 2; ++w) {
+        uint4* dst = reinterpret_cast<uint4*>(p.x[w] + 2 * (x.b * p.stride[w][0] + x.h * p.stride[w][1] + row * p.stride[w][2])) + chunk;
+        dst[0] = Kv4Decode<T>::decode8(word[k][w][0], m[k][w]);
+        dst[4] = Kv4Decode<T>::decode8(word[k][w][1], m[k][w]);
+      }
     }
   }
 }
@@ -254,9 +284,8 @@ RowsParams rows_params(const tb200_kv4_rows_args& a) {
 
 template <typename T, int D>
 int launch_rows(RowsParams p, int batch, RowsWork work, int num_sms, cudaStream_t stream) {
-  const int unit_rows = kThreads / (D / 8) * kPerThread;
-  p.row_blocks = (p.rows + unit_rows - 1) / unit_rows;
-  p.units = static_cast<long long>(batch) * p.heads * p.row_blocks;
+  p.n_bh = static_cast<long long>(batch) * p.heads;
+  p.units = p.n_bh * ((p.rows + RowsShape<D>::kUnitRows - 1) / RowsShape<D>::kUnitRows);
   const long long most = static_cast<long long>(num_sms) * 8;
   const dim3 grid(static_cast<unsigned>(p.units < most ? p.units : most));
   cudaError_t e;
