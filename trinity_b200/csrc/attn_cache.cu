@@ -17,6 +17,8 @@
 //            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 #include <math.h>
 
+#include <type_traits>
+
 #include "cache_line.cuh"
 
 namespace tb200 {
@@ -46,11 +48,14 @@ template <typename T, int NG> __device__ __forceinline__ void load_meta(const ui
   }
 }
 
-constexpr int kTile = 64;     // keys of a tile
-constexpr int kStages = 2;
-constexpr int kMinTiles = kWarps;
-
+// Tile (keys), stages of a warp's ring and CTAs per SM of an instance.  An unrolled tile of 64 keys gives the scheduler the
+// most to interleave; with two column blocks at D = 128 its registers no longer fit and 32 keys are faster (42 against 60 us
+// for five rows of 16 sequences), as 64 keys are elsewhere (24 long sequences: 55 against 59 us).
+template <int D, int NT> struct DecShape {
+  static constexpr int kTile = D == 128 && NT == 2 ? 32 : 64, kStages = 2, kCtas = D == 64 && NT == 1 ? 3 : 2;
+};
 template <int D, int NT> struct DecSmem {
+  static constexpr int kTile = DecShape<D, NT>::kTile, kStages = DecShape<D, NT>::kStages;
   static constexpr int kR = 8 * NT;
   static constexpr int kCodes = kTile * D / 2;             // bytes of one tile's codes
   static constexpr int kMeta = kTile * (D / 64) * 4;
@@ -64,10 +69,10 @@ template <int D, int NT> struct DecSmem {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel(const __grid_constant__ CacheAttnParams p) {
+__global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode_kernel(const __grid_constant__ CacheAttnParams p) {
   using L = DecSmem<D, NT>;
   constexpr int NG = D / 64;
-  constexpr int R = L::kR;
+  constexpr int R = L::kR, kTile = L::kTile, kStages = L::kStages;
   // fp16 outputs are worth the centred codes (see above); bf16's own rounding is sixteen times coarser than what they gain
   constexpr bool kCentre = !IsBf16<T>::value;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -86,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
   __syncthreads();
 
   Walk wk;
-  if (!wk.begin(p, kTile, R, kMinTiles)) return;
+  if (!wk.begin(p, kTile, R, kWarps)) return;
   uint32_t used = 0;    // tiles this warp has taken through its ring
   bool ok = true;
 
@@ -218,187 +223,194 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) cache_decode_kernel
       // every key of the tile visible to every row of the sequence?
       const bool full = k0 + kTile - 1 <= sq.n - sq.r && (p.window == 0 || k0 > sq.n - 1 - p.window || k0 + kTile - 1 < p.sinks);
 
-      float s[kTile / 16][NT][4];   // scores without the row's factor cf: keys g (rows 2t, 2t + 1) and g + 8 of sixteen; then probabilities
-#pragma unroll
-      for (int sp = 0; sp < kTile / 16; ++sp) {
-        // MMA row (slot) 2a + e of eight is key a + 4 e: the four lanes of a column pair then read neighbouring rows
-        const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
-        float acc[NT][NG][4];
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          const uint2 w0 = *reinterpret_cast<const uint2*>(kc + key0 * (D / 2) + gr * 32 + t * 8);
-          const uint2 w1 = *reinterpret_cast<const uint2*>(kc + key1 * (D / 2) + gr * 32 + t * 8);
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint32_t x0 = ((ks & 2) ? w0.y : w0.x) >> ((ks & 1) * 8), x1 = ((ks & 2) ? w1.y : w1.x) >> ((ks & 1) * 8);
-            const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (ks == 0) mma_f16_first(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
-              else mma_f16(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
-            }
-          }
-        }
-        float2 m0[NG], m1[NG];
-        load_meta<T, NG>(km + key0 * (NG * 4), m0);
-        load_meta<T, NG>(km + key1 * (NG * 4), m1);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float y0 = m0[0].y * qs[nt][0][c], y1 = m1[0].y * qs[nt][0][c];
-            if constexpr (NG == 2) {
-              y0 = fmaf(m0[1].y, qs[nt][1][c], y0);
-              y1 = fmaf(m1[1].y, qs[nt][1][c], y1);
-            }
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-              y0 = fmaf(m0[gr].x, acc[nt][gr][c], y0);
-              y1 = fmaf(m1[gr].x, acc[nt][gr][2 + c], y1);
-            }
-            s[sp][nt][c] = y0;
-            s[sp][nt][2 + c] = y1;
-            if (!full) {
-              const int a = k0 + key0, d = k0 + key1, pos = cpos[nt][c];
-              if (!(a <= pos && (p.window == 0 || a > pos - p.window || a < p.sinks))) s[sp][nt][c] = -INFINITY;
-              if (!(d <= pos && (p.window == 0 || d > pos - p.window || d < p.sinks))) s[sp][nt][2 + c] = -INFINITY;
-            }
-          }
-      }
-
-      // ---- running maximum of the scores and of the V scales: what a thread sees of either decides whether the warp has
-      //      to look closer
-      uint32_t big = 0;
-#pragma unroll
-      for (int i = 0; i < kTile / 32; ++i) {
-        const int key = i * 32 + lane;
-        bool alive = true;
-        if (!full) {
-          const int a = k0 + key;
-          alive = a < sq.n && (p.window == 0 || a > sq.n - sq.r - p.window || a < p.sinks);
-        }
-        float2 mv[NG];
-        load_meta<T, NG>(vm + key * (NG * 4), mv);
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          const uint32_t u = __float_as_uint(mv[gr].x);
-          if (alive && u < 0x7f800000u) big = max(big, u);
-        }
-      }
-      float top[NT][2];
-      bool grown = static_cast<int>(big >> 23) > ev;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
-#pragma unroll
-          for (int sp = 1; sp < kTile / 16; ++sp) x = max3(x, s[sp][nt][c], s[sp][nt][2 + c]);
-          top[nt][c] = x * cf[nt][c];
-          grown |= top[nt][c] > mx[nt][c] + kSlack;
-        }
-      if (__any_sync(0xffffffffu, grown)) {
-        const int ev_new = max(ev, static_cast<int>(__reduce_max_sync(0xffffffffu, big) >> 23));
-        const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 + ev - ev_new, 0)) << 23);   // 2^(ev - ev_new)
-        ev = ev_new;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float m_new = top[nt][c];
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
-            m_new = fmaxf(m_new, mx[nt][c]);
-            const float a = (m_new == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - m_new)) * shrink;
-            mx[nt][c] = m_new;
-            shift[nt][c] = static_cast<float>(132 - ev) - (m_new == -INFINITY ? 0.f : m_new);   // 5 - (ev - 127): with p <= 2^kSlack, p s < 2^14
-            l[nt][c] *= a;
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-              z[nt][gr][c] *= a;
-              if (kCentre) o8[nt][gr][c] *= a;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                o[nt][gr][i][c] *= a;
-                o[nt][gr][i][2 + c] *= a;
-              }
-            }
-          }
-      }
-
-#pragma unroll
-      for (int sp = 0; sp < kTile / 16; ++sp)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            s[sp][nt][c] = fast_exp2(fmaf(s[sp][nt][c], cf[nt][c], shift[nt][c]));
-            s[sp][nt][2 + c] = fast_exp2(fmaf(s[sp][nt][2 + c], cf[nt][c], shift[nt][c]));
-            l[nt][c] += s[sp][nt][c] + s[sp][nt][2 + c];
-          }
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
-        // a tile's products are summed from zero and then added in fp32: the tensor core's additions truncate, and over
-        // thousands of keys with codes of one sign that would add up
-        float part[NT][4][4], part8[NT][4];
+      // A tile that every row sees altogether is one stretch of code without a branch (what the scheduler can interleave ends
+      // at a branch: with the masks behind branches of their own, the loop took a fifth longer).
+      auto tile = [&](auto whole_tile) {
+        constexpr bool full = decltype(whole_tile)::value;
+        float s[kTile / 16][NT][4];   // scores without the row's factor cf: keys g (rows 2t, 2t + 1) and g + 8 of sixteen; then probabilities
 #pragma unroll
         for (int sp = 0; sp < kTile / 16; ++sp) {
+          // MMA row (slot) 2a + e of eight is key a + 4 e: the four lanes of a column pair then read neighbouring rows
           const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
-          const float2 m0 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key0 * NG + gr) * 4));
-          const float2 m1 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key1 * NG + gr) * 4));
-          const float c0 = kCentre ? fmaf(8.f, m0.x, m0.y) : m0.y, c1 = kCentre ? fmaf(8.f, m1.x, m1.y) : m1.y;
-          uint32_t pf[NT][2];
+          float acc[NT][NG][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float* e = s[sp][nt];
-            float w[4] = {e[0] * m0.x, e[1] * m0.x, e[2] * m1.x, e[3] * m1.x};
-            if (full) {
-              z[nt][gr][0] = fmaf(e[2], c1, fmaf(e[0], c0, z[nt][gr][0]));
-              z[nt][gr][1] = fmaf(e[3], c1, fmaf(e[1], c0, z[nt][gr][1]));
-            } else {   // what a row does not see may hold anything: 0 * inf and 0 * NaN must not arise
+          for (int gr = 0; gr < NG; ++gr) {
+            const uint2 w0 = *reinterpret_cast<const uint2*>(kc + key0 * (D / 2) + gr * 32 + t * 8);
+            const uint2 w1 = *reinterpret_cast<const uint2*>(kc + key1 * (D / 2) + gr * 32 + t * 8);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if (e[i] > 0.f) z[nt][gr][i & 1] = fmaf(e[i], i < 2 ? c0 : c1, z[nt][gr][i & 1]);
-                else w[i] = 0.f;
+            for (int ks = 0; ks < 4; ++ks) {
+              const uint32_t x0 = ((ks & 2) ? w0.y : w0.x) >> ((ks & 1) * 8), x1 = ((ks & 2) ? w1.y : w1.x) >> ((ks & 1) * 8);
+              const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (ks == 0) mma_f16_first(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
+                else mma_f16(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][ks][0], qf[nt][gr][ks][1]);
               }
             }
-            pf[nt][0] = transpose8x8(Pack2<__half>::pack(w[0], w[1]));
-            pf[nt][1] = transpose8x8(Pack2<__half>::pack(w[2], w[3]));
-            if constexpr (kCentre) {
-              if (sp == 0) mma_f16_first(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
-              else mma_f16(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
-            }
           }
-          // MMA columns 2t, 2t+1 (and 2t+8, 2t+9) of V^T are keys t, t + 4 (and t + 8, t + 12); row g of the four row tiles
-          // holds elements 8 g + {0, 2, 4, 6}, row g + 8 the odd ones
-          const uint8_t* vp = vc + (sp * 16 + t) * (D / 2) + gr * 32 + g * 4;
-          const uint32_t wa = *reinterpret_cast<const uint32_t*>(vp), wb = *reinterpret_cast<const uint32_t*>(vp + 4 * (D / 2));
-          const uint32_t wc = *reinterpret_cast<const uint32_t*>(vp + 8 * (D / 2)), wd = *reinterpret_cast<const uint32_t*>(vp + 12 * (D / 2));
-          const uint32_t xl = __byte_perm(wa, wb, 0x5410), xh = __byte_perm(wa, wb, 0x7632);
-          const uint32_t yl = __byte_perm(wc, wd, 0x5410), yh = __byte_perm(wc, wd, 0x7632);
+          float2 m0[NG], m1[NG];
+          load_meta<T, NG>(km + key0 * (NG * 4), m0);
+          load_meta<T, NG>(km + key1 * (NG * 4), m1);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t x0 = ((i & 2) ? xh : xl) >> ((i & 1) * 8), y0 = ((i & 2) ? yh : yl) >> ((i & 1) * 8);
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (sp == 0) mma_f16_first(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
-              else mma_f16(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+            for (int c = 0; c < 2; ++c) {
+              float y0 = m0[0].y * qs[nt][0][c], y1 = m1[0].y * qs[nt][0][c];
+              if constexpr (NG == 2) {
+                y0 = fmaf(m0[1].y, qs[nt][1][c], y0);
+                y1 = fmaf(m1[1].y, qs[nt][1][c], y1);
+              }
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr) {
+                y0 = fmaf(m0[gr].x, acc[nt][gr][c], y0);
+                y1 = fmaf(m1[gr].x, acc[nt][gr][2 + c], y1);
+              }
+              s[sp][nt][c] = y0;
+              s[sp][nt][2 + c] = y1;
+              if (!full) {
+                const int a = k0 + key0, d = k0 + key1, pos = cpos[nt][c];
+                if (!(a <= pos && (p.window == 0 || a > pos - p.window || a < p.sinks))) s[sp][nt][c] = -INFINITY;
+                if (!(d <= pos && (p.window == 0 || d > pos - p.window || d < p.sinks))) s[sp][nt][2 + c] = -INFINITY;
+              }
             }
+        }
+
+        // ---- running maximum of the scores and of the V scales: what a thread sees of either decides whether the warp has
+        //      to look closer
+        uint32_t big = 0;
+#pragma unroll
+        for (int i = 0; i < kTile / 32; ++i) {
+          const int key = i * 32 + lane;
+          bool alive = true;
+          if (!full) {
+            const int a = k0 + key;
+            alive = a < sq.n && (p.window == 0 || a > sq.n - sq.r - p.window || a < p.sinks);
+          }
+          float2 mv[NG];
+          load_meta<T, NG>(vm + key * (NG * 4), mv);
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            const uint32_t u = __float_as_uint(mv[gr].x);
+            if (alive && u < 0x7f800000u) big = max(big, u);
           }
         }
+        float top[NT][2];
+        bool grown = static_cast<int>(big >> 23) > ev;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            if constexpr (kCentre) o8[nt][gr][c] += part8[nt][c];
+            float x = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
+#pragma unroll
+            for (int sp = 1; sp < kTile / 16; ++sp) x = max3(x, s[sp][nt][c], s[sp][nt][2 + c]);
+            top[nt][c] = x * cf[nt][c];
+            grown |= top[nt][c] > mx[nt][c] + kSlack;
+          }
+        if (__any_sync(0xffffffffu, grown)) {
+          const int ev_new = max(ev, static_cast<int>(__reduce_max_sync(0xffffffffu, big) >> 23));
+          const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 + ev - ev_new, 0)) << 23);   // 2^(ev - ev_new)
+          ev = ev_new;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float m_new = top[nt][c];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
+              m_new = fmaxf(m_new, mx[nt][c]);
+              const float a = (m_new == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - m_new)) * shrink;
+              mx[nt][c] = m_new;
+              shift[nt][c] = static_cast<float>(132 - ev) - (m_new == -INFINITY ? 0.f : m_new);   // 5 - (ev - 127): with p <= 2^kSlack, p s < 2^14
+              l[nt][c] *= a;
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr) {
+                z[nt][gr][c] *= a;
+                if (kCentre) o8[nt][gr][c] *= a;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  o[nt][gr][i][c] *= a;
+                  o[nt][gr][i][2 + c] *= a;
+                }
+              }
+            }
+        }
+
+#pragma unroll
+        for (int sp = 0; sp < kTile / 16; ++sp)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              s[sp][nt][c] = fast_exp2(fmaf(s[sp][nt][c], cf[nt][c], shift[nt][c]));
+              s[sp][nt][2 + c] = fast_exp2(fmaf(s[sp][nt][2 + c], cf[nt][c], shift[nt][c]));
+              l[nt][c] += s[sp][nt][c] + s[sp][nt][2 + c];
+            }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          // a tile's products are summed from zero and then added in fp32: the tensor core's additions truncate, and over
+          // thousands of keys with codes of one sign that would add up
+          float part[NT][4][4], part8[NT][4];
+#pragma unroll
+          for (int sp = 0; sp < kTile / 16; ++sp) {
+            const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
+            const float2 m0 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key0 * NG + gr) * 4));
+            const float2 m1 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key1 * NG + gr) * 4));
+            const float c0 = kCentre ? fmaf(8.f, m0.x, m0.y) : m0.y, c1 = kCentre ? fmaf(8.f, m1.x, m1.y) : m1.y;
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const float* e = s[sp][nt];
+              float w[4] = {e[0] * m0.x, e[1] * m0.x, e[2] * m1.x, e[3] * m1.x};
+              if (full) {
+                z[nt][gr][0] = fmaf(e[2], c1, fmaf(e[0], c0, z[nt][gr][0]));
+                z[nt][gr][1] = fmaf(e[3], c1, fmaf(e[1], c0, z[nt][gr][1]));
+              } else {   // what a row does not see may hold anything: 0 * inf and 0 * NaN must not arise
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if (e[i] > 0.f) z[nt][gr][i & 1] = fmaf(e[i], i < 2 ? c0 : c1, z[nt][gr][i & 1]);
+                  else w[i] = 0.f;
+                }
+              }
+              pf[nt][0] = transpose8x8(Pack2<__half>::pack(w[0], w[1]));
+              pf[nt][1] = transpose8x8(Pack2<__half>::pack(w[2], w[3]));
+              if constexpr (kCentre) {
+                if (sp == 0) mma_f16_first(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
+                else mma_f16(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
+              }
+            }
+            // MMA columns 2t, 2t+1 (and 2t+8, 2t+9) of V^T are keys t, t + 4 (and t + 8, t + 12); row g of the four row tiles
+            // holds elements 8 g + {0, 2, 4, 6}, row g + 8 the odd ones
+            const uint8_t* vp = vc + (sp * 16 + t) * (D / 2) + gr * 32 + g * 4;
+            const uint32_t wa = *reinterpret_cast<const uint32_t*>(vp), wb = *reinterpret_cast<const uint32_t*>(vp + 4 * (D / 2));
+            const uint32_t wc = *reinterpret_cast<const uint32_t*>(vp + 8 * (D / 2)), wd = *reinterpret_cast<const uint32_t*>(vp + 12 * (D / 2));
+            const uint32_t xl = __byte_perm(wa, wb, 0x5410), xh = __byte_perm(wa, wb, 0x7632);
+            const uint32_t yl = __byte_perm(wc, wd, 0x5410), yh = __byte_perm(wc, wd, 0x7632);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              o[nt][gr][i][c] += part[nt][i][c];
-              o[nt][gr][i][2 + c] += part[nt][i][2 + c];
+              const uint32_t x0 = ((i & 2) ? xh : xl) >> ((i & 1) * 8), y0 = ((i & 2) ? yh : yl) >> ((i & 1) * 8);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (sp == 0) mma_f16_first(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+                else mma_f16(part[nt][i], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, pf[nt][0], pf[nt][1]);
+              }
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if constexpr (kCentre) o8[nt][gr][c] += part8[nt][c];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                o[nt][gr][i][c] += part[nt][i][c];
+                o[nt][gr][i][2 + c] += part[nt][i][2 + c];
+              }
             }
           }
         }
-      }
+      };
+      if (full) tile(std::true_type{});
+      else tile(std::false_type{});
       __syncwarp();   // every lane has read the slot
       if (v + kStages * kWarps < v1) issue(v + kStages * kWarps, slot);
       ++used;
@@ -552,11 +564,13 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   return TB200_OK;
 }
 
-// CTAs of the decode kernel that an SM holds: by shared memory (72 KB with 8 query rows, 90 KB with 16 at D = 128)
-constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-
 // New rows per sequence up to which a call runs a decode kernel.
 constexpr int kDecodeTokens4 = 32, kDecodeTokens16 = 32;
+
+int kv4_ctas(int head_dim, int nt) {
+  if (head_dim == 128) return nt == 1 ? DecShape<128, 1>::kCtas : DecShape<128, 2>::kCtas;
+  return nt == 1 ? DecShape<64, 1>::kCtas : DecShape<64, 2>::kCtas;
+}
 
 struct AttnPlan {
   bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
@@ -582,7 +596,7 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
     return pl;
   }
   pl.nt = rows <= 8 ? 1 : 2;
-  pl.stretches = kv4 ? num_sms * ctas_per_sm(pl.nt) : cache16_stretches(pl.nt, num_sms);
+  pl.stretches = kv4 ? num_sms * kv4_ctas(a->head_dim, pl.nt) : cache16_stretches(pl.nt, num_sms);
   pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * a->head_dim * sizeof(float), 256);
   pl.part_ml = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * 2 * sizeof(float), 256);
   pl.split = align_up(static_cast<size_t>(pl.stretches) * sizeof(int4), 256);
