@@ -450,16 +450,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
         for (int c = 0; c < BKV / 32; ++c) tmem_ld_x32(tmem_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         tmem_wait_ld();
 
-        if (k0 + BKV - 1 > key_limit) {  // these columns touch the causal diagonal or the end of the keys
-#pragma unroll
-          for (int c = 0; c < BKV; ++c)
-            if (k0 + c > key_limit) s[c] = 0xff800000u;  // -inf
-        }
         if constexpr (SEQ) {
-          if (k0 < win_low && k0 + BKV - 1 >= few) {  // these touch the keys before the window
+          if (k0 + BKV - 1 > key_limit || (k0 < win_low && k0 + BKV - 1 >= few)) {
+            // the columns [win_low, key_limit] and those below `few`, as one bit each: a test of a bit per column instead of
+            // two or four comparisons (most tiles of a short window are cut on one side or the other)
+            auto below = [](int n) -> uint32_t { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; };
+#pragma unroll
+            for (int w = 0; w < BKV / 32; ++w) {
+              const int c0 = k0 + w * 32;
+              const uint32_t seen = (below(key_limit + 1 - c0) & ~below(win_low - c0)) | (below(few - c0) & below(key_limit + 1 - c0));
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!((seen >> c) & 1u)) s[w * 32 + c] = 0xff800000u;  // -inf
+            }
+          }
+        } else {
+          if (k0 + BKV - 1 > key_limit) {  // these columns touch the causal diagonal or the end of the keys
 #pragma unroll
             for (int c = 0; c < BKV; ++c)
-              if (k0 + c < win_low && k0 + c >= few) s[c] = 0xff800000u;
+              if (k0 + c > key_limit) s[c] = 0xff800000u;  // -inf
           }
         }
         float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
@@ -689,8 +698,13 @@ __global__ void attn_combine_kernel(const float* __restrict__ part_o, const floa
       const bool on = s < splits;
       ml[s] = on ? __ldcg(reinterpret_cast<const float2*>(part_ml + (s * rows + row) * 2)) : make_float2(-INFINITY, 0.f);
       const float* ps = part_o + ((on ? s : 0) * rows + row) * D + lane * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) po[s][i] = on ? __ldcg(ps + i) : 0.f;
+      if constexpr (V == 4) {
+        const float4 f = on ? __ldcg(reinterpret_cast<const float4*>(ps)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        po[s][0] = f.x; po[s][1] = f.y; po[s][2] = f.z; po[s][3] = f.w;
+      } else {
+        const float2 f = on ? __ldcg(reinterpret_cast<const float2*>(ps)) : make_float2(0.f, 0.f);
+        po[s][0] = f.x; po[s][1] = f.y;
+      }
     }
     float m = -INFINITY;
 #pragma unroll
