@@ -244,6 +244,23 @@ def test_attn_window(shape, dt):
     check_rows(out, want, q, k.double(), v.double(), lens, rows, d ** -0.5, dt)
 
 
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("size,flat", [(1e30, True), (1e30, False), (3e7, True), (1.0, True), (1e-5, False), (1e-12, False), (1e-12, True)])
+def test_kv4_attn_values_of_any_size(size, flat, rows):
+    """V scales and minima far from 1, or no scale at all (a group of equal values); keys whose scale is 0."""
+    dt, b, hq, hkv, d, length, n = torch.bfloat16, 1, 4, 1, 128, 512, 500
+    cache = filled_cache(b, hkv, length, d, dt, 7)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    v = torch.randn(b, hkv, length, 2 if flat else d, generator=g, device=DEV).repeat_interleave(64 if flat else 1, -1) * size
+    k = torch.randn(b, hkv, length, 2, generator=g, device=DEV).repeat_interleave(64, -1)
+    ops.kv4_append(cache, k.to(dt), v.to(dt), 0)
+    q = torch.randn(b, hq, rows, d, generator=g, device=DEV).to(dt)
+    out = torch.full((b, hq, rows, d), 7.0, dtype=dt, device=DEV)
+    ops.kv4_attn(q, cache, ints([n]), sm_scale=0.1, out=out)
+    k64, v64 = values64(cache, "k"), values64(cache, "v")
+    check_rows(out, attention64(q, k64, v64, [n], [rows], 0, 0, 0.1), q, k64, v64, [n], [rows], 0.1, dt)
+
+
 @pytest.mark.parametrize("s", [1, 4, 130])
 @pytest.mark.parametrize("kv4", [True, False])
 def test_rows_nobody_sees_may_hold_anything(kv4, s):

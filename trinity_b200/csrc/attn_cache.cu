@@ -14,6 +14,9 @@
 //            keeps the largest p s below 2^14), the second sum is fp32, and for fp16 outputs the 8 is taken out with the SAME
 //            rounded probabilities (an MMA against a constant 8), so that the rounding error is that of centred codes, 2.6
 //            times smaller; bf16 outputs are rounded sixteen times more coarsely than that and do without.
+//   H = 2    four query rows or fewer (one token of up to four query heads per kv head): they fill half of the eight columns,
+//            so columns 4 to 7 repeat them, and each column takes the probabilities of half the keys: a thread then has two
+//            scores of sixteen keys to work on instead of four, and a row comes in two shares like those of two warps.
 //            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 #include <math.h>
 
@@ -51,12 +54,12 @@ template <typename T, int NG> __device__ __forceinline__ void load_meta(const ui
 // Tile (keys), stages of a warp's ring and CTAs per SM of an instance.  An unrolled tile of 64 keys gives the scheduler the
 // most to interleave; with two column blocks at D = 128 its registers no longer fit and 32 keys are faster (42 against 60 us
 // for five rows of 16 sequences), as 64 keys are elsewhere (24 long sequences: 55 against 59 us).
-template <int D, int NT> struct DecShape {
-  static constexpr int kTile = D == 128 && NT == 2 ? 32 : 64, kStages = 2, kCtas = D == 64 && NT == 1 ? 3 : 2;
+template <int D, int NT, int H> struct DecShape {
+  static constexpr int kTile = D == 128 && NT == 2 ? 32 : 64, kStages = 2, kCtas = NT == 1 && (D == 64 || H == 2) ? 3 : 2;
 };
-template <int D, int NT> struct DecSmem {
-  static constexpr int kTile = DecShape<D, NT>::kTile, kStages = DecShape<D, NT>::kStages;
-  static constexpr int kR = 8 * NT;
+template <int D, int NT, int H> struct DecSmem {
+  static constexpr int kTile = DecShape<D, NT, H>::kTile, kStages = DecShape<D, NT, H>::kStages;
+  static constexpr int kR = 8 * NT / H;                    // query rows of a unit
   static constexpr int kCodes = kTile * D / 2;             // bytes of one tile's codes
   static constexpr int kMeta = kTile * (D / 64) * 4;
   static constexpr int kStage = 2 * (kCodes + kMeta);      // K codes, V codes, K meta, V meta
@@ -68,9 +71,10 @@ template <int D, int NT> struct DecSmem {
   static constexpr int kTotal = kBarOff + kWarps * kStages * 8 + 16;
 };
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode_kernel(const __grid_constant__ CacheAttnParams p) {
-  using L = DecSmem<D, NT>;
+template <typename T, int D, int NT, int H>
+__global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_decode_kernel(const __grid_constant__ CacheAttnParams p) {
+  using L = DecSmem<D, NT, H>;
+  constexpr int KN = 2 / H;   // keys of sixteen whose scores a thread works on
   constexpr int NG = D / 64;
   constexpr int R = L::kR, kTile = L::kTile, kStages = L::kStages;
   // fp16 outputs are worth the centred codes (see above); bf16's own rounding is sixteen times coarser than what they gain
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
     int cpos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int m = rt * R + nt * 8 + g;
+      const int m = rt * R + (nt * 8 + g) % R;
       const bool live = m < n_rows;
       const int tok = live ? m / p.group : 0;
       const int hq = h * p.group + (live ? m - tok * p.group : 0);
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
         cf[nt][c] = fmaxf(__shfl_sync(0xffffffffu, down, src) * (p.scale_log2 * 16777216.f), 1.17549435e-38f);
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[gr], src) * u * 5.9604644775390625e-8f;   // 2^-24
-        const int mc = rt * R + nt * 8 + 2 * t + c;
+        const int mc = rt * R + (nt * 8 + 2 * t + c) % R;
         cpos[nt][c] = mc < n_rows ? sq.n - sq.r + mc / p.group : -1;
       }
     }
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
         mx[nt][c] = -INFINITY;
         l[nt][c] = shift[nt][c] = 0.f;
       }
-    int ev = 30;   // biased exponent of the largest V scale so far
+    int ev = 60;   // biased exponent of the largest V scale so far, at least this
 
     for (int v = v0 + warp; v < v1; v += kWarps) {
       const uint32_t slot = used % kStages;
@@ -227,7 +231,8 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
       // at a branch: with the masks behind branches of their own, the loop took a fifth longer).
       auto tile = [&](auto whole_tile) {
         constexpr bool full = decltype(whole_tile)::value;
-        float s[kTile / 16][NT][4];   // scores without the row's factor cf: keys g (rows 2t, 2t + 1) and g + 8 of sixteen; then probabilities
+        // scores without the row's factor cf, then probabilities: rows 2t and 2t + 1, keys g and (H == 1) g + 8 of sixteen
+        float s[kTile / 16][NT][2 * KN];
 #pragma unroll
         for (int sp = 0; sp < kTile / 16; ++sp) {
           // MMA row (slot) 2a + e of eight is key a + 4 e: the four lanes of a column pair then read neighbouring rows
@@ -248,36 +253,31 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
               }
             }
           }
-          float2 m0[NG], m1[NG];
-          load_meta<T, NG>(km + key0 * (NG * 4), m0);
-          load_meta<T, NG>(km + key1 * (NG * 4), m1);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int j = 0; j < KN; ++j) {
+            const int key = H == 2 ? key0 + (t >> 1) * 8 : key0 + j * 8;
+            float2 m[NG];
+            load_meta<T, NG>(km + key * (NG * 4), m);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float y0 = m0[0].y * qs[nt][0][c], y1 = m1[0].y * qs[nt][0][c];
-              if constexpr (NG == 2) {
-                y0 = fmaf(m0[1].y, qs[nt][1][c], y0);
-                y1 = fmaf(m1[1].y, qs[nt][1][c], y1);
-              }
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int gr = 0; gr < NG; ++gr) {
-                y0 = fmaf(m0[gr].x, acc[nt][gr][c], y0);
-                y1 = fmaf(m1[gr].x, acc[nt][gr][2 + c], y1);
+              for (int c = 0; c < 2; ++c) {
+                float y = m[0].y * qs[nt][0][c];
+                if constexpr (NG == 2) y = fmaf(m[1].y, qs[nt][1][c], y);
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) y = fmaf(m[gr].x, H == 2 ? (t < 2 ? acc[nt][gr][c] : acc[nt][gr][2 + c]) : acc[nt][gr][2 * j + c], y);
+                if (!full) {
+                  const int a = k0 + key, pos = cpos[nt][c];
+                  if (!(a <= pos && (p.window == 0 || a > pos - p.window || a < p.sinks))) y = -INFINITY;
+                }
+                s[sp][nt][2 * j + c] = y;
               }
-              s[sp][nt][c] = y0;
-              s[sp][nt][2 + c] = y1;
-              if (!full) {
-                const int a = k0 + key0, d = k0 + key1, pos = cpos[nt][c];
-                if (!(a <= pos && (p.window == 0 || a > pos - p.window || a < p.sinks))) s[sp][nt][c] = -INFINITY;
-                if (!(d <= pos && (p.window == 0 || d > pos - p.window || d < p.sinks))) s[sp][nt][2 + c] = -INFINITY;
-              }
-            }
+          }
         }
 
         // ---- running maximum of the scores and of the V scales: what a thread sees of either decides whether the warp has
         //      to look closer
-        uint32_t big = 0;
+        int big = 0;
 #pragma unroll
         for (int i = 0; i < kTile / 32; ++i) {
           const int key = i * 32 + lane;
@@ -290,24 +290,27 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
           load_meta<T, NG>(vm + key * (NG * 4), mv);
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr) {
-            const uint32_t u = __float_as_uint(mv[gr].x);
-            if (alive && u < 0x7f800000u) big = max(big, u);
+            const int u = __float_as_int(mv[gr].x), w = __float_as_int(fabsf(mv[gr].y));
+            // lo counts where it is 2^60 times the scale: the sums of p lo have to stay in fp32 too
+            if (alive && u < 0x7f800000 && w < 0x7f800000) big = max(big, max(u, w - (60 << 23)));
           }
         }
         float top[NT][2];
-        bool grown = static_cast<int>(big >> 23) > ev;
+        bool grown = (big >> 23) > ev;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(s[0][nt][c], s[0][nt][2 + c]);
+            float x = s[0][nt][c];
 #pragma unroll
-            for (int sp = 1; sp < kTile / 16; ++sp) x = max3(x, s[sp][nt][c], s[sp][nt][2 + c]);
+            for (int sp = 0; sp < kTile / 16; ++sp)
+#pragma unroll
+              for (int j = 0; j < KN; ++j) x = fmaxf(x, s[sp][nt][2 * j + c]);
             top[nt][c] = x * cf[nt][c];
             grown |= top[nt][c] > mx[nt][c] + kSlack;
           }
         if (__any_sync(0xffffffffu, grown)) {
-          const int ev_new = max(ev, static_cast<int>(__reduce_max_sync(0xffffffffu, big) >> 23));
+          const int ev_new = max(ev, __reduce_max_sync(0xffffffffu, big) >> 23);
           const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 + ev - ev_new, 0)) << 23);   // 2^(ev - ev_new)
           ev = ev_new;
 #pragma unroll
@@ -340,11 +343,12 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              s[sp][nt][c] = fast_exp2(fmaf(s[sp][nt][c], cf[nt][c], shift[nt][c]));
-              s[sp][nt][2 + c] = fast_exp2(fmaf(s[sp][nt][2 + c], cf[nt][c], shift[nt][c]));
-              l[nt][c] += s[sp][nt][c] + s[sp][nt][2 + c];
-            }
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int j = 0; j < KN; ++j) {
+                s[sp][nt][2 * j + c] = fast_exp2(fmaf(s[sp][nt][2 * j + c], cf[nt][c], shift[nt][c]));
+                l[nt][c] += s[sp][nt][2 * j + c];
+              }
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
           // a tile's products are summed from zero and then added in fp32: the tensor core's additions truncate, and over
@@ -352,27 +356,37 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
           float part[NT][4][4], part8[NT][4];
 #pragma unroll
           for (int sp = 0; sp < kTile / 16; ++sp) {
-            const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4, key1 = key0 + 8;
-            const float2 m0 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key0 * NG + gr) * 4));
-            const float2 m1 = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + (key1 * NG + gr) * 4));
-            const float c0 = kCentre ? fmaf(8.f, m0.x, m0.y) : m0.y, c1 = kCentre ? fmaf(8.f, m1.x, m1.y) : m1.y;
+            const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4 + (H == 2 ? (t >> 1) * 8 : 0);
+            float2 m[KN];
+            float lo8[KN];
+#pragma unroll
+            for (int j = 0; j < KN; ++j) {
+              m[j] = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + ((key0 + j * 8) * NG + gr) * 4));
+              lo8[j] = kCentre ? fmaf(8.f, m[j].x, m[j].y) : m[j].y;
+            }
             uint32_t pf[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const float* e = s[sp][nt];
-              float w[4] = {e[0] * m0.x, e[1] * m0.x, e[2] * m1.x, e[3] * m1.x};
-              if (full) {
-                z[nt][gr][0] = fmaf(e[2], c1, fmaf(e[0], c0, z[nt][gr][0]));
-                z[nt][gr][1] = fmaf(e[3], c1, fmaf(e[1], c0, z[nt][gr][1]));
-              } else {   // what a row does not see may hold anything: 0 * inf and 0 * NaN must not arise
+              float w[2 * KN];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if (e[i] > 0.f) z[nt][gr][i & 1] = fmaf(e[i], i < 2 ? c0 : c1, z[nt][gr][i & 1]);
-                  else w[i] = 0.f;
+              for (int j = 0; j < KN; ++j)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const float e = s[sp][nt][2 * j + c];
+                  w[2 * j + c] = e * m[j].x;
+                  if (full) z[nt][gr][c] = fmaf(e, lo8[j], z[nt][gr][c]);
+                  // what a row does not see may hold anything: 0 * inf and 0 * NaN must not arise
+                  else if (e > 0.f) z[nt][gr][c] = fmaf(e, lo8[j], z[nt][gr][c]);
+                  else w[2 * j + c] = 0.f;
                 }
+              const uint32_t x = transpose8x8(Pack2<__half>::pack(w[0], w[1]));
+              if constexpr (H == 2) {   // columns 0 to 3 take the keys 0 to 7 of sixteen, columns 4 to 7 the others
+                pf[nt][0] = g < 4 ? x : 0u;
+                pf[nt][1] = g < 4 ? 0u : x;
+              } else {
+                pf[nt][0] = x;
+                pf[nt][1] = transpose8x8(Pack2<__half>::pack(w[2 * KN - 2], w[2 * KN - 1]));
               }
-              pf[nt][0] = transpose8x8(Pack2<__half>::pack(w[0], w[1]));
-              pf[nt][1] = transpose8x8(Pack2<__half>::pack(w[2], w[3]));
               if constexpr (kCentre) {
                 if (sp == 0) mma_f16_first(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
                 else mma_f16(part8[nt], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[nt][0], pf[nt][1]);
@@ -419,8 +433,8 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
     // ---- this warp's share of the segment into shared memory: o relative to its own maximum
     __syncthreads();   // every warp is done with its ring
     using M = MergeSmem<D, NT>;
-    float* wm = reinterpret_cast<float*>(smem) + warp * R * M::kPitch;
-    float2* wml = reinterpret_cast<float2*>(smem + M::kMlOff) + warp * R;
+    float* wm = reinterpret_cast<float*>(smem) + warp * M::kR * M::kPitch;
+    float2* wml = reinterpret_cast<float2*>(smem + M::kMlOff) + warp * M::kR;
     const float fe = __uint_as_float(static_cast<uint32_t>(ev - 5) << 23);   // 2^(ev - 127 - 5): out of the accumulators' scale
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -444,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
         }
       }
     __syncthreads();
-    merge_segment<T, D, NT>(p, smem, wk, sg);
+    merge_segment<T, D, NT, H>(p, smem, wk, sg);
     fence_proxy_async_smem();   // the next bulk copies overwrite what was just read and written
     __syncthreads();
     wk.x += v1 - v0;
@@ -455,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT>::kCtas) cache_decode
 // begins in stretch c and goes on behind its end, if there is one; its first part is in slot 2c + 1, the others in the slots
 // 2c' of the stretches c' it covers.  The four warps share the parts; sums are taken in a fixed order.
 constexpr int kCombineThreads = 128, kCombineRows = 4;
-template <typename T, int D, int NT>
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(kCombineThreads) cache_combine_kernel(const __grid_constant__ CacheAttnParams p) {
-  constexpr int R = 8 * NT, V = D / 32;
+  constexpr int V = D / 32;
   extern __shared__ float weights[];                                 // [rows][stretches]
   __shared__ float red[4][kCombineRows][D];
   pdl_launch_dependents();
@@ -567,14 +581,17 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
 // New rows per sequence up to which a call runs a decode kernel.
 constexpr int kDecodeTokens4 = 32, kDecodeTokens16 = 32;
 
-int kv4_ctas(int head_dim, int nt) {
-  if (head_dim == 128) return nt == 1 ? DecShape<128, 1>::kCtas : DecShape<128, 2>::kCtas;
-  return nt == 1 ? DecShape<64, 1>::kCtas : DecShape<64, 2>::kCtas;
+// Query rows of a unit: the smallest form that holds a sequence's rows of one kv head, else as many as there are.  Four rows:
+// see H at cache_decode_kernel.
+int unit_rows_for(int64_t rows, bool kv4) { return kv4 && rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
+int kv4_ctas(int head_dim, int unit_rows) {
+  if (head_dim == 128) return unit_rows == 4 ? DecShape<128, 1, 2>::kCtas : unit_rows == 8 ? DecShape<128, 1, 1>::kCtas : DecShape<128, 2, 1>::kCtas;
+  return unit_rows == 4 ? DecShape<64, 1, 2>::kCtas : unit_rows == 8 ? DecShape<64, 1, 1>::kCtas : DecShape<64, 2, 1>::kCtas;
 }
 
 struct AttnPlan {
   bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
-  int nt = 1;                // decode: MMA column blocks of a unit
+  int unit_rows = 8;         // decode: query rows of a unit
   int stretches = 0;
   int kv_splits = 1;         // prompt
   size_t part_o = 0, part_ml = 0, split = 0, cache16 = 0;   // bytes; cache16: of one of the two caches
@@ -595,10 +612,10 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
     if (kv4) pl.cache16 = align_up(static_cast<size_t>(a->batch) * a->n_kv_heads * a->cache_len * a->head_dim * 2, 256);
     return pl;
   }
-  pl.nt = rows <= 8 ? 1 : 2;
-  pl.stretches = kv4 ? num_sms * kv4_ctas(a->head_dim, pl.nt) : cache16_stretches(pl.nt, num_sms);
-  pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * a->head_dim * sizeof(float), 256);
-  pl.part_ml = align_up(static_cast<size_t>(pl.stretches) * 2 * 8 * pl.nt * 2 * sizeof(float), 256);
+  pl.unit_rows = unit_rows_for(rows, kv4);
+  pl.stretches = kv4 ? num_sms * kv4_ctas(a->head_dim, pl.unit_rows) : cache16_stretches(num_sms);
+  pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * pl.unit_rows * a->head_dim * sizeof(float), 256);
+  pl.part_ml = align_up(static_cast<size_t>(pl.stretches) * 2 * pl.unit_rows * 2 * sizeof(float), 256);
   pl.split = align_up(static_cast<size_t>(pl.stretches) * sizeof(int4), 256);
   return pl;
 }
@@ -624,37 +641,45 @@ CacheAttnParams make_params(const tb200_cache_attn_args* a, const DeviceState* s
   return p;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int H>
 int launch_decode(const CacheAttnParams& p, cudaStream_t stream) {
-  using L = DecSmem<D, NT>;
+  using L = DecSmem<D, NT, H>;
   static bool attr_set[32] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_set[dev & 31]) {
-    if (cudaFuncSetAttribute(cache_decode_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return TB200_ERR_CUDA;
+    if (cudaFuncSetAttribute(cache_decode_kernel<T, D, NT, H>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess)
+      return TB200_ERR_CUDA;
     attr_set[dev & 31] = true;
   }
-  if (launch_chained(cache_decode_kernel<T, D, NT>, dim3(p.stretches), dim3(kThreads), L::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
+  if (launch_chained(cache_decode_kernel<T, D, NT, H>, dim3(p.stretches), dim3(kThreads), L::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
 }
+template <typename T, int D>
+int run_kv4(const CacheAttnParams& p, int unit_rows, cudaStream_t stream) {
+  if (unit_rows == 4) return launch_decode<T, D, 1, 2>(p, stream);
+  return unit_rows == 8 ? launch_decode<T, D, 1, 1>(p, stream) : launch_decode<T, D, 2, 1>(p, stream);
+}
+template <typename T>
+int run_kv4(const CacheAttnParams& p, int head_dim, int unit_rows, cudaStream_t stream) {
+  return head_dim == 128 ? run_kv4<T, 128>(p, unit_rows, stream) : run_kv4<T, 64>(p, unit_rows, stream);
+}
 
-template <typename T, int D, int NT>
+template <typename T, int D, int R>
 int launch_combine(const CacheAttnParams& p, cudaStream_t stream) {
-  if (launch_chained(cache_combine_kernel<T, D, NT>, dim3(p.stretches, 8 * NT / kCombineRows), dim3(kCombineThreads),
+  if (launch_chained(cache_combine_kernel<T, D, R>, dim3(p.stretches, R / kCombineRows), dim3(kCombineThreads),
                      kCombineRows * p.stretches * sizeof(float), stream, p) != cudaSuccess)
     return TB200_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
 }
-template <typename T>
-int launch_combine(const CacheAttnParams& p, int head_dim, int nt, cudaStream_t stream) {
-  if (head_dim == 128) return nt == 1 ? launch_combine<T, 128, 1>(p, stream) : launch_combine<T, 128, 2>(p, stream);
-  return nt == 1 ? launch_combine<T, 64, 1>(p, stream) : launch_combine<T, 64, 2>(p, stream);
+template <typename T, int D>
+int launch_combine(const CacheAttnParams& p, int unit_rows, cudaStream_t stream) {
+  if (unit_rows == 4) return launch_combine<T, D, 4>(p, stream);
+  return unit_rows == 8 ? launch_combine<T, D, 8>(p, stream) : launch_combine<T, D, 16>(p, stream);
 }
-
 template <typename T>
-int run_kv4(const CacheAttnParams& p, int head_dim, int nt, cudaStream_t stream) {
-  if (head_dim == 128) return nt == 1 ? launch_decode<T, 128, 1>(p, stream) : launch_decode<T, 128, 2>(p, stream);
-  return nt == 1 ? launch_decode<T, 64, 1>(p, stream) : launch_decode<T, 64, 2>(p, stream);
+int launch_combine(const CacheAttnParams& p, int head_dim, int unit_rows, cudaStream_t stream) {
+  return head_dim == 128 ? launch_combine<T, 128>(p, unit_rows, stream) : launch_combine<T, 64>(p, unit_rows, stream);
 }
 
 int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, const CacheAttnParams& p, int num_sms, cudaStream_t stream) {
@@ -703,12 +728,12 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   p.split = reinterpret_cast<int4*>(static_cast<uint8_t*>(a->workspace) + pl.part_o + pl.part_ml);
   // positions on the line of tiles are 32-bit numbers
   const int64_t rows = static_cast<int64_t>(a->rows) * p.group;
-  if ((rows / (8 * pl.nt) + 1) * a->n_kv_heads * a->batch * static_cast<double>(a->cache_len / 16 + 2) >= 2147483648.0) return TB200_ERR_UNSUPPORTED;
-  if (!kv4) status = launch_cache16(p, *a, pl.nt, stream);
-  else if (a->dtype == TB200_BF16) status = run_kv4<__nv_bfloat16>(p, a->head_dim, pl.nt, stream);
-  else status = run_kv4<__half>(p, a->head_dim, pl.nt, stream);
+  if ((rows / pl.unit_rows + 1) * a->n_kv_heads * a->batch * static_cast<double>(a->cache_len / 16 + 2) >= 2147483648.0) return TB200_ERR_UNSUPPORTED;
+  if (!kv4) status = launch_cache16(p, *a, pl.unit_rows, stream);
+  else if (a->dtype == TB200_BF16) status = run_kv4<__nv_bfloat16>(p, a->head_dim, pl.unit_rows, stream);
+  else status = run_kv4<__half>(p, a->head_dim, pl.unit_rows, stream);
   if (status != TB200_OK) return status;
-  return launch_cache_combine(p, a->dtype, a->head_dim, pl.nt, stream);
+  return launch_cache_combine(p, a->dtype, a->head_dim, pl.unit_rows, stream);
 }
 
 size_t workspace_bytes(const tb200_cache_attn_args* a, bool kv4) {
@@ -720,8 +745,8 @@ size_t workspace_bytes(const tb200_cache_attn_args* a, bool kv4) {
 
 }  // namespace
 
-int launch_cache_combine(const CacheAttnParams& p, int dtype, int head_dim, int nt, cudaStream_t stream) {
-  return dtype == TB200_BF16 ? launch_combine<__nv_bfloat16>(p, head_dim, nt, stream) : launch_combine<__half>(p, head_dim, nt, stream);
+int launch_cache_combine(const CacheAttnParams& p, int dtype, int head_dim, int unit_rows, cudaStream_t stream) {
+  return dtype == TB200_BF16 ? launch_combine<__nv_bfloat16>(p, head_dim, unit_rows, stream) : launch_combine<__half>(p, head_dim, unit_rows, stream);
 }
 
 }  // namespace tb200

@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_decode16_kernel(const __gri
         }
       }
     __syncthreads();
-    merge_segment<T, D, NT>(p, smem, wk, sg);
+    merge_segment<T, D, NT, 1>(p, smem, wk, sg);
     fence_proxy_async_smem();   // the next copies overwrite what was just read and written
     __syncthreads();
     wk.x += sg.v1 - sg.v0;
@@ -288,9 +288,10 @@ int launch16(const CacheAttnParams& p, const CacheMaps& maps, int head_dim, int 
 
 }  // namespace
 
-int cache16_stretches(int, int num_sms) { return 2 * num_sms; }   // two CTAs per SM: 97 KB of shared memory each
+int cache16_stretches(int num_sms) { return 2 * num_sms; }   // two CTAs per SM: 97 KB of shared memory each
 
-int launch_cache16(const CacheAttnParams& p, const tb200_cache_attn_args& a, int nt, cudaStream_t stream) {
+int launch_cache16(const CacheAttnParams& p, const tb200_cache_attn_args& a, int unit_rows, cudaStream_t stream) {
+  const int nt = unit_rows / 8;
   CacheMaps maps;
   const uint64_t d = static_cast<uint64_t>(a.head_dim);
   const uint64_t dims[4] = {d, static_cast<uint64_t>(a.cache_len), static_cast<uint64_t>(a.n_kv_heads), static_cast<uint64_t>(a.batch)};

@@ -162,12 +162,12 @@ template <int D, int NT> struct MergeSmem {
   static constexpr int kMlOff = kWarps * kR * kPitch * 4;    // float2 [warps][R] behind float [warps][R][pitch]
   static constexpr int kBytes = kMlOff + kWarps * kR * 8;
 };
-// The four warps' shares in a fixed order: into o where the unit lies in this stretch altogether, else into the stretch's
+// The four warps' shares (of each row H from each warp) in a fixed order: into o where the unit lies in this stretch altogether, else into the stretch's
 // partial results.  Called by the whole CTA, with the shares written and a barrier behind them.
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int H>
 __device__ __forceinline__ void merge_segment(const CacheAttnParams& p, const uint8_t* smem, const Walk& wk, const Segment& sg) {
   using M = MergeSmem<D, NT>;
-  constexpr int R = M::kR;
+  constexpr int R = M::kR / H;
   const bool whole = sg.v0 == 0 && sg.v1 == wk.sq.tiles;
   if (threadIdx.x == 0 && wk.x + sg.v1 - sg.v0 >= wk.x_end)   // the stretch's last segment
     p.split[blockIdx.x] = make_int4(sg.b, sg.h, sg.rt, sg.v0 == 0 && !whole ? (wk.x + wk.sq.tiles - 1) / wk.ln.per - static_cast<int>(blockIdx.x) + 1 : 0);
@@ -178,11 +178,11 @@ __device__ __forceinline__ void merge_segment(const CacheAttnParams& p, const ui
     const int m = i / (D / 4), d = (i % (D / 4)) * 4;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, mlall[w * R + m].x);
+    for (int w = 0; w < kWarps * H; ++w) top = fmaxf(top, mlall[w * R + m].x);
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kWarps * H; ++w) {
       const float2 ml = mlall[w * R + m];
       const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
       const float4 a = *reinterpret_cast<const float4*>(mall + (w * R + m) * M::kPitch + d);
@@ -211,9 +211,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 // attn_cache.cu
-int launch_cache_combine(const CacheAttnParams& p, int dtype, int head_dim, int nt, cudaStream_t stream);
+int launch_cache_combine(const CacheAttnParams& p, int dtype, int head_dim, int unit_rows, cudaStream_t stream);
 // attn_win.cu: the decode kernel over 16-bit caches, in a ChainScope; p.stretches as cache16_stretches says
-int launch_cache16(const CacheAttnParams& p, const tb200_cache_attn_args& a, int nt, cudaStream_t stream);
-int cache16_stretches(int nt, int num_sms);
+int launch_cache16(const CacheAttnParams& p, const tb200_cache_attn_args& a, int unit_rows, cudaStream_t stream);   // 8 or 16
+int cache16_stretches(int num_sms);
 
 }  // namespace tb200
