@@ -206,6 +206,11 @@ SHAPES = [  # b, hq, hkv, d, s, cache length, lens, rows, window, sinks
     (2, 6, 2, 64, 513, 516, [514, 513], [513, 400], 1, 0),
     (2, 6, 2, 128, 260, 1200, [1111, 300], [260, 260], 128, 300),
     (1, 2, 1, 128, 40, 20000, [19999], [40], 5000, 128),
+    (2, 14, 2, 64, 45, 400, [400, 45], [45, 30], 50, 3),
+    (1, 71, 1, 64, 40, 300, [300], [39], 0, 0),
+    (2, 12, 2, 128, 100, 1000, [900, 100], [100, 64], 150, 20),
+    (3, 32, 8, 128, 300, 2048, [2000, 300, 20], [300, 290, 300], 700, 4),
+    (2, 16, 2, 64, 33, 3000, [3000, 1029], [33, 32], 0, 0),
 ]
 
 

@@ -27,6 +27,9 @@
 // sixteen keys.  (With tiles at multiples of 128 and a tile for the first positions, 4000 queries under a window of 1000:
 // 105 us.)  Rows of V that no query of the item sees are cleared in shared memory before they meet a probability of 0,
 // because a cache may hold anything there.
+// A query tile packs `pack` query heads that share a kv head: row r is token r / pack of the tile's tokens, head r % pack of
+// the pack.  Few tokens then still fill a tile, and the tokens of a tile lie closer together, so that less of a window's or
+// the diagonal's tiles is masked; the host takes the pack with the fewest key tiles to walk.
 //
 // One thread owns one query row.  (Two threads per row were measured slower on B200 -- 0.418 ms against 0.353 ms on
 // the Llama-3-8B B8 S2048 prefill: the row-max exchange costs more than the extra warps hide -- and so was a variant
@@ -99,6 +102,8 @@ struct Attn2Params {
   const int32_t* kv_lens;
   const int32_t* q_rows;
   int cache_len, window, sinks;
+  int pack, tokens;  // query heads of a query tile, tokens of a query tile (tokens * pack <= BQ)
+  FastDiv d_pack;
   long long o_stride[3];
 };
 
@@ -127,7 +132,7 @@ template <bool SEQ> __device__ __forceinline__ Item decode_item(const Attn2Param
   it.b = fdiv(r1, p.d_hq);
   it.hq = r1 - it.b * p.Hq;
   it.hkv = fdiv(it.hq, p.d_group);
-  it.q0 = (p.n_blocks - 1 - blk) * 2 * BQ;
+  it.q0 = (p.n_blocks - 1 - blk) * 2 * (SEQ ? p.tokens : BQ);   // SEQ: hq counts packs of heads
   if constexpr (SEQ) {
     const int n = max(0, min(__ldg(p.kv_lens + it.b), p.cache_len));
     it.rows = p.q_rows ? max(0, min(__ldg(p.q_rows + it.b), p.S)) : p.S;
@@ -139,9 +144,9 @@ template <bool SEQ> __device__ __forceinline__ Item decode_item(const Attn2Param
     it.gap = apart ? low - it.head : 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int q0t = it.q0 + t * BQ;
+      const int q0t = it.q0 + t * p.tokens;
       if (q0t >= it.rows) continue;
-      it.last = it.past + min(q0t + BQ, it.rows) - 1 - it.gap;
+      it.last = it.past + min(q0t + p.tokens, it.rows) - 1 - it.gap;
       it.nt[t] = max(0, it.last) / BKV + 1;   // without a visible key (last < 0): one masked tile makes the zeros
     }
   } else
@@ -241,11 +246,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
           if ((t == 0 ? it.nt[0] : it.nt[1]) == 0) continue;
           if (loads > 0 && !mbar_wait(&q_empty[t], (loads - 1) & 1, ctx, 400)) { ok = false; break; }
           if (lane == 0) {
-            mbar_arrive_expect_tx(&q_full[t], L::kTile);
+            mbar_arrive_expect_tx(&q_full[t], SEQ ? p.tokens * p.pack * D * 2 : L::kTile);
 #pragma unroll
             for (int dc = 0; dc < D / 64; ++dc) {
               uint8_t* dst = smem + L::kQOff + t * L::kTile + dc * (BQ * 128);
-              if constexpr (SEQ) tma_load_4d(dst, &p.map_q, &q_full[t], dc * 64, it.q0 + t * BQ, it.hq, it.b);
+              if constexpr (SEQ) tma_load_5d(dst, &p.map_q, &q_full[t], dc * 64, 0, it.q0 + t * p.tokens, it.hq, it.b);
               else tma_load_3d(dst, &p.map_q, &q_full[t], dc * 64, it.q0 + t * BQ, it.b * p.Hq + it.hq);
             }
           }
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
         const Item it = decode_item<SEQ>(p, i);
         my_nt = t == 0 ? it.nt[0] : it.nt[1];
         k_first = it.j_begin * BKV;
-        const int qi = it.q0 + t * BQ + r_in;
+        const int qi = SEQ ? it.q0 + t * p.tokens + fdiv(r_in, p.d_pack) : it.q0 + t * BQ + r_in;
         key_limit = p.causal ? min(p.past + qi, p.kv_len - 1) : p.kv_len - 1;
         if constexpr (SEQ) {
           key_limit = it.past + qi - it.gap;
@@ -532,8 +537,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
       // ---- end of the item: hand the factor each row of O is to be multiplied with to the output warpgroup (which
       //      waits for the last P V itself) and go on to the next item at once
       const Item it = decode_item<SEQ>(p, i);
-      const int qi = it.q0 + t * BQ + r_in;
-      const bool row_ok = qi < (SEQ ? it.rows : p.S);
+      const int tok = SEQ ? fdiv(r_in, p.d_pack) : r_in;
+      const int qi = it.q0 + t * (SEQ ? p.tokens : BQ) + tok;
+      const bool row_ok = SEQ ? qi < it.rows && tok < p.tokens : qi < p.S;
       if (my_nt > 0) {
         if (handed > 0 && !mbar_wait(&stat_empty[t], (handed - 1) & 1, ctx, 411)) { ok = false; break; }
         stat[t * BQ + r_in] = (p.kv_splits > 1) ? 1.f : ((l > 0.f) ? 1.f / l : 0.f);
@@ -544,7 +550,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
       if (p.kv_splits > 1) {
         // this item saw only a share of the keys: its unnormalised accumulator, exponent reference and row sum are
         // left for attn_combine_kernel.  A share without keys leaves the neutral element.
-        const long long prow = ((static_cast<long long>(it.sp) * p.B + it.b) * p.Hq + it.hq) * p.S + qi;
+        const long long prow = (SEQ ? ((static_cast<long long>(it.sp) * p.B + it.b) * p.Hq + it.hq) * p.pack + r_in - tok * p.pack
+                                    : (static_cast<long long>(it.sp) * p.B + it.b) * p.Hq + it.hq) * p.S + qi;
         if (row_ok) {
           p.part_ml[prow * 2] = my_nt > 0 ? m_use : -INFINITY;
           p.part_ml[prow * 2 + 1] = my_nt > 0 ? l : 0.f;
@@ -588,11 +595,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
         if (!mbar_wait(&pv_done[t], (total - 1) & 1, ctx, 409)) { ok = false; break; }
         tc_fence_after();
         const uint32_t tmem_o = tmem_base + 2 * BKV + t * D + lane_sel;
-        const int q0t = it.q0 + t * BQ;
+        const int q0t = it.q0 + t * (SEQ ? p.tokens : BQ);
         uint32_t o[32];
         if (p.kv_splits > 1) {
-          const int qi = q0t + r_in;
-          const long long prow = ((static_cast<long long>(it.sp) * p.B + it.b) * p.Hq + it.hq) * p.S + qi;
+          const int tok = SEQ ? fdiv(r_in, p.d_pack) : r_in;
+          const int qi = q0t + tok;
+          const bool row_ok = SEQ ? qi < it.rows && tok < p.tokens : qi < p.S;
+          const long long prow = (SEQ ? ((static_cast<long long>(it.sp) * p.B + it.b) * p.Hq + it.hq) * p.pack + r_in - tok * p.pack
+                                      : (static_cast<long long>(it.sp) * p.B + it.b) * p.Hq + it.hq) * p.S + qi;
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             tmem_ld_x32(tmem_o + c * 32, o);
@@ -602,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
               __syncwarp();
               if (lane == 0) mbar_arrive(&o_free[t]);
             }
-            if (qi < (SEQ ? it.rows : p.S)) {
+            if (row_ok) {
               uint4* d = reinterpret_cast<uint4*>(p.part_o + prow * D + c * 32);
 #pragma unroll
               for (int e = 0; e < 8; ++e) d[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
@@ -637,17 +647,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
         fence_proxy_async_smem();
         named_barrier_sync(1, 128);
         if constexpr (SEQ) {
-          if (q0t + BQ <= it.rows || it.rows == p.S) {
+          if (q0t + p.tokens <= it.rows || it.rows == p.S) {
             if (tid == 0) {
 #pragma unroll
-              for (int dc = 0; dc < D / 64; ++dc) tma_store_4d(&p.map_o, stage + dc * (BQ * 128), dc * 64, q0t, it.hq, it.b);
+              for (int dc = 0; dc < D / 64; ++dc) tma_store_5d(&p.map_o, stage + dc * (BQ * 128), dc * 64, 0, q0t, it.hq, it.b);
               tma_store_commit();
             }
           } else {  // rows behind the sequence's last one stay as they are
-            T* o = static_cast<T*>(p.o2) + it.b * p.o_stride[0] + it.hq * p.o_stride[1];
-            for (int i = tid; i < (it.rows - q0t) * (D / 8); i += 128) {
+            T* o = static_cast<T*>(p.o2) + it.b * p.o_stride[0] + static_cast<long long>(it.hq) * p.pack * p.o_stride[1];
+            for (int i = tid; i < (it.rows - q0t) * p.pack * (D / 8); i += 128) {
               const int r = i / (D / 8), c = i % (D / 8);
-              *reinterpret_cast<uint4*>(o + static_cast<long long>(q0t + r) * p.o_stride[2] + c * 8) =
+              const int tok = fdiv(r, p.d_pack);
+              *reinterpret_cast<uint4*>(o + (r - tok * p.pack) * p.o_stride[1] + (q0t + tok) * p.o_stride[2] + c * 8) =
                   *reinterpret_cast<const uint4*>(stage + (c >> 3) * (BQ * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
             }
           }
@@ -745,14 +756,15 @@ int launch_one(const Attn2Params& p, dim3 grid, int num_sms, cudaStream_t stream
   if (launch_chained(attn_fwd2_kernel<T, D, SEQ>, grid, dim3(kThreads, 1, 1), Smem2<D>::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
   if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
   if (p.kv_splits > 1) {
-    const long long rows = static_cast<long long>(p.B) * p.Hq * p.S;
+    const int heads = SEQ ? p.Hq * p.pack : p.Hq;
+    const long long rows = static_cast<long long>(p.B) * heads * p.S;
     long long blocks = (rows * 32 + 255) / 256;
     if (blocks > num_sms * 8) blocks = num_sms * 8;
     CombineSeq seq;
     seq.q_rows = p.q_rows;
     for (int i = 0; i < 3; ++i) seq.o_stride[i] = p.o_stride[i];
     if (launch_chained(attn_combine_kernel<T, D, SEQ>, dim3(static_cast<unsigned>(blocks), 1, 1), dim3(256, 1, 1), 0, stream, p.part_o, p.part_ml,
-                       static_cast<T*>(p.o2), p.lse2, p.kv_splits, p.B, p.Hq, p.S, seq) != cudaSuccess)
+                       static_cast<T*>(p.o2), p.lse2, p.kv_splits, p.B, heads, p.S, seq) != cudaSuccess)
       return TB200_ERR_CUDA;
     if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
   }
@@ -762,7 +774,8 @@ int launch_one(const Attn2Params& p, dim3 grid, int num_sms, cudaStream_t stream
 // The items of a launch and the launch itself, once the tensors are described.
 template <bool SEQ>
 int finish_launch(Attn2Params& p, int dtype, int D, const DeviceState* st, cudaStream_t stream) {
-  p.n_blocks = (p.S + 2 * BQ - 1) / (2 * BQ);
+  const int item_rows = 2 * (SEQ ? p.tokens : BQ);
+  p.n_blocks = (p.S + item_rows - 1) / item_rows;
   const long long items = static_cast<long long>(p.n_blocks) * p.kv_splits * p.Hq * p.B;
   if (items > 0x7fffffffLL) return TB200_ERR_INVALID;
   p.n_items = static_cast<int>(items);
@@ -831,6 +844,25 @@ int launch_attn_fwd_pingpong(const AttnLaunch& a, cudaStream_t stream) {
   return finish_launch<false>(p, a.dtype, a.D, st, stream);
 }
 
+// Query heads per query tile: of the divisors of the group the one with the fewest (query tile pair, key tile) steps.
+int attn_seq_pack(int S, int Hq, int Hkv, int cache_len, int window, int sinks) {
+  const int group = Hq / Hkv;
+  int best = 1;
+  double least = 0;
+  for (int pack = 1; pack <= group && pack <= BQ; ++pack) {
+    if (group % pack) continue;
+    const int item = 2 * (BQ / pack);
+    double keys = cache_len;   // of an item; without a window the causal half of the new rows is the same for every pack
+    if (window > 0 && window + item + sinks < cache_len) keys = window + item + sinks;
+    const double steps = static_cast<double>(Hq / pack) * ((S + item - 1) / item) * static_cast<int64_t>((keys + BKV - 1) / BKV);
+    if (pack == 1 || steps < least) {
+      best = pack;
+      least = steps;
+    }
+  }
+  return best;
+}
+
 // The same kernel over caches with per-sequence lengths; arguments are validated by the caller.
 int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
   int status = TB200_OK;
@@ -838,7 +870,10 @@ int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
   if (!st) return status;
   Attn2Params p;
   memset(&p, 0, sizeof(p));
-  p.B = a.B; p.S = a.S; p.Hq = a.Hq; p.Hkv = a.Hkv; p.kv_len = a.cache_len; p.causal = 1;
+  p.pack = a.pack;
+  p.tokens = BQ / a.pack;
+  p.d_pack = make_fastdiv(static_cast<uint32_t>(a.pack));
+  p.B = a.B; p.S = a.S; p.Hq = a.Hq / a.pack; p.Hkv = a.Hkv; p.kv_len = a.cache_len; p.causal = 1;
   p.cache_len = a.cache_len; p.window = a.window; p.sinks = a.sinks;
   p.kv_lens = a.kv_lens; p.q_rows = a.q_rows;
   p.scale_log2 = a.sm_scale * kLog2e;
@@ -858,14 +893,22 @@ int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
     return make_tensor_map(map, base, 4, dims, strides, box);
   };
   static_assert(BQ == BKV, "one box size for queries and keys");
-  if ((status = map4(&p.map_q, a.q, a.S, a.Hq, a.q_stride, BQ)) != TB200_OK) return status;
+  auto map5 = [&](CUtensorMap* map, const void* base, const int64_t (&st3)[3]) {   // (D, heads of a pack, rows, packs, batch)
+    const uint64_t d = static_cast<uint64_t>(a.D);
+    const uint64_t dims[5] = {d, static_cast<uint64_t>(a.pack), static_cast<uint64_t>(a.S), static_cast<uint64_t>(p.Hq), static_cast<uint64_t>(a.B)};
+    const uint64_t strides[4] = {a.Hq > 1 ? static_cast<uint64_t>(st3[1]) * 2 : d * 2, a.S > 1 ? static_cast<uint64_t>(st3[2]) * 2 : d * 2,
+                                 a.Hq > 1 ? static_cast<uint64_t>(st3[1]) * 2 * a.pack : d * 2, a.B > 1 ? static_cast<uint64_t>(st3[0]) * 2 : d * 2};
+    const uint32_t box[5] = {64, static_cast<uint32_t>(a.pack), static_cast<uint32_t>(p.tokens), 1, 1};
+    return make_tensor_map(map, base, 5, dims, strides, box);
+  };
+  if ((status = map5(&p.map_q, a.q, a.q_stride)) != TB200_OK) return status;
   if ((status = map4(&p.map_k, a.k_cache, a.cache_len, a.Hkv, a.k_stride, BQ)) != TB200_OK) return status;
   if ((status = map4(&p.map_v, a.v_cache, a.cache_len, a.Hkv, a.v_stride, BQ)) != TB200_OK) return status;
   if (a.sinks > 0) {
     if ((status = map4(&p.map_k16, a.k_cache, a.cache_len, a.Hkv, a.k_stride, 16)) != TB200_OK) return status;
     if ((status = map4(&p.map_v16, a.v_cache, a.cache_len, a.Hkv, a.v_stride, 16)) != TB200_OK) return status;
   }
-  if ((status = map4(&p.map_o, a.o, a.S, a.Hq, a.o_stride, BQ)) != TB200_OK) return status;
+  if ((status = map5(&p.map_o, a.o, a.o_stride)) != TB200_OK) return status;
   return finish_launch<true>(p, a.dtype, a.D, st, stream);
 }
 

@@ -593,7 +593,7 @@ struct AttnPlan {
   bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
   int unit_rows = 8;         // decode: query rows of a unit
   int stretches = 0;
-  int kv_splits = 1;         // prompt
+  int pack = 1, kv_splits = 1;   // prompt
   size_t part_o = 0, part_ml = 0, split = 0, cache16 = 0;   // bytes; cache16: of one of the two caches
   size_t total() const { return part_o + part_ml + split + 2 * cache16; }
 };
@@ -603,7 +603,10 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   pl.prompt = a->rows > (kv4 ? kDecodeTokens4 : kDecodeTokens16);
   if (pl.prompt) {
     const int64_t seen = a->window > 0 ? static_cast<int64_t>(a->window) + a->rows + a->sinks : a->cache_len;
-    pl.kv_splits = attn_kv_splits(a->batch, a->rows, a->n_q_heads, static_cast<int>(seen < a->cache_len ? seen : a->cache_len), num_sms);
+    pl.pack = attn_seq_pack(a->rows, a->n_q_heads, a->n_kv_heads, a->cache_len, a->window, a->sinks);
+    // the splits count blocks of 256 rows: tokens times packed heads
+    pl.kv_splits = attn_kv_splits(a->batch, (a->rows + 128 / pl.pack - 1) / (128 / pl.pack) * 128, a->n_q_heads / pl.pack,
+                                  static_cast<int>(seen < a->cache_len ? seen : a->cache_len), num_sms);
     if (pl.kv_splits > 1) {
       const size_t prows = static_cast<size_t>(pl.kv_splits) * a->batch * a->n_q_heads * a->rows;
       pl.part_o = align_up(prows * a->head_dim * sizeof(float), 256);
@@ -691,6 +694,7 @@ int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, con
   s.sm_scale = a->sm_scale;
   s.q = a->q; s.o = a->o;
   s.kv_lens = a->kv_lens; s.q_rows = a->q_rows;
+  s.pack = pl.pack;
   s.kv_splits = pl.kv_splits;
   s.part_o = reinterpret_cast<float*>(ws);
   s.part_ml = reinterpret_cast<float*>(ws + pl.part_o);

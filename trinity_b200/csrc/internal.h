@@ -195,10 +195,12 @@ struct AttnSeqLaunch {
   int64_t q_stride[3] = {}, k_stride[3] = {}, v_stride[3] = {}, o_stride[3] = {};
   const int32_t* kv_lens = nullptr;
   const int32_t* q_rows = nullptr;
+  int pack = 1;                     // query heads per query tile (attn_seq_pack)
   int kv_splits = 1;
   float* part_o = nullptr;          // (kv_splits,B,Hq,S,D) fp32
   float* part_ml = nullptr;         // (kv_splits,B,Hq,S,2) fp32
 };
+int attn_seq_pack(int S, int Hq, int Hkv, int cache_len, int window, int sinks);
 int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream);
 // attn_kf.cu: the same kernel with the KeyFormer statistic (noise tiles by TMA; kv_len a multiple of 8)
 int launch_attn_fwd_keyformer(const AttnLaunch& a, cudaStream_t stream);
