@@ -578,8 +578,13 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   return TB200_OK;
 }
 
-// New rows per sequence up to which a call runs a decode kernel.
-constexpr int kDecodeTokens4 = 32, kDecodeTokens16 = 32;
+// Decode kernel or prompt kernel, by the query rows of a sequence that share a kv head (new tokens x query heads per kv head).
+// 16 bits: the prompt kernel packs the rows into tiles of 128, the decode kernel reads the cache once per 16 rows.  16
+// sequences of 2048 positions, 32/8 heads, decode and prompt kernel in us: 16 rows 34 / 37, 32 rows 37 / 37, 64 rows 62 / 37;
+// one head per kv head 16 rows 34 / 37; 71 heads on one, a single token, 4 x 16384 positions: 21 / 21.
+// 4 bits: the prompt kernel needs the visible rows in 16 bits first: 32 rows 40 / 65, 64 rows 68 / 66, 96 rows 97 / 66; 71
+// heads, a single token 23 / 25.  A single token never takes that copy (its workspace is that of all the cache).
+bool takes_prompt_kernel(int64_t rows, int tokens, bool kv4) { return kv4 ? rows > 64 && tokens > 1 : rows > 16; }
 
 // Query rows of a unit: the smallest form that holds a sequence's rows of one kv head, else as many as there are.  Four rows:
 // see H at cache_decode_kernel.
@@ -600,7 +605,7 @@ struct AttnPlan {
 AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   AttnPlan pl;
   const int64_t rows = static_cast<int64_t>(a->rows) * (a->n_q_heads / a->n_kv_heads);
-  pl.prompt = a->rows > (kv4 ? kDecodeTokens4 : kDecodeTokens16);
+  pl.prompt = takes_prompt_kernel(rows, a->rows, kv4);
   if (pl.prompt) {
     const int64_t seen = a->window > 0 ? static_cast<int64_t>(a->window) + a->rows + a->sinks : a->cache_len;
     pl.pack = attn_seq_pack(a->rows, a->n_q_heads, a->n_kv_heads, a->cache_len, a->window, a->sinks);
