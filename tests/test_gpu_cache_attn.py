@@ -350,6 +350,61 @@ def test_write_then_attend_token_by_token():
     assert ops.device_status() == 0
 
 
+def test_empty_batches_and_no_rows():
+    dt = torch.bfloat16
+    for b, s in ((0, 3), (2, 0)):
+        cache = ops.kv4_cache(b, 2, 16, 64, dt, DEV)
+        x = torch.zeros(b, 2, s, 64, dtype=dt, device=DEV)
+        lens = torch.zeros(b, dtype=torch.int32, device=DEV)
+        ops.kv4_append(cache, x, x, 0)
+        assert ops.kv4_read(cache, 0, s)[0].shape == (b, 2, s, 64)
+        assert ops.kv4_attn(x, cache, lens).shape == (b, 2, s, 64)
+        assert ops.attn_window(x, torch.zeros(b, 2, 16, 64, dtype=dt, device=DEV), torch.zeros(b, 2, 16, 64, dtype=dt, device=DEV), lens, window=4).shape == x.shape
+
+
+def test_offsets_past_32_bits():
+    """Caches whose codes, or whose 16-bit rows, take more than 4 GiB: rows at the far end, and a window there."""
+    dt, d, h = torch.bfloat16, 128, 2
+    g = torch.Generator(device=DEV).manual_seed(4)
+    for kv4, length in ((True, 40_000_000), (False, 12_000_000)):
+        new, window, sinks = 20, 100, 4
+        n = length - 8
+        q, k, v = (torch.randn(1, x, new, d, generator=g, device=DEV).to(dt) for x in (4, h, h))
+        first, tail = slice(0, sinks), slice(n - new - window, n)
+        if kv4:
+            cache = ops.Kv4Cache(*[torch.empty(1, h, length, d // 2, dtype=torch.uint8, device=DEV) for _ in range(2)],
+                                 *[torch.empty(1, h, length, d // 64, 2, dtype=dt, device=DEV) for _ in range(2)])
+            old = torch.randn(1, h, window, d, generator=g, device=DEV).to(dt)
+            ops.kv4_append(cache, old, old, 0, rows=ints([sinks]))
+            ops.kv4_append(cache, old, old, n - new - window)
+            ops.kv4_append(cache, k, v, n - new)
+            kr, vr = ops.kv4_read(cache, n - new, new)
+            assert ((kr.double() - k.double()).abs() <= (k.double().amax(-1) - k.double().amin(-1)).amax() / 15).all()
+            outs = [ops.kv4_attn(q[:, :, -r:], cache, ints([n]), window=window, sinks=sinks, sm_scale=0.1) for r in (1, new)]
+            part = ops.Kv4Cache(*[torch.cat([t[:, :, first], t[:, :, tail]], 2).contiguous() for t in cache])
+            k64, v64 = values64(part, "k"), values64(part, "v")
+        else:
+            kc, vc = torch.empty(1, h, length, d, dtype=dt, device=DEV), torch.empty(1, h, length, d, dtype=dt, device=DEV)
+            for t, x in ((kc, k), (vc, v)):
+                t[:, :, first] = torch.randn(1, h, sinks, d, generator=g, device=DEV).to(dt)
+                t[:, :, tail] = torch.randn(1, h, window + new, d, generator=g, device=DEV).to(dt)
+                t[:, :, n - new:n] = x
+            outs = [ops.attn_window(q[:, :, -r:], kc, vc, ints([n]), window=window, sinks=sinks, sm_scale=0.1) for r in (1, new)]
+            k64, v64 = (torch.cat([t[:, :, first], t[:, :, tail]], 2).double() for t in (kc, vc))
+            del kc, vc
+        # the same keys in a short cache, with the window at the same distance: the first ones stay, the rest is the tail
+        m = sinks + window + new
+        for r, out in zip((1, new), outs):
+            at = torch.arange(m - r, m, device=DEV)[:, None]
+            j = torch.arange(m, device=DEV)[None, :]
+            seen = (j <= at) & ((j > at - window) | (j < sinks))
+            z = torch.einsum("bhgrd,bhnd->bhgrn", q[:, :, -r:].double().unflatten(1, (h, 2)), k64) * 0.1
+            p = torch.softmax(z.masked_fill(~seen, -math.inf), -1)
+            want = torch.einsum("bhgrn,bhnd->bhgrd", p, v64).flatten(1, 2)
+            check_rows(out, want, q[:, :, -r:], k64, v64, [m], [r], 0.1, dt)
+        del outs
+
+
 def test_two_streams_at_once():
     """Calls on two streams have workspaces of their own."""
     shape = (4, 32, 8, 128, 1, 4096, [4096, 4000, 100, 2222], [1] * 4, 0, 0)

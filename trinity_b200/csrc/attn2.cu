@@ -853,7 +853,7 @@ int attn_seq_pack(int S, int Hq, int Hkv, int cache_len, int window, int sinks) 
     if (group % pack) continue;
     const int item = 2 * (BQ / pack);
     double keys = cache_len;   // of an item; without a window the causal half of the new rows is the same for every pack
-    if (window > 0 && window + item + sinks < cache_len) keys = window + item + sinks;
+    if (window > 0 && static_cast<int64_t>(window) + item + sinks < cache_len) keys = window + item + sinks;
     const double steps = static_cast<double>(Hq / pack) * ((S + item - 1) / item) * static_cast<int64_t>((keys + BKV - 1) / BKV);
     if (pack == 1 || steps < least) {
       best = pack;

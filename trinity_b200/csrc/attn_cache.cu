@@ -561,6 +561,7 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   if (a->batch < 0 || a->rows < 0 || a->n_kv_heads < 1 || a->n_q_heads < 1 || a->n_q_heads % a->n_kv_heads || a->cache_len < 1) return TB200_ERR_INVALID;
   if (a->batch > kMaxExtent || a->cache_len > kMaxExtent || static_cast<int64_t>(a->n_q_heads) * a->rows > kMaxExtent) return TB200_ERR_INVALID;
   if (a->window < 0 || a->sinks < 0 || !(a->sm_scale >= 1e-30f) || !(a->sm_scale < INFINITY)) return TB200_ERR_INVALID;
+  if (a->batch == 0 || a->rows == 0) return TB200_OK;   // nothing to read or write: empty tensors have no address
   if (!a->q || !a->o || !a->kv_lens || a->q == a->o || !aligned16(a->q) || !aligned16(a->o) || !aligned4(a->kv_lens) || !aligned4(a->q_rows))
     return TB200_ERR_INVALID;
   const int64_t ext[3] = {a->batch, a->n_q_heads, a->rows};
@@ -602,13 +603,18 @@ struct AttnPlan {
   size_t part_o = 0, part_ml = 0, split = 0, cache16 = 0;   // bytes; cache16: of one of the two caches
   size_t total() const { return part_o + part_ml + split + 2 * cache16; }
 };
+// A window as long as the cache hides nothing; first positions matter only beside a window.
+int window_of(const tb200_cache_attn_args* a) { return a->window < a->cache_len ? a->window : 0; }
+int sinks_of(const tb200_cache_attn_args* a) { return window_of(a) > 0 ? (a->sinks < a->cache_len ? a->sinks : a->cache_len) : 0; }
+
 AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   AttnPlan pl;
+  const int window = window_of(a), sinks = sinks_of(a);
   const int64_t rows = static_cast<int64_t>(a->rows) * (a->n_q_heads / a->n_kv_heads);
   pl.prompt = takes_prompt_kernel(rows, a->rows, kv4);
   if (pl.prompt) {
-    const int64_t seen = a->window > 0 ? static_cast<int64_t>(a->window) + a->rows + a->sinks : a->cache_len;
-    pl.pack = attn_seq_pack(a->rows, a->n_q_heads, a->n_kv_heads, a->cache_len, a->window, a->sinks);
+    const int64_t seen = window > 0 ? static_cast<int64_t>(window) + a->rows + sinks : a->cache_len;
+    pl.pack = attn_seq_pack(a->rows, a->n_q_heads, a->n_kv_heads, a->cache_len, window, sinks);
     // the splits count blocks of 256 rows: tokens times packed heads
     pl.kv_splits = attn_kv_splits(a->batch, (a->rows + 128 / pl.pack - 1) / (128 / pl.pack) * 128, a->n_q_heads / pl.pack,
                                   static_cast<int>(seen < a->cache_len ? seen : a->cache_len), num_sms);
@@ -633,8 +639,8 @@ CacheAttnParams make_params(const tb200_cache_attn_args* a, const DeviceState* s
   memset(&p, 0, sizeof(p));
   p.B = a->batch; p.S = a->rows; p.Hq = a->n_q_heads; p.Hkv = a->n_kv_heads; p.group = a->n_q_heads / a->n_kv_heads;
   p.cache_len = a->cache_len;
-  p.window = a->window < a->cache_len ? a->window : 0;   // a window as long as the cache hides nothing
-  p.sinks = p.window > 0 ? (a->sinks < a->cache_len ? a->sinks : a->cache_len) : 0;
+  p.window = window_of(a);
+  p.sinks = sinks_of(a);
   p.scale_log2 = a->sm_scale * kLog2e;
   p.q = static_cast<const uint8_t*>(a->q);
   p.o = static_cast<uint8_t*>(a->o);

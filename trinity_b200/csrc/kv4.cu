@@ -255,6 +255,7 @@ int check_rows(const tb200_kv4_rows_args* a) {
   if (a->dtype != TB200_BF16 && a->dtype != TB200_F16) return TB200_ERR_UNSUPPORTED;
   if (a->head_dim != 64 && a->head_dim != 128) return TB200_ERR_UNSUPPORTED;
   if (a->batch < 0 || a->rows < 0 || a->n_kv_heads < 1 || a->cache_len < 0 || (a->cache_len & 3) || a->reserved != 0) return TB200_ERR_INVALID;
+  if (a->batch == 0 || a->rows == 0 || a->cache_len == 0) return TB200_OK;   // nothing to read or write: empty tensors have no address
   if (!a->k || !a->v || !a->k_codes || !a->v_codes || !a->k_meta || !a->v_meta) return TB200_ERR_INVALID;
   if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_codes) || !aligned16(a->v_codes) || !aligned16(a->k_meta) || !aligned16(a->v_meta))
     return TB200_ERR_INVALID;
