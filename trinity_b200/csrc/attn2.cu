@@ -687,7 +687,8 @@ struct CombineSeq {   // SEQ: where o goes and which rows exist
   const int32_t* q_rows;
   long long o_stride[3];
 };
-template <typename T, int D, bool SEQ>
+// kMaxSplits: few shares need few registers, and more rows are under way at a time.
+template <typename T, int D, bool SEQ, int kMaxSplits>
 __global__ void attn_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, T* __restrict__ o2,
                                     float* __restrict__ lse2, int splits, int B, int Hq, int S, const CombineSeq seq) {
   constexpr int V = D / 32;
@@ -700,8 +701,7 @@ __global__ void attn_combine_kernel(const float* __restrict__ part_o, const floa
     if constexpr (SEQ) {
       if (seq.q_rows && static_cast<int>(row % S) >= __ldg(seq.q_rows + row / (static_cast<long long>(S) * Hq))) continue;
     }
-    // all the shares' loads are in flight together (at most 16 shares): one trip to L2, not one per share
-    constexpr int kMaxSplits = 16;
+    // all the shares' loads are in flight together: one trip to L2, not one per share
     float2 ml[kMaxSplits];
     float po[kMaxSplits][V];
 #pragma unroll
@@ -763,7 +763,8 @@ int launch_one(const Attn2Params& p, dim3 grid, int num_sms, cudaStream_t stream
     CombineSeq seq;
     seq.q_rows = p.q_rows;
     for (int i = 0; i < 3; ++i) seq.o_stride[i] = p.o_stride[i];
-    if (launch_chained(attn_combine_kernel<T, D, SEQ>, dim3(static_cast<unsigned>(blocks), 1, 1), dim3(256, 1, 1), 0, stream, p.part_o, p.part_ml,
+    auto* combine = SEQ && p.kv_splits <= 4 ? attn_combine_kernel<T, D, SEQ, SEQ ? 4 : 16> : attn_combine_kernel<T, D, SEQ, 16>;
+    if (launch_chained(combine, dim3(static_cast<unsigned>(blocks), 1, 1), dim3(256, 1, 1), 0, stream, p.part_o, p.part_ml,
                        static_cast<T*>(p.o2), p.lse2, p.kv_splits, p.B, heads, p.S, seq) != cudaSuccess)
       return TB200_ERR_CUDA;
     if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
