@@ -30,6 +30,8 @@
 // A query tile packs `pack` query heads that share a kv head: row r is token r / pack of the tile's tokens, head r % pack of
 // the pack.  Few tokens then still fill a tile, and the tokens of a tile lie closer together, so that less of a window's or
 // the diagonal's tiles is masked; the host takes the pack with the fewest key tiles to walk.
+// With Out != T everything is computed in fp16 on q, K and V that were divided by powers of two (per row, per kv head), and
+// written in bf16: what a 4-bit cache stands for has more digits than bf16 keeps.
 //
 // One thread owns one query row.  (Two threads per row were measured slower on B200 -- 0.418 ms against 0.353 ms on
 // the Llama-3-8B B8 S2048 prefill: the row-max exchange costs more than the extra warps hide -- and so was a variant
@@ -37,6 +39,8 @@
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -104,6 +108,8 @@ struct Attn2Params {
   int cache_len, window, sinks;
   int pack, tokens;  // query heads of a query tile, tokens of a query tile (tokens * pack <= BQ)
   FastDiv d_pack;
+  const float* q_factor;      // SEQ with Out != T: what the rows of q and the heads' K and V have been divided by (powers of two)
+  const float4* head_factor;  // (.y: K, .w: V)
   long long o_stride[3];
 };
 
@@ -167,7 +173,7 @@ template <bool SEQ> __device__ __forceinline__ Item decode_item(const Attn2Param
   return it;
 }
 
-template <typename T, int D, bool SEQ>
+template <typename T, int D, bool SEQ, typename Out>
 __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_constant__ Attn2Params p) {
   using L = Smem2<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -432,6 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
 
     for (int i = blockIdx.x; ok && i < p.n_items; i += gridDim.x) {
       int my_nt, k_first, key_limit, win_low = 0, few = 0;   // SEQ: all of them places on the item's line
+      float scale_log2 = p.scale_log2, v_factor = 1.f;
       {  // only what the key loop needs stays live through it; the item is decoded again for the output addresses
         const Item it = decode_item<SEQ>(p, i);
         my_nt = t == 0 ? it.nt[0] : it.nt[1];
@@ -442,6 +449,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
           key_limit = it.past + qi - it.gap;
           win_low = p.window > 0 ? max(it.head, key_limit - p.window + 1) : 0;
           few = it.few;
+          if constexpr (!std::is_same<Out, T>::value) {
+            const float4 f = __ldcg(p.head_factor + it.b * p.Hkv + it.hkv);
+            const int tok = fdiv(r_in, p.d_pack);
+            const long long row = (static_cast<long long>(it.b) * p.Hq + it.hq) * p.pack + r_in - tok * p.pack;
+            // never 0: a hidden score is -inf times this
+            if (qi < it.rows && tok < p.tokens) scale_log2 = fmaxf(p.scale_log2 * f.y * __ldcg(p.q_factor + row * p.S + qi), 1.17549435e-38f);
+            v_factor = f.w;
+          }
         }
       }
       float m_use = -INFINITY, l = 0.f;
@@ -485,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
           mx3 = max3(mx3, __uint_as_float(s[c + 6]), __uint_as_float(s[c + 7]));
         }
         const float rowmax = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-        const float m_new = fmaxf(m_use, rowmax * p.scale_log2);
+        const float m_new = fmaxf(m_use, rowmax * scale_log2);
         const bool grow = m_new > m_use + kRescaleThreshold;  // true on the first tile (m_use = -inf)
         float alpha = 1.f;
         if (grow) {
@@ -506,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
         }
         const float neg_mref = (m_use == -INFINITY) ? 0.f : -m_use;
         // packed fp32x2 arithmetic: one FMA and one ADD instruction per two elements; P leaves in two halves of 64 keys
-        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+        const float2 sc2 = make_float2(scale_log2, scale_log2);
         const float2 nm2 = make_float2(neg_mref, neg_mref);
         float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -542,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
       const bool row_ok = SEQ ? qi < it.rows && tok < p.tokens : qi < p.S;
       if (my_nt > 0) {
         if (handed > 0 && !mbar_wait(&stat_empty[t], (handed - 1) & 1, ctx, 411)) { ok = false; break; }
-        stat[t * BQ + r_in] = (p.kv_splits > 1) ? 1.f : ((l > 0.f) ? 1.f / l : 0.f);
+        stat[t * BQ + r_in] = (p.kv_splits > 1) ? v_factor : ((l > 0.f) ? v_factor / l : 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&stat_full[t]);
         ++handed;
@@ -615,7 +630,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
             if (row_ok) {
               uint4* d = reinterpret_cast<uint4*>(p.part_o + prow * D + c * 32);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) d[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              for (int e = 0; e < 8; ++e) {
+                if constexpr (!std::is_same<Out, T>::value) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) o[4 * e + k] = __float_as_uint(__uint_as_float(o[4 * e + k]) * f);
+                }
+                d[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              }
             }
           }
           continue;
@@ -637,10 +658,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
           uint8_t* row = stage + (c >> 1) * (BQ * 128) + r_in * 128;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint4 v = make_uint4(Pack2<T>::pack(__uint_as_float(o[8 * k]) * f, __uint_as_float(o[8 * k + 1]) * f),
-                                       Pack2<T>::pack(__uint_as_float(o[8 * k + 2]) * f, __uint_as_float(o[8 * k + 3]) * f),
-                                       Pack2<T>::pack(__uint_as_float(o[8 * k + 4]) * f, __uint_as_float(o[8 * k + 5]) * f),
-                                       Pack2<T>::pack(__uint_as_float(o[8 * k + 6]) * f, __uint_as_float(o[8 * k + 7]) * f));
+            const uint4 v = make_uint4(Pack2<Out>::pack(__uint_as_float(o[8 * k]) * f, __uint_as_float(o[8 * k + 1]) * f),
+                                       Pack2<Out>::pack(__uint_as_float(o[8 * k + 2]) * f, __uint_as_float(o[8 * k + 3]) * f),
+                                       Pack2<Out>::pack(__uint_as_float(o[8 * k + 4]) * f, __uint_as_float(o[8 * k + 5]) * f),
+                                       Pack2<Out>::pack(__uint_as_float(o[8 * k + 6]) * f, __uint_as_float(o[8 * k + 7]) * f));
             *reinterpret_cast<uint4*>(row + ((((c & 1) * 4 + k) ^ (r_in & 7)) << 4)) = v;
           }
         }
@@ -654,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
               tma_store_commit();
             }
           } else {  // rows behind the sequence's last one stay as they are
-            T* o = static_cast<T*>(p.o2) + it.b * p.o_stride[0] + static_cast<long long>(it.hq) * p.pack * p.o_stride[1];
+            Out* o = static_cast<Out*>(p.o2) + it.b * p.o_stride[0] + static_cast<long long>(it.hq) * p.pack * p.o_stride[1];
             for (int i = tid; i < (it.rows - q0t) * p.pack * (D / 8); i += 128) {
               const int r = i / (D / 8), c = i % (D / 8);
               const int tok = fdiv(r, p.d_pack);
@@ -743,17 +764,17 @@ __global__ void attn_combine_kernel(const float* __restrict__ part_o, const floa
   }
 }
 
-template <typename T, int D, bool SEQ>
+template <typename T, int D, bool SEQ, typename Out>
 int launch_one(const Attn2Params& p, dim3 grid, int num_sms, cudaStream_t stream) {
   static bool attr_set[32] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_set[dev & 31]) {
-    if (cudaFuncSetAttribute(attn_fwd2_kernel<T, D, SEQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem2<D>::kTotal) != cudaSuccess)
+    if (cudaFuncSetAttribute(attn_fwd2_kernel<T, D, SEQ, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem2<D>::kTotal) != cudaSuccess)
       return TB200_ERR_CUDA;
     attr_set[dev & 31] = true;
   }
-  if (launch_chained(attn_fwd2_kernel<T, D, SEQ>, grid, dim3(kThreads, 1, 1), Smem2<D>::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
+  if (launch_chained(attn_fwd2_kernel<T, D, SEQ, Out>, grid, dim3(kThreads, 1, 1), Smem2<D>::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
   if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
   if (p.kv_splits > 1) {
     const int heads = SEQ ? p.Hq * p.pack : p.Hq;
@@ -763,9 +784,9 @@ int launch_one(const Attn2Params& p, dim3 grid, int num_sms, cudaStream_t stream
     CombineSeq seq;
     seq.q_rows = p.q_rows;
     for (int i = 0; i < 3; ++i) seq.o_stride[i] = p.o_stride[i];
-    auto* combine = SEQ && p.kv_splits <= 4 ? attn_combine_kernel<T, D, SEQ, SEQ ? 4 : 16> : attn_combine_kernel<T, D, SEQ, 16>;
+    auto* combine = SEQ && p.kv_splits <= 4 ? attn_combine_kernel<Out, D, SEQ, SEQ ? 4 : 16> : attn_combine_kernel<Out, D, SEQ, 16>;
     if (launch_chained(combine, dim3(static_cast<unsigned>(blocks), 1, 1), dim3(256, 1, 1), 0, stream, p.part_o, p.part_ml,
-                       static_cast<T*>(p.o2), p.lse2, p.kv_splits, p.B, heads, p.S, seq) != cudaSuccess)
+                       static_cast<Out*>(p.o2), p.lse2, p.kv_splits, p.B, heads, p.S, seq) != cudaSuccess)
       return TB200_ERR_CUDA;
     if (cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
   }
@@ -785,10 +806,16 @@ int finish_launch(Attn2Params& p, int dtype, int D, const DeviceState* st, cudaS
   p.d_hq = make_fastdiv(static_cast<uint32_t>(p.Hq));
   p.d_group = make_fastdiv(static_cast<uint32_t>(p.Hq / p.Hkv));
   const dim3 grid(static_cast<unsigned>(p.n_items < st->num_sms ? p.n_items : st->num_sms), 1, 1);  // persistent: one CTA per SM
-  if (dtype == TB200_BF16) {
-    return D == 128 ? launch_one<__nv_bfloat16, 128, SEQ>(p, grid, st->num_sms, stream) : launch_one<__nv_bfloat16, 64, SEQ>(p, grid, st->num_sms, stream);
+  if constexpr (SEQ) {
+    if (p.q_factor != nullptr)   // computed in fp16, written in bf16
+      return D == 128 ? launch_one<__half, 128, SEQ, __nv_bfloat16>(p, grid, st->num_sms, stream)
+                      : launch_one<__half, 64, SEQ, __nv_bfloat16>(p, grid, st->num_sms, stream);
   }
-  return D == 128 ? launch_one<__half, 128, SEQ>(p, grid, st->num_sms, stream) : launch_one<__half, 64, SEQ>(p, grid, st->num_sms, stream);
+  if (dtype == TB200_BF16) {
+    return D == 128 ? launch_one<__nv_bfloat16, 128, SEQ, __nv_bfloat16>(p, grid, st->num_sms, stream)
+                    : launch_one<__nv_bfloat16, 64, SEQ, __nv_bfloat16>(p, grid, st->num_sms, stream);
+  }
+  return D == 128 ? launch_one<__half, 128, SEQ, __half>(p, grid, st->num_sms, stream) : launch_one<__half, 64, SEQ, __half>(p, grid, st->num_sms, stream);
 }
 
 
@@ -877,6 +904,8 @@ int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
   p.B = a.B; p.S = a.S; p.Hq = a.Hq / a.pack; p.Hkv = a.Hkv; p.kv_len = a.cache_len; p.causal = 1;
   p.cache_len = a.cache_len; p.window = a.window; p.sinks = a.sinks;
   p.kv_lens = a.kv_lens; p.q_rows = a.q_rows;
+  p.q_factor = a.q_factor;
+  p.head_factor = reinterpret_cast<const float4*>(a.head_factor);
   p.scale_log2 = a.sm_scale * kLog2e;
   p.o2 = a.o;
   for (int i = 0; i < 3; ++i) p.o_stride[i] = a.o_stride[i];

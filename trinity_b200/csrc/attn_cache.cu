@@ -600,8 +600,9 @@ struct AttnPlan {
   int unit_rows = 8;         // decode: query rows of a unit
   int stretches = 0;
   int pack = 1, kv_splits = 1;   // prompt
-  size_t part_o = 0, part_ml = 0, split = 0, cache16 = 0;   // bytes; cache16: of one of the two caches
-  size_t total() const { return part_o + part_ml + split + 2 * cache16; }
+  size_t part_o = 0, part_ml = 0, split = 0;               // bytes
+  size_t cache16 = 0, q16 = 0, q_factor = 0, head_factor = 0;   // prompt on 4 bits: one of the two caches; bf16: q and the factors
+  size_t total() const { return part_o + part_ml + split + 2 * cache16 + q16 + q_factor + head_factor; }
 };
 // A window as long as the cache hides nothing; first positions matter only beside a window.
 int window_of(const tb200_cache_attn_args* a) { return a->window < a->cache_len ? a->window : 0; }
@@ -624,6 +625,12 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
       pl.part_ml = align_up(prows * 2 * sizeof(float), 256);
     }
     if (kv4) pl.cache16 = align_up(static_cast<size_t>(a->batch) * a->n_kv_heads * a->cache_len * a->head_dim * 2, 256);
+    if (kv4 && a->dtype == TB200_BF16) {
+      const size_t q_rows = static_cast<size_t>(a->batch) * a->n_q_heads * a->rows;
+      pl.q16 = align_up(q_rows * a->head_dim * 2, 256);
+      pl.q_factor = align_up(q_rows * sizeof(float), 256);
+      pl.head_factor = align_up(static_cast<size_t>(a->batch) * a->n_kv_heads * 4 * sizeof(float), 256);
+    }
     return pl;
   }
   pl.unit_rows = unit_rows_for(rows, kv4);
@@ -712,10 +719,25 @@ int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, con
   s.k_cache = a->k_cache; s.v_cache = a->v_cache;
   for (int i = 0; i < 3; ++i) { s.q_stride[i] = a->q_stride[i]; s.o_stride[i] = a->o_stride[i]; s.k_stride[i] = a->k_stride[i]; s.v_stride[i] = a->v_stride[i]; }
   if (kv4) {
-    uint8_t* k16 = ws + pl.part_o + pl.part_ml;
-    const int status = launch_kv4_read_seen(*a, p.window, p.sinks, k16, k16 + pl.cache16, num_sms, stream);
+    Kv4PromptOperands to;
+    uint8_t* at = ws + pl.part_o + pl.part_ml;
+    to.k16 = at;
+    to.v16 = at += pl.cache16;
+    at += pl.cache16;
+    if (a->dtype == TB200_BF16) {
+      to.q16 = at;
+      to.q_factor = reinterpret_cast<float*>(at += pl.q16);
+      to.head_factor = reinterpret_cast<float*>(at += pl.q_factor);
+      s.q = to.q16;
+      s.q_factor = to.q_factor;
+      s.head_factor = to.head_factor;
+      s.q_stride[2] = a->head_dim;
+      s.q_stride[1] = static_cast<int64_t>(a->rows) * a->head_dim;
+      s.q_stride[0] = s.q_stride[1] * a->n_q_heads;
+    }
+    const int status = launch_kv4_prompt_operands(*a, p.window, p.sinks, to, num_sms, stream);
     if (status != TB200_OK) return status;
-    s.k_cache = k16; s.v_cache = k16 + pl.cache16;
+    s.k_cache = to.k16; s.v_cache = to.v16;
     s.k_stride[2] = s.v_stride[2] = a->head_dim;
     s.k_stride[1] = s.v_stride[1] = static_cast<int64_t>(a->cache_len) * a->head_dim;
     s.k_stride[0] = s.v_stride[0] = s.k_stride[1] * a->n_kv_heads;

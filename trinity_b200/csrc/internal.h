@@ -195,6 +195,8 @@ struct AttnSeqLaunch {
   int64_t q_stride[3] = {}, k_stride[3] = {}, v_stride[3] = {}, o_stride[3] = {};
   const int32_t* kv_lens = nullptr;
   const int32_t* q_rows = nullptr;
+  const float* q_factor = nullptr;  // not null: q and the caches are fp16, divided by these powers of two, o is bf16; (B,Hq,S)
+  const float* head_factor = nullptr;   // (B,Hkv,4): .y of K, .w of V
   int pack = 1;                     // query heads per query tile (attn_seq_pack)
   int kv_splits = 1;
   float* part_o = nullptr;          // (kv_splits,B,Hq,S,D) fp32
@@ -260,8 +262,17 @@ int launch_kv_compact(const tb200_kv_compact_args& a, cudaStream_t stream);
 // Element strides of the (batch, head, row) axes with extents ext: steps of 16 bytes, and with `written` rows that do
 // not overlap.  Axes of one element are not looked at.
 int check_strides(const int64_t (&stride)[3], const int64_t (&ext)[3], int head_dim, bool written);
-// The positions of a 4-bit cache that some query row of its sequence sees, as contiguous 16-bit caches
-// (B, Hkv, cache_len, D); the other positions of k16 and v16 are left as they are.
-int launch_kv4_read_seen(const tb200_cache_attn_args& a, int window, int sinks, void* k16, void* v16, int num_sms, cudaStream_t stream);
+// A prompt's operands out of a 4-bit cache: the positions that some query row of its sequence sees as contiguous 16-bit
+// caches (B, Hkv, cache_len, D), other positions left as they are.  fp16: the values, rounded.  bf16: in fp16, divided by a
+// power of two per head (head_factor (B, Hkv, 4): 1 / factor and factor of K, of V), and q (B, Hq, rows, D) likewise by one
+// per row (q_factor); q16, q_factor and head_factor are not used for fp16.
+struct Kv4PromptOperands {
+  void* k16 = nullptr;
+  void* v16 = nullptr;
+  void* q16 = nullptr;
+  float* q_factor = nullptr;
+  float* head_factor = nullptr;
+};
+int launch_kv4_prompt_operands(const tb200_cache_attn_args& a, int window, int sinks, const Kv4PromptOperands& to, int num_sms, cudaStream_t stream);
 
 }  // namespace tb200

@@ -27,6 +27,7 @@ struct RowsParams {
   uint8_t* meta[2];
   const int32_t* q_rows;    // SEEN
   int q_rows_max, window, sinks;
+  const float4* head_factor;
 };
 
 template <typename T> struct Bits;   // a 16-bit value and its raw bits
@@ -179,21 +180,153 @@ __global__ void __launch_bounds__(kThreads, 4) kv4_append_kernel(const __grid_co
   }
 }
 
-// SEEN: only the positions that some query row of the sequence sees (a prompt's attention reads the 16-bit rows next).
+// The positions some query row of sequence b sees: [low, n) and those below few.
+struct SeenRows {
+  int low, few;
+};
+__device__ __forceinline__ SeenRows seen_rows(const RowsParams& p, int b, int n) {
+  const int r = p.q_rows ? max(0, min(p.q_rows[b], p.q_rows_max)) : p.q_rows_max;
+  SeenRows s;
+  s.low = r == 0 ? n : p.window > 0 ? n - r - p.window + 1 : 0;
+  s.few = r > 0 ? p.sinks : 0;
+  return s;
+}
+
+// Eight codes as fp16 values of (lo + c s) * down.
+__device__ __forceinline__ uint4 decode8_scaled(uint32_t word, uint32_t meta, float down) {
+  const float2 sl = Pack2<__nv_bfloat16>::unpack(meta);
+  const float s = sl.x * down, lo = sl.y * down;
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = Pack2<__half>::pack(fmaf(static_cast<float>((word >> (8 * i)) & 15u), s, lo), fmaf(static_cast<float>((word >> (8 * i + 4)) & 15u), s, lo));
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// A power of two that brings `top` to [2^to, 2^(to + 1)), and its inverse.
+__device__ __forceinline__ float2 power_for(float top, int to) {
+  const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 40);
+  return make_float2(__uint_as_float(static_cast<uint32_t>(254 + to - ex) << 23), __uint_as_float(static_cast<uint32_t>(ex - to) << 23));
+}
+
+// bf16 prompts on a 4-bit cache: the powers of two.  CTAs (i < kv heads, b): the largest magnitude among the seen rows of one
+// (sequence, kv head) of K and of V, from s and lo alone; the CTAs behind them: rows of q, a warp each.  Infinities and NaN do
+// not count.
+struct FactorParams {
+  RowsParams rows;
+  int batch, q_heads;
+  const uint8_t* q;
+  long long q_stride[3];
+  uint8_t* q16;
+  float* q_factor;
+  float4* head_factor;
+};
+constexpr int kFactorThreads = 1024;
+template <int D>
+__global__ void __launch_bounds__(kFactorThreads) kv4_factors_kernel(const __grid_constant__ FactorParams f) {
+  const RowsParams& p = f.rows;
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float red[2][kFactorThreads / 32];
+  for (int b = blockIdx.y; b < f.batch; b += gridDim.y) {
+    if (blockIdx.x < p.heads) {
+      const long long bh = static_cast<long long>(b) * p.heads + blockIdx.x;
+      const int n = max(0, min(p.n_rows[b], p.rows));
+      const SeenRows seen = seen_rows(p, b, n);
+      const int low = max(seen.low, 0), few = min(seen.few, low);
+      float top[2] = {0.f, 0.f};
+#pragma unroll 4
+      for (int i = threadIdx.x; i < few + n - low; i += kFactorThreads) {
+        const long long crow = bh * p.cache_len + (i < few ? i : i - few + low);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t u[D / 64];
+          if constexpr (D == 128) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p.meta[w]) + crow);
+            u[0] = v.x; u[1] = v.y;
+          } else {
+            u[0] = __ldg(reinterpret_cast<const uint32_t*>(p.meta[w]) + crow);
+          }
+#pragma unroll
+          for (int g = 0; g < D / 64; ++g) {
+            const float2 sl = Pack2<__nv_bfloat16>::unpack(u[g]);
+            const float x = fmaxf(fabsf(sl.y), fabsf(fmaf(15.f, sl.x, sl.y)));
+            top[w] = fmaxf(top[w], x < INFINITY ? x : 0.f);
+          }
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], d));
+        if (lane == 0) red[w][warp] = top[w];
+      }
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          top[w] = red[w][lane];
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], d));
+        }
+        const float2 k = power_for(top[0], 14), v = power_for(top[1], 14);   // below 2^15: fp16 ends at 65504
+        if (lane == 0) f.head_factor[bh] = make_float4(k.x, k.y, v.x, v.y);
+      }
+      __syncthreads();
+      continue;
+    }
+    constexpr int V = D / 32;   // columns per lane
+    const int rows = f.q_heads * p.q_rows_max, stride = (gridDim.x - p.heads) * (kFactorThreads / 32);
+    const int live = p.q_rows ? p.q_rows[b] : p.q_rows_max;
+    for (int row = (blockIdx.x - p.heads) * (kFactorThreads / 32) + warp; row < rows; row += stride) {
+      const int h = row / p.q_rows_max, i = row - h * p.q_rows_max;
+      if (i >= live) continue;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(f.q + 2 * (b * f.q_stride[0] + h * f.q_stride[1] + i * f.q_stride[2])) + lane * (V / 2);
+      float2 x[V / 2];
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) {
+        x[e] = Pack2<__nv_bfloat16>::unpack(src[e]);
+        const float m = fmaxf(fabsf(x[e].x), fabsf(x[e].y));
+        top = fmaxf(top, m < INFINITY ? m : 0.f);
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float2 pw = power_for(top, 3);
+      const long long out = static_cast<long long>(b) * rows + row;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(f.q16 + out * D * 2) + lane * (V / 2);
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) dst[e] = Pack2<__half>::pack(x[e].x * pw.x, x[e].y * pw.x);
+      if (lane == 0) f.q_factor[out] = pw.y;
+    }
+  }
+}
+
+// SEEN: only the positions that some query row of the sequence sees (a prompt's attention reads the 16-bit rows next), bf16 as
+// scaled fp16.
 template <typename T, int D, bool SEEN>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constant__ RowsParams p) {
   using S = RowsShape<D>;
-  if constexpr (SEEN) pdl_launch_dependents();
+  if constexpr (SEEN) {
+    pdl_launch_dependents();
+    pdl_wait();   // the factors
+  }
   const int r_in = threadIdx.x / S::kLanes, lane = threadIdx.x % S::kLanes;
   const int chunk = (lane >> 2) * 8 + (lane & 3);
   for (long long u = blockIdx.x; u < p.units; u += gridDim.x) {
     const Unit x = find_unit(p, u, S::kUnitRows);
     if (x.row0 >= x.n) continue;
     int low = 0, few = 0;
+    float down[2] = {1.f, 1.f};
     if constexpr (SEEN) {
-      const int r = p.q_rows ? max(0, min(p.q_rows[x.b], p.q_rows_max)) : p.q_rows_max;
-      low = r == 0 ? x.n : p.window > 0 ? x.n - r - p.window + 1 : 0;
-      few = r > 0 ? p.sinks : 0;
+      const SeenRows seen = seen_rows(p, x.b, x.n);
+      low = seen.low;
+      few = seen.few;
+      if constexpr (IsBf16<T>::value) {
+        const float4 f = __ldcg(p.head_factor + x.bh);
+        down[0] = f.x;
+        down[1] = f.z;
+      }
     }
     uint32_t word[kPerThread][2][2], m[kPerThread][2];
     bool live[kPerThread];
@@ -220,8 +353,13 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constan
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         uint4* dst = reinterpret_cast<uint4*>(p.x[w] + 2 * (x.b * p.stride[w][0] + x.h * p.stride[w][1] + row * p.stride[w][2])) + chunk;
-        dst[0] = Kv4Decode<T>::decode8(word[k][w][0], m[k][w]);
-        dst[4] = Kv4Decode<T>::decode8(word[k][w][1], m[k][w]);
+        if constexpr (SEEN && IsBf16<T>::value) {
+          dst[0] = decode8_scaled(word[k][w][0], m[k][w], down[w]);
+          dst[4] = decode8_scaled(word[k][w][1], m[k][w], down[w]);
+        } else {
+          dst[0] = Kv4Decode<T>::decode8(word[k][w][0], m[k][w]);
+          dst[4] = Kv4Decode<T>::decode8(word[k][w][1], m[k][w]);
+        }
       }
     }
   }
@@ -305,12 +443,13 @@ int launch_rows(const RowsParams& p, int dtype, int head_dim, int batch, RowsWor
 
 }  // namespace
 
-int launch_kv4_read_seen(const tb200_cache_attn_args& a, int window, int sinks, void* k16, void* v16, int num_sms, cudaStream_t stream) {
+int launch_kv4_prompt_operands(const tb200_cache_attn_args& a, int window, int sinks, const Kv4PromptOperands& to, int num_sms, cudaStream_t stream) {
   RowsParams p;
   memset(&p, 0, sizeof(p));
   p.n_rows = a.kv_lens; p.rows = a.cache_len; p.heads = a.n_kv_heads; p.cache_len = a.cache_len;
-  p.x[0] = static_cast<uint8_t*>(k16);
-  p.x[1] = static_cast<uint8_t*>(v16);
+  p.n_bh = static_cast<long long>(a.batch) * a.n_kv_heads;
+  p.x[0] = static_cast<uint8_t*>(to.k16);
+  p.x[1] = static_cast<uint8_t*>(to.v16);
   for (int w = 0; w < 2; ++w) {
     p.stride[w][2] = a.head_dim;
     p.stride[w][1] = static_cast<long long>(a.cache_len) * a.head_dim;
@@ -321,6 +460,25 @@ int launch_kv4_read_seen(const tb200_cache_attn_args& a, int window, int sinks, 
   p.meta[0] = static_cast<uint8_t*>(const_cast<void*>(a.k_meta));
   p.meta[1] = static_cast<uint8_t*>(const_cast<void*>(a.v_meta));
   p.q_rows = a.q_rows; p.q_rows_max = a.rows; p.window = window; p.sinks = sinks;
+  p.head_factor = reinterpret_cast<const float4*>(to.head_factor);
+  if (a.dtype == TB200_BF16) {
+    FactorParams f;
+    f.rows = p;
+    f.q = static_cast<const uint8_t*>(a.q);
+    for (int i = 0; i < 3; ++i) f.q_stride[i] = a.q_stride[i];
+    f.q16 = static_cast<uint8_t*>(to.q16);
+    f.q_factor = to.q_factor;
+    f.head_factor = reinterpret_cast<float4*>(to.head_factor);
+    f.q_heads = a.n_q_heads;
+    f.batch = a.batch;
+    // a warp per row of q, at most sixteen CTAs' worth of them per SM over the whole batch
+    const long long q_ctas = (static_cast<long long>(a.n_q_heads) * a.rows + kFactorThreads / 32 - 1) / (kFactorThreads / 32);
+    const long long most = static_cast<long long>(num_sms) * 16 / a.batch + 1;
+    const dim3 grid(static_cast<unsigned>(a.n_kv_heads + (q_ctas < most ? q_ctas : most)), static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535));
+    const cudaError_t e = a.head_dim == 128 ? launch_chained(kv4_factors_kernel<128>, grid, dim3(kFactorThreads), 0, stream, f)
+                                            : launch_chained(kv4_factors_kernel<64>, grid, dim3(kFactorThreads), 0, stream, f);
+    if (e != cudaSuccess || cudaGetLastError() != cudaSuccess) return TB200_ERR_CUDA;
+  }
   return launch_rows(p, a.dtype, a.head_dim, a.batch, kReadSeen, num_sms, stream);
 }
 
