@@ -629,13 +629,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
             }
             if (row_ok) {
               uint4* d = reinterpret_cast<uint4*>(p.part_o + prow * D + c * 32);
+              if constexpr (SEQ) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                if constexpr (!std::is_same<Out, T>::value) {
+                for (int e = 0; e < 32; e += 8) {   // whole 32-byte sectors: a row per thread, nothing else would fill them
+                  float y[8];
 #pragma unroll
-                  for (int k = 0; k < 4; ++k) o[4 * e + k] = __float_as_uint(__uint_as_float(o[4 * e + k]) * f);
+                  for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(o[e + k]) * f;
+                  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(d + e / 4), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]),
+                               "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]) : "memory");
                 }
-                d[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
               }
             }
           }

@@ -602,7 +602,8 @@ struct AttnPlan {
   int pack = 1, kv_splits = 1;   // prompt
   size_t part_o = 0, part_ml = 0, split = 0;               // bytes
   size_t cache16 = 0, q16 = 0, q_factor = 0, head_factor = 0;   // prompt on 4 bits: one of the two caches; bf16: q and the factors
-  size_t total() const { return part_o + part_ml + split + 2 * cache16 + q16 + q_factor + head_factor; }
+  // + what brings the caller's address up to a multiple of 256
+  size_t total() const { return part_o == 0 && cache16 == 0 ? 0 : part_o + part_ml + split + 2 * cache16 + q16 + q_factor + head_factor + 256; }
 };
 // A window as long as the cache hides nothing; first positions matter only beside a window.
 int window_of(const tb200_cache_attn_args* a) { return a->window < a->cache_len ? a->window : 0; }
@@ -703,8 +704,7 @@ int launch_combine(const CacheAttnParams& p, int head_dim, int unit_rows, cudaSt
   return head_dim == 128 ? launch_combine<T, 128>(p, unit_rows, stream) : launch_combine<T, 64>(p, unit_rows, stream);
 }
 
-int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, const CacheAttnParams& p, int num_sms, cudaStream_t stream) {
-  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, const CacheAttnParams& p, uint8_t* ws, int num_sms, cudaStream_t stream) {
   AttnSeqLaunch s;
   s.dtype = a->dtype;
   s.B = a->batch; s.S = a->rows; s.Hq = a->n_q_heads; s.Hkv = a->n_kv_heads; s.D = a->head_dim; s.cache_len = a->cache_len;
@@ -756,13 +756,13 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   CacheAttnParams p = make_params(a, st);
   const AttnPlan pl = plan_attn(a, kv4, st->num_sms);
   if (pl.total() > 0 && (!a->workspace || a->workspace_bytes < pl.total())) return TB200_ERR_WORKSPACE;
-  if (!aligned16(a->workspace)) return TB200_ERR_INVALID;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(align_up(reinterpret_cast<size_t>(a->workspace), 256));
   ChainScope chain;
-  if (pl.prompt) return run_prompt(a, kv4, pl, p, st->num_sms, stream);
+  if (pl.prompt) return run_prompt(a, kv4, pl, p, ws, st->num_sms, stream);
   p.stretches = pl.stretches;
-  p.part_o = static_cast<float*>(a->workspace);
-  p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
-  p.split = reinterpret_cast<int4*>(static_cast<uint8_t*>(a->workspace) + pl.part_o + pl.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + pl.part_o);
+  p.split = reinterpret_cast<int4*>(ws + pl.part_o + pl.part_ml);
   // positions on the line of tiles are 32-bit numbers
   const int64_t rows = static_cast<int64_t>(a->rows) * p.group;
   if ((rows / pl.unit_rows + 1) * a->n_kv_heads * a->batch * static_cast<double>(a->cache_len / 16 + 2) >= 2147483648.0) return TB200_ERR_UNSUPPORTED;
