@@ -211,6 +211,11 @@ SHAPES = [  # b, hq, hkv, d, s, cache length, lens, rows, window, sinks
     (2, 12, 2, 128, 100, 1000, [900, 100], [100, 64], 150, 20),
     (3, 32, 8, 128, 300, 2048, [2000, 300, 20], [300, 290, 300], 700, 4),
     (2, 16, 2, 64, 33, 3000, [3000, 1029], [33, 32], 0, 0),
+    (2, 8, 2, 128, 1, 30000, [30000, 777], [1, 1], 0, 0),
+    (3, 12, 2, 64, 2, 40000, [40000, 9, 20011], [2, 1, 2], 0, 0),
+    (2, 20, 2, 128, 1, 24000, [11, 23999], [1, 1], 12000, 100),
+    (70, 16, 8, 64, 1, 600, [600 - 8 * i for i in range(70)], [1] * 69 + [0], 0, 0),
+    (40, 8, 8, 128, 2, 400, [10 * i for i in range(40)], [2] * 40, 0, 0),
 ]
 
 
@@ -290,9 +295,10 @@ def test_rows_nobody_sees_may_hold_anything(kv4, s):
     assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("length", [2048, 24000])
 @pytest.mark.parametrize("kv4", [True, False])
-def test_same_bits_every_time_and_from_a_graph(kv4):
-    shape = (5, 16, 4, 128, 1, 2048, [2048, 77, 1500, 0, 640], [1] * 5, 0, 0)
+def test_same_bits_every_time_and_from_a_graph(kv4, length):
+    shape = (5, 16, 4, 128, 1, length, [length, 77, 1500, 0, 640], [1] * 5, 0, 0)
     b, hq, hkv, d, s, length, lens, rows, window, sinks = shape
     dt = torch.float16
     q, out, kw = case(shape, dt)
@@ -407,7 +413,7 @@ def test_offsets_past_32_bits():
 
 def test_two_streams_at_once():
     """Calls on two streams have workspaces of their own."""
-    shape = (4, 32, 8, 128, 1, 4096, [4096, 4000, 100, 2222], [1] * 4, 0, 0)
+    shape = (4, 32, 8, 128, 1, 16384, [16384, 4000, 100, 9999], [1] * 4, 0, 0)
     b, hq, hkv, d, s, length, lens, rows, window, sinks = shape
     caches = [filled_cache(b, hkv, length, d, torch.bfloat16, i) for i in range(2)]
     q, _, kw = case(shape, torch.bfloat16)

@@ -68,7 +68,8 @@ template <int D, int NT, int H> struct DecSmem {
   static constexpr int kBarOff = kWarps * kRing;
   // the merge buffers take the place of the rings, which are empty by then
   static_assert(MergeSmem<D, NT>::kBytes <= kBarOff, "the merge buffers must fit where the rings were");
-  static constexpr int kTotal = kBarOff + kWarps * kStages * 8 + 16;
+  static constexpr int kShareOff = kBarOff + kWarps * kStages * 8 + 16;
+  static constexpr int kTotal = kShareOff + ShareSmem<D, kR>::kBytes;
 };
 
 template <typename T, int D, int NT, int H>
@@ -458,10 +459,10 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
         }
       }
     __syncthreads();
-    merge_segment<T, D, NT, H>(p, smem, wk, sg);
+    merge_segment<T, D, NT, H>(p, smem, smem + L::kShareOff, wk, sg);
     fence_proxy_async_smem();   // the next bulk copies overwrite what was just read and written
     __syncthreads();
-    wk.x += v1 - v0;
+    wk.advance(p, sg);
   }
 }
 
@@ -595,9 +596,13 @@ int kv4_ctas(int head_dim, int unit_rows) {
   return unit_rows == 4 ? DecShape<64, 1, 2>::kCtas : unit_rows == 8 ? DecShape<64, 1, 1>::kCtas : DecShape<64, 2, 1>::kCtas;
 }
 
+constexpr int kClusterKeys = 256;
+
 struct AttnPlan {
   bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
   int unit_rows = 8;         // decode: query rows of a unit
+  int row_tiles = 1;         // units per (sequence, kv head) at most
+  int cluster = 0;           // CTAs per unit, 0: the line
   int stretches = 0;
   int pack = 1, kv_splits = 1;   // prompt
   size_t part_o = 0, part_ml = 0, split = 0;               // bytes
@@ -635,7 +640,20 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
     return pl;
   }
   pl.unit_rows = unit_rows_for(rows, kv4);
-  pl.stretches = kv4 ? num_sms * kv4_ctas(a->head_dim, pl.unit_rows) : cache16_stretches(num_sms);
+  pl.row_tiles = static_cast<int>((rows + pl.unit_rows - 1) / pl.unit_rows);
+  const int ctas = kv4 ? num_sms * kv4_ctas(a->head_dim, pl.unit_rows) : cache16_stretches(num_sms);
+  // A cluster per unit where the CTAs that are resident at a time can give every warp at most kClusterKeys keys; with more the
+  // line is faster, which does not care how long each sequence is.
+  const int64_t units = static_cast<int64_t>(a->batch) * a->n_kv_heads * pl.row_tiles;
+  int cluster = 1;
+  while (cluster < 8 && units * cluster * 2 <= ctas) cluster *= 2;
+  const int64_t keys = window > 0 && static_cast<int64_t>(window) + a->rows + sinks < a->cache_len ? static_cast<int64_t>(window) + a->rows + sinks : a->cache_len;
+  if (units <= ctas && keys <= static_cast<int64_t>(kClusterKeys) * kWarps * cluster) {
+    pl.cluster = cluster;
+    pl.stretches = static_cast<int>(units * cluster);
+    return pl;
+  }
+  pl.stretches = ctas;
   pl.part_o = align_up(static_cast<size_t>(pl.stretches) * 2 * pl.unit_rows * a->head_dim * sizeof(float), 256);
   pl.part_ml = align_up(static_cast<size_t>(pl.stretches) * 2 * pl.unit_rows * 2 * sizeof(float), 256);
   pl.split = align_up(static_cast<size_t>(pl.stretches) * sizeof(int4), 256);
@@ -674,8 +692,7 @@ int launch_decode(const CacheAttnParams& p, cudaStream_t stream) {
       return TB200_ERR_CUDA;
     attr_set[dev & 31] = true;
   }
-  if (launch_chained(cache_decode_kernel<T, D, NT, H>, dim3(p.stretches), dim3(kThreads), L::kTotal, stream, p) != cudaSuccess) return TB200_ERR_CUDA;
-  return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+  return launch_decode_grid(cache_decode_kernel<T, D, NT, H>, p, L::kTotal, stream, p);
 }
 template <typename T, int D>
 int run_kv4(const CacheAttnParams& p, int unit_rows, cudaStream_t stream) {
@@ -760,6 +777,8 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   ChainScope chain;
   if (pl.prompt) return run_prompt(a, kv4, pl, p, ws, st->num_sms, stream);
   p.stretches = pl.stretches;
+  p.row_tiles = pl.row_tiles;
+  p.cluster = pl.cluster;
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = reinterpret_cast<float*>(ws + pl.part_o);
   p.split = reinterpret_cast<int4*>(ws + pl.part_o + pl.part_ml);
@@ -769,7 +788,7 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   if (!kv4) status = launch_cache16(p, *a, pl.unit_rows, stream);
   else if (a->dtype == TB200_BF16) status = run_kv4<__nv_bfloat16>(p, a->head_dim, pl.unit_rows, stream);
   else status = run_kv4<__half>(p, a->head_dim, pl.unit_rows, stream);
-  if (status != TB200_OK) return status;
+  if (status != TB200_OK || pl.cluster > 0) return status;
   return launch_cache_combine(p, a->dtype, a->head_dim, pl.unit_rows, stream);
 }
 

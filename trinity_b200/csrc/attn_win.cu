@@ -26,7 +26,8 @@ template <int D, int NT> struct Smem16 {
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kBarOff = kWarps * kStages * kStage;
   static_assert(MergeSmem<D, NT>::kBytes <= kBarOff, "the merge buffers must fit where the rings were");
-  static constexpr int kTotal = kBarOff + kWarps * kStages * 8 + 16 + 1024;   // + slack to align the base to 1 KiB
+  static constexpr int kShareOff = kBarOff + kWarps * kStages * 8 + 16;
+  static constexpr int kTotal = kShareOff + ShareSmem<D, 8 * NT>::kBytes + 1024;   // + slack to align the base to 1 KiB
 };
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -259,10 +260,10 @@ __global__ void __launch_bounds__(kThreads, 2) cache_decode16_kernel(const __gri
         }
       }
     __syncthreads();
-    merge_segment<T, D, NT, 1>(p, smem, wk, sg);
+    merge_segment<T, D, NT, 1>(p, smem, smem + L::kShareOff, wk, sg);
     fence_proxy_async_smem();   // the next copies overwrite what was just read and written
     __syncthreads();
-    wk.x += sg.v1 - sg.v0;
+    wk.advance(p, sg);
   }
 }
 
@@ -276,8 +277,7 @@ int launch16(const CacheAttnParams& p, const CacheMaps& maps, cudaStream_t strea
     if (cudaFuncSetAttribute(cache_decode16_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) != cudaSuccess) return TB200_ERR_CUDA;
     attr_set[dev & 31] = true;
   }
-  if (launch_chained(cache_decode16_kernel<T, D, NT>, dim3(p.stretches), dim3(kThreads), L::kTotal, stream, p, maps) != cudaSuccess) return TB200_ERR_CUDA;
-  return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+  return launch_decode_grid(cache_decode16_kernel<T, D, NT>, p, L::kTotal, stream, p, maps);
 }
 
 template <typename T>

@@ -8,6 +8,9 @@
 //            of the lengths.  A unit that lies within one CTA's stretch is finished there; the others leave a partial
 //            result (accumulator, maximum, sum) per stretch, which cache_combine_kernel merges in the order of the keys.
 //   warp     takes every fourth tile of a stretch.
+//   cluster  with few keys a unit is one cluster's instead: C CTAs (1, 2, 4 or 8) share its tiles evenly and merge their
+//            results through distributed shared memory.  One launch, no scratch: one token on 1037 positions, 32/8 heads,
+//            takes CLUSTER_NOTE.
 #pragma once
 
 #include <math.h>
@@ -25,6 +28,7 @@ constexpr int kThreads = kWarps * 32;
 struct CacheAttnParams {
   int B, S, Hq, Hkv, group, cache_len, window, sinks;
   int row_tiles;             // units per (sequence, kv head) at most
+  int cluster;               // 0: the line; else CTAs per unit
   float scale_log2;
   const uint8_t* q;
   uint8_t* o;
@@ -123,7 +127,25 @@ struct Walk {
   Seq sq;
   int x, x_end;              // positions on the line: of the current segment, of the stretch's end
   int base, b;               // the line's position of the sequence's first tile; the sequence
+  Segment own;               // cluster: this CTA's share of its unit
   __device__ __forceinline__ bool begin(const CacheAttnParams& p, int tile, int unit_rows, int min_tiles) {   // false: nothing to do
+    if (p.cluster > 0) {
+      int u = static_cast<int>(blockIdx.x) / p.cluster;
+      const int rank = static_cast<int>(blockIdx.x) - u * p.cluster;
+      own.rt = u % p.row_tiles;
+      u /= p.row_tiles;
+      own.h = u % p.Hkv;
+      own.b = u / p.Hkv;
+      sq = load_seq(p, own.b, tile, unit_rows);
+      own.n_rows = sq.r * p.group;
+      if (own.rt * unit_rows >= own.n_rows) return false;   // every CTA of the cluster
+      const int per = (sq.tiles + p.cluster - 1) / p.cluster;
+      own.v0 = min(sq.tiles, rank * per);
+      own.v1 = min(sq.tiles, own.v0 + per);
+      x = 0;
+      x_end = 1;
+      return true;
+    }
     ln = walk_line(p, tile, unit_rows, min_tiles, blockIdx.x);
     x = ln.per * static_cast<int>(blockIdx.x);
     x_end = min(x + ln.per, ln.total);
@@ -136,7 +158,9 @@ struct Walk {
     sq = load_seq(p, b, tile, unit_rows);
     return true;
   }
+  __device__ __forceinline__ void advance(const CacheAttnParams& p, const Segment& s) { x += p.cluster > 0 ? 1 : s.v1 - s.v0; }
   __device__ __forceinline__ Segment segment(const CacheAttnParams& p, int tile, int unit_rows) {
+    if (p.cluster > 0) return own;
     while (x >= base + sq.tiles * sq.units) {
       base += sq.tiles * sq.units;
       sq = load_seq(p, ++b, tile, unit_rows);
@@ -162,14 +186,42 @@ template <int D, int NT> struct MergeSmem {
   static constexpr int kMlOff = kWarps * kR * kPitch * 4;    // float2 [warps][R] behind float [warps][R][pitch]
   static constexpr int kBytes = kMlOff + kWarps * kR * 8;
 };
-// The four warps' shares (of each row H from each warp) in a fixed order: into o where the unit lies in this stretch altogether, else into the stretch's
-// partial results.  Called by the whole CTA, with the shares written and a barrier behind them.
+// A CTA's share of a unit, for its cluster.
+template <int D, int R> struct ShareSmem {
+  static constexpr int kMlOff = R * D * 4;                   // float2 [R] behind float [R][D]
+  static constexpr int kBytes = kMlOff + R * 8;
+};
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t cluster_addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr) : "memory");
+  return v;
+}
+// Columns d to d + 3 of the unit's row m, divided by its sum, into o.
+template <typename T, int R>
+__device__ __forceinline__ void store_row(const CacheAttnParams& p, const Segment& sg, int m, int d, const float4& acc, float sum) {
+  const int mr = sg.rt * R + m;
+  if (mr >= sg.n_rows) return;
+  const float inv = sum > 0.f ? 1.f / sum : sum;   // 0: the row sees nothing; NaN stays
+  const int tok = mr / p.group;
+  T* op = reinterpret_cast<T*>(p.o) + sg.b * p.os[0] + (sg.h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + d;
+  *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
+}
+
+// The four warps' shares (of each row H from each warp) in a fixed order: into o where the unit lies in this stretch
+// altogether, else into the stretch's partial results, or with a cluster into `share` and from there, all CTAs' in the order
+// of their keys, into o.  Called by the whole CTA, with the shares written and a barrier behind them.
 template <typename T, int D, int NT, int H>
-__device__ __forceinline__ void merge_segment(const CacheAttnParams& p, const uint8_t* smem, const Walk& wk, const Segment& sg) {
+__device__ __forceinline__ void merge_segment(const CacheAttnParams& p, const uint8_t* smem, uint8_t* share, const Walk& wk, const Segment& sg) {
   using M = MergeSmem<D, NT>;
   constexpr int R = M::kR / H;
-  const bool whole = sg.v0 == 0 && sg.v1 == wk.sq.tiles;
-  if (threadIdx.x == 0 && wk.x + sg.v1 - sg.v0 >= wk.x_end)   // the stretch's last segment
+  using S = ShareSmem<D, R>;
+  const bool whole = p.cluster > 0 ? p.cluster == 1 : sg.v0 == 0 && sg.v1 == wk.sq.tiles;
+  if (p.cluster == 0 && threadIdx.x == 0 && wk.x + sg.v1 - sg.v0 >= wk.x_end)   // the stretch's last segment
     p.split[blockIdx.x] = make_int4(sg.b, sg.h, sg.rt, sg.v0 == 0 && !whole ? (wk.x + wk.sq.tiles - 1) / wk.ln.per - static_cast<int>(blockIdx.x) + 1 : 0);
   const float* mall = reinterpret_cast<const float*>(smem);
   const float2* mlall = reinterpret_cast<const float2*>(smem + M::kMlOff);
@@ -190,18 +242,71 @@ __device__ __forceinline__ void merge_segment(const CacheAttnParams& p, const ui
       acc.x = fmaf(f, a.x, acc.x); acc.y = fmaf(f, a.y, acc.y); acc.z = fmaf(f, a.z, acc.z); acc.w = fmaf(f, a.w, acc.w);
     }
     if (whole) {
-      const int mr = sg.rt * R + m;
-      if (mr < sg.n_rows) {
-        const float inv = sum > 0.f ? 1.f / sum : sum;   // 0: the row sees nothing; NaN stays
-        const int tok = mr / p.group;
-        T* op = reinterpret_cast<T*>(p.o) + sg.b * p.os[0] + (sg.h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + d;
-        *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
-      }
+      store_row<T, R>(p, sg, m, d, acc, sum);
+    } else if (p.cluster > 0) {
+      *reinterpret_cast<float4*>(share + i * 16) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(share + S::kMlOff + m * 8) = make_float2(top, sum);
     } else {
       *reinterpret_cast<float4*>(p.part_o + (static_cast<long long>(slot_out) * R + m) * D + d) = acc;
       if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot_out) * R + m) * 2) = make_float2(top, sum);
     }
   }
+  if (p.cluster <= 1) return;
+  cluster_sync_all();
+  const int rank = static_cast<int>(cluster_ctarank());
+  const uint32_t base = smem_u32(share);
+  for (int i = rank * kThreads + threadIdx.x; i < R * D / 4; i += p.cluster * kThreads) {
+    const int m = i / (D / 4), d = (i % (D / 4)) * 4;
+    float2 ml[8];
+    float4 a[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {   // all loads under way at once
+      ml[r] = make_float2(-INFINITY, 0.f);
+      a[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < p.cluster) {
+        const uint32_t peer = mapa_u32(base, r);
+        ml[r] = ld_cluster_f32x2(peer + S::kMlOff + m * 8);
+        a[r] = ld_cluster_f32x4(peer + i * 16);
+      }
+    }
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) top = fmaxf(top, ml[r].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float f = ml[r].x == -INFINITY ? 0.f : fast_exp2(ml[r].x - top);
+      sum = fmaf(f, ml[r].y, sum);
+      acc.x = fmaf(f, a[r].x, acc.x); acc.y = fmaf(f, a[r].y, acc.y); acc.z = fmaf(f, a[r].z, acc.z); acc.w = fmaf(f, a[r].w, acc.w);
+    }
+    store_row<T, R>(p, sg, m, d, acc, sum);
+  }
+  cluster_sync_all();   // nobody's shared memory goes away while a peer still reads it
+}
+
+// The launch of a decode kernel: p.stretches CTAs, in clusters where the parameters say so.
+template <typename... KArgs, typename... Args>
+inline int launch_decode_grid(void (*kernel)(KArgs...), const CacheAttnParams& p, size_t smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.stretches));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (p.cluster > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (chain_next_launch()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args&&>(args)...) == cudaSuccess && cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {

@@ -332,13 +332,6 @@ _KV4_ROWS = struct.Struct("@8i2P2P3q3q4P")
 _CACHE_ATTN = struct.Struct("@9if2P3q3q2P2P3q3q4PPN")
 
 
-def _pack(layout: struct.Struct, *fields) -> bytes:
-    try:
-        return layout.pack(*fields)
-    except struct.error as e:
-        raise ValueError(f"an argument is no whole number or out of range: {e}") from None
-
-
 def _refuse_rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int):
     if not t.is_cuda:
         raise ValueError("trinity_b200 operators take CUDA tensors (there is no CPU path)")
@@ -380,9 +373,9 @@ def _kv4_parts(cache: Kv4Cache, index: int):
             or half % 32):
         raise ValueError(f"codes must be uint8 (B, Hkv, L, D / 2), meta 16-bit (B, Hkv, L, D / 64, 2), alike for k and v; not "
                          + ", ".join(f"{t.dtype} {tuple(t.shape)}" for t in cache))
-    for t in cache:
-        if t.get_device() != index or not t.is_contiguous():
-            raise ValueError(f"the parts of a 4-bit cache must be contiguous tensors on cuda:{index}")
+    if not (kc.get_device() == vc.get_device() == km.get_device() == vm.get_device() == index
+            and kc.is_contiguous() and vc.is_contiguous() and km.is_contiguous() and vm.is_contiguous()):
+        raise ValueError(f"the parts of a 4-bit cache must be contiguous tensors on cuda:{index}")
     return b, h, length, 2 * half, dt
 
 
@@ -395,7 +388,7 @@ def _device_index(t: torch.Tensor) -> int:
 
 def _on_device(index: int, call, *args):
     """call(*args) with device `index` the current one."""
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         return call(*args)
     with torch.cuda.device(index):
         return call(*args)
@@ -408,11 +401,13 @@ def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int) -> None
     ks, vs = _rows4(k, "k", shape, dt, index), _rows4(v, "v", shape, dt, index)
     one = isinstance(start, int)
     kc, vc, km, vm = cache
-    args = L.Kv4RowsArgs.from_buffer_copy(_pack(
-        _KV4_ROWS,
-        _dt(k), b, h, count, d, length, start if one else 0, 0, 0 if one else _ints(start, "start", b, index), _ints(rows, "rows", b, index),
-        k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr()))
-    status = getattr(L.load(), name)(C.byref(args), _raw_stream(index))
+    try:
+        packed = _KV4_ROWS.pack(
+            _dt(k), b, h, count, d, length, start if one else 0, 0, 0 if one else _ints(start, "start", b, index), _ints(rows, "rows", b, index),
+            k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr())
+    except struct.error as e:
+        raise ValueError(f"an argument is no whole number or out of range: {e}") from None
+    status = getattr(L.load(), name)(C.byref(L.Kv4RowsArgs.from_buffer_copy(packed)), _raw_stream(index))
     if status:
         L.check(status, name)
 
@@ -446,6 +441,9 @@ def kv4_read(cache: Kv4Cache, start: Union[int, torch.Tensor], count: int, rows:
     return k_out, v_out
 
 
+_WORKSPACE_BYTES = {n: n + "_workspace_bytes" for n in ("tb200_attn_window", "tb200_kv4_attn")}
+
+
 def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index: int):
     lib = L.load()
     b, h, length, d, dt = dims
@@ -460,11 +458,15 @@ def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dim
             out.zero_()
     shape = (b, hq, s, d)
     qs, os_ = _rows4(q, "q", shape, dt, index), _rows4(out, "out", shape, dt, index)
-    args = L.CacheAttnArgs.from_buffer_copy(_pack(
-        _CACHE_ATTN, _dt(q), b, s, hq, h, d, length, window, sinks, sm_scale, q.data_ptr(), out.data_ptr(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2],
-        _ints(kv_lens, "kv_lens", b, index), _ints(q_rows, "q_rows", b, index), *caches, 0, 0))
+    try:
+        packed = _CACHE_ATTN.pack(
+            _dt(q), b, s, hq, h, d, length, window, sinks, sm_scale, q.data_ptr(), out.data_ptr(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2],
+            _ints(kv_lens, "kv_lens", b, index), _ints(q_rows, "q_rows", b, index), *caches, 0, 0)
+    except struct.error as e:
+        raise ValueError(f"an argument is no whole number or out of range: {e}") from None
+    args = L.CacheAttnArgs.from_buffer_copy(packed)
     ref = C.byref(args)
-    need = getattr(lib, name + "_workspace_bytes")(ref)
+    need = getattr(lib, _WORKSPACE_BYTES[name])(ref)
     if need:
         ws = Workspace.get(q.device, need, name)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
