@@ -413,7 +413,7 @@ def test_offsets_past_32_bits():
 
 def test_two_streams_at_once():
     """Calls on two streams have workspaces of their own."""
-    shape = (4, 32, 8, 128, 1, 16384, [16384, 4000, 100, 9999], [1] * 4, 0, 0)
+    shape = (4, 32, 8, 128, 1, 24000, [24000, 4000, 100, 9999], [1] * 4, 0, 0)
     b, hq, hkv, d, s, length, lens, rows, window, sinks = shape
     caches = [filled_cache(b, hkv, length, d, torch.bfloat16, i) for i in range(2)]
     q, _, kw = case(shape, torch.bfloat16)

@@ -596,7 +596,7 @@ int kv4_ctas(int head_dim, int unit_rows) {
   return unit_rows == 4 ? DecShape<64, 1, 2>::kCtas : unit_rows == 8 ? DecShape<64, 1, 1>::kCtas : DecShape<64, 2, 1>::kCtas;
 }
 
-constexpr int kClusterKeys = 256;
+constexpr int kClusterKeys = 640;
 
 struct AttnPlan {
   bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
@@ -642,8 +642,10 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   pl.unit_rows = unit_rows_for(rows, kv4);
   pl.row_tiles = static_cast<int>((rows + pl.unit_rows - 1) / pl.unit_rows);
   const int ctas = kv4 ? num_sms * kv4_ctas(a->head_dim, pl.unit_rows) : cache16_stretches(num_sms);
-  // A cluster per unit where the CTAs that are resident at a time can give every warp at most kClusterKeys keys; with more the
-  // line is faster, which does not care how long each sequence is.
+  // A cluster per unit where the CTAs that are resident at a time give every warp kClusterKeys keys or fewer: one launch, no
+  // partial results through HBM.  With more keys the line is safer, which does not care how long each sequence is.  Token on
+  // 4 bits, 16 sequences of 32/8 heads, line and clusters in us: 2048 positions each 20.6 / 16.3, 4096 28.6 / 22.6; up to 8192
+  // of different lengths 30.9 / 34.9 (1280 keys a warp).
   const int64_t units = static_cast<int64_t>(a->batch) * a->n_kv_heads * pl.row_tiles;
   int cluster = 1;
   while (cluster < 8 && units * cluster * 2 <= ctas) cluster *= 2;
