@@ -216,6 +216,10 @@ SHAPES = [  # b, hq, hkv, d, s, cache length, lens, rows, window, sinks
     (2, 20, 2, 128, 1, 24000, [11, 23999], [1, 1], 12000, 100),
     (70, 16, 8, 64, 1, 600, [600 - 8 * i for i in range(70)], [1] * 69 + [0], 0, 0),
     (40, 8, 8, 128, 2, 400, [10 * i for i in range(40)], [2] * 40, 0, 0),
+    (33, 4, 2, 64, 300, 400, [i * 12 for i in range(33)], [(i * 97) % 301 for i in range(33)], 0, 0),
+    (128, 2, 2, 128, 270, 320, [320 - i for i in range(128)], [0] * 127 + [270], 50, 4),
+    (129, 2, 1, 64, 90, 128, [i % 129 for i in range(129)], [i % 91 for i in range(129)], 0, 0),
+    (3, 4, 2, 64, 80, 4000, [4000, 2222, 0], [80, 0, 33], 0, 0),
 ]
 
 
