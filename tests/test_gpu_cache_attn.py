@@ -220,6 +220,9 @@ SHAPES = [  # b, hq, hkv, d, s, cache length, lens, rows, window, sinks
     (128, 2, 2, 128, 270, 320, [320 - i for i in range(128)], [0] * 127 + [270], 50, 4),
     (129, 2, 1, 64, 90, 128, [i % 129 for i in range(129)], [i % 91 for i in range(129)], 0, 0),
     (3, 4, 2, 64, 80, 4000, [4000, 2222, 0], [80, 0, 33], 0, 0),
+    (2, 71, 1, 64, 1, 60000, [60000, 12345], [1, 1], 0, 0),
+    (9, 96, 4, 64, 2, 2100, [i * 240 for i in range(9)], [2, 1, 0] * 3, 0, 0),
+    (38, 192, 8, 64, 1, 200, [200 - 5 * i for i in range(38)], [1] * 38, 64, 2),
 ]
 
 

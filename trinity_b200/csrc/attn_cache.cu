@@ -14,10 +14,10 @@
 //            keeps the largest p s below 2^14), the second sum is fp32, and for fp16 outputs the 8 is taken out with the SAME
 //            rounded probabilities (an MMA against a constant 8), so that the rounding error is that of centred codes, 2.6
 //            times smaller; bf16 outputs are rounded sixteen times more coarsely than that and do without.
+//            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 //   H = 2    four query rows or fewer (one token of up to four query heads per kv head): they fill half of the eight columns,
 //            so columns 4 to 7 repeat them, and each column takes the probabilities of half the keys: a thread then has two
 //            scores of sixteen keys to work on instead of four, and a row comes in two shares like those of two warps.
-//            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 #include <math.h>
 
 #include <type_traits>
@@ -466,91 +466,82 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
   }
 }
 
-// Merges the partial results of the units that lie in several stretches.  CTA (c, y): rows 4y to 4y + 3 of the unit that
-// begins in stretch c and goes on behind its end, if there is one; its first part is in slot 2c + 1, the others in the slots
-// 2c' of the stretches c' it covers.  The four warps share the parts; sums are taken in a fixed order.
-constexpr int kCombineThreads = 128, kCombineRows = 4;
-template <typename T, int D, int R>
+// Merges the partial results of the units that lie in several stretches.  CTA (x, y): rows y * kRows to y * kRows + kRows - 1
+// of record x's unit.  The unit begins in stretch c; its first part is in slot 2c + 1, the others in the slots 2c' of the
+// stretches c' it covers.  A group of D / 4 threads takes every kSteps-th part of a row, and the groups' sums are added in a
+// fixed order.  One row per CTA where units have many parts (one sequence of 71 heads, 65536 positions, 99 parts a unit: 22 us
+// for both kernels instead of 27 with four rows), else as many as make two groups a row.
+constexpr int kCombineThreads = 128, kCombineAhead = 4;
+template <typename T, int D, int R, int kRows>
 __global__ void __launch_bounds__(kCombineThreads) cache_combine_kernel(const __grid_constant__ CacheAttnParams p) {
-  constexpr int V = D / 32;
-  extern __shared__ float weights[];                                 // [rows][stretches]
-  __shared__ float red[4][kCombineRows][D];
+  constexpr int kLanes = D / 4, kGroups = kCombineThreads / kLanes, kSteps = kGroups / kRows;
+  __shared__ float4 red[kGroups][kLanes];
+  __shared__ float red_sum[kGroups];
   pdl_launch_dependents();
-  const int c = blockIdx.x, m0 = blockIdx.y * kCombineRows;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int row = group % kRows, step = group / kRows;
   pdl_wait();
-  const int4 rec = __ldcg(p.split + c);
+  const int4 rec = __ldcg(p.split + blockIdx.x);
+  int b = rec.x, h = rec.y, rt = rec.z, c = blockIdx.x;
+  if (p.record_per_unit) {
+    const int bh = c / p.row_tiles;
+    rt = c - bh * p.row_tiles;
+    b = bh / p.Hkv;
+    h = bh - b * p.Hkv;
+    c = rec.x;
+  }
+  const int m = blockIdx.y * kRows + row, mr = rt * R + m;
+  const int r = p.q_rows ? max(0, min(__ldg(p.q_rows + b), p.S)) : p.S;
+  if (rt * R + static_cast<int>(blockIdx.y) * kRows >= r * p.group) return;   // (a unit without rows has left no record)
   const int parts = rec.w;
   if (parts == 0) return;
-  const int b = rec.x, h = rec.y, rt = rec.z;
-  const int r = p.q_rows ? max(0, min(__ldg(p.q_rows + b), p.S)) : p.S;
-  if (rt * R + m0 >= r * p.group) return;
-  auto slot = [&](int i, int m) { return static_cast<long long>(2 * (c + i) + (i == 0 ? 1 : 0)) * R + m0 + m; };
-  float acc[kCombineRows][V], first[kCombineRows][V];
-  auto fetch = [&](int i, float (&v)[kCombineRows][V]) {
-#pragma unroll
-    for (int m = 0; m < kCombineRows; ++m) {
-      const float* src = p.part_o + slot(i, m) * D + lane * V;
-      if constexpr (V == 4) {
-        const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
-        v[m][0] = f.x; v[m][1] = f.y; v[m][2] = f.z; v[m][3] = f.w;
-      } else {
-        const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
-        v[m][0] = f.x; v[m][1] = f.y;
-      }
+  auto slot = [&](int i) { return static_cast<long long>(2 * (c + i) + (i == 0 ? 1 : 0)) * R + m; };
+  auto load = [&](int i, float4& v, float2& ml) {
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    ml = make_float2(-INFINITY, 0.f);
+    if (i < parts) {
+      v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot(i) * D) + lane);
+      ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot(i));
     }
   };
-  if (warp < parts) fetch(warp, first);   // on its way while the weights are made
-  // warp w: the weights of row w's parts, their maximum and sum
+  float4 v[kCombineAhead];
+  float2 ml[kCombineAhead];
+#pragma unroll
+  for (int k = 0; k < kCombineAhead; ++k) load(step + k * kSteps, v[k], ml[k]);
   float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(p.part_ml + slot(i, warp) * 2));
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  float sum = 0.f;
-  for (int i = lane; i < parts; i += 32) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot(i, warp) * 2));
-    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-    weights[warp * p.stretches + i] = f;
-    sum = fmaf(f, ml.y, sum);
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  __syncthreads();
-#pragma unroll
-  for (int m = 0; m < kCombineRows; ++m)
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[m][e] = warp < parts ? first[m][e] * weights[m * p.stretches + warp] : 0.f;
 #pragma unroll 4
-  for (int i = warp + 4; i < parts; i += 4) {
-    fetch(i, first);
+  for (int i = lane; i < parts; i += kLanes) top = fmaxf(top, __ldcg(p.part_ml + slot(i) * 2));
 #pragma unroll
-    for (int m = 0; m < kCombineRows; ++m) {
-      const float f = weights[m * p.stretches + i];
+  for (int d = kLanes / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = step; i0 < parts; i0 += kCombineAhead * kSteps) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[m][e] = fmaf(f, first[m][e], acc[m][e]);
+    for (int k = 0; k < kCombineAhead; ++k) {
+      const float f = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top);
+      sum = fmaf(f, ml[k].y, sum);
+      acc.x = fmaf(f, v[k].x, acc.x); acc.y = fmaf(f, v[k].y, acc.y); acc.z = fmaf(f, v[k].z, acc.z); acc.w = fmaf(f, v[k].w, acc.w);
+    }
+#pragma unroll
+    for (int k = 0; k < kCombineAhead; ++k) load(i0 + (kCombineAhead + k) * kSteps, v[k], ml[k]);
+  }
+  if constexpr (kSteps > 1) {
+    red[group][lane] = acc;
+    if (lane == 0) red_sum[group] = sum;
+    __syncthreads();
+    if (step > 0) return;
+#pragma unroll
+    for (int i = 1; i < kSteps; ++i) {
+      const float4 a = red[i * kRows + row][lane];
+      acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
+      sum += red_sum[i * kRows + row];
     }
   }
-#pragma unroll
-  for (int m = 0; m < kCombineRows; ++m)
-#pragma unroll
-    for (int e = 0; e < V; ++e) red[warp][m][lane * V + e] = acc[m][e];
-  __syncthreads();
-  const int mr = rt * R + m0 + warp;
   if (mr >= r * p.group) return;
   const float inv = sum > 0.f ? 1.f / sum : sum;   // 0: the row sees nothing; NaN stays
   const int tok = mr / p.group;
-  T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + lane * V;
-#pragma unroll
-  for (int e = 0; e < V; e += 2) {
-    float y[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      y[k] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) y[k] += red[w][warp][lane * V + e + k];
-    }
-    *reinterpret_cast<uint32_t*>(op + e) = Pack2<T>::pack(y[0] * inv, y[1] * inv);
-  }
+  T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + lane * 4;
+  *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
 }
 
 constexpr int kMaxExtent = 1 << 30;
@@ -589,10 +580,17 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
 bool takes_prompt_kernel(int64_t rows, int tokens, bool kv4) { return kv4 ? rows > 64 && tokens > 1 : rows > 16; }
 
 // Query rows of a unit: the smallest form that holds a sequence's rows of one kv head, else as many as there are.  Four rows:
-// see H at cache_decode_kernel.
-int unit_rows_for(int64_t rows, bool kv4) { return kv4 && rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
+// see H at cache_decode_kernel.  24 rows (4 bits, D = 64: with D = 128 the accumulators do not fit): a tile takes 4/3 of the
+// instructions of one of 16 rows, for the codes become operands once for all columns, so it is taken where that saves a third
+// of the units or so.  In us with 16 and 24 rows, fp16, one token: 4 sequences of 71 heads on one, 131072 positions
+// 69 / 59, 65536 41 / 38; 16 sequences of 192 heads on 8, 16384 positions 102 / 78.
+int unit_rows_for(int64_t rows, int head_dim, bool kv4) {
+  if (kv4 && head_dim == 64 && (rows + 23) / 24 * 4 < (rows + 15) / 16 * 3) return 24;
+  return kv4 && rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+}
 int kv4_ctas(int head_dim, int unit_rows) {
   if (head_dim == 128) return unit_rows == 4 ? DecShape<128, 1, 2>::kCtas : unit_rows == 8 ? DecShape<128, 1, 1>::kCtas : DecShape<128, 2, 1>::kCtas;
+  if (unit_rows == 24) return DecShape<64, 3, 1>::kCtas;
   return unit_rows == 4 ? DecShape<64, 1, 2>::kCtas : unit_rows == 8 ? DecShape<64, 1, 1>::kCtas : DecShape<64, 2, 1>::kCtas;
 }
 
@@ -639,18 +637,26 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
     }
     return pl;
   }
-  pl.unit_rows = unit_rows_for(rows, kv4);
-  pl.row_tiles = static_cast<int>((rows + pl.unit_rows - 1) / pl.unit_rows);
-  const int ctas = kv4 ? num_sms * kv4_ctas(a->head_dim, pl.unit_rows) : cache16_stretches(num_sms);
+  const int64_t keys = window > 0 && static_cast<int64_t>(window) + a->rows + sinks < a->cache_len ? static_cast<int64_t>(window) + a->rows + sinks : a->cache_len;
+  int ctas = 0, cluster = 1;
+  int64_t units = 0;
+  auto deal = [&](int unit_rows) {
+    pl.unit_rows = unit_rows;
+    pl.row_tiles = static_cast<int>((rows + unit_rows - 1) / unit_rows);
+    ctas = kv4 ? num_sms * kv4_ctas(a->head_dim, unit_rows) : cache16_stretches(num_sms);
+    units = static_cast<int64_t>(a->batch) * a->n_kv_heads * pl.row_tiles;
+    for (cluster = 1; cluster < 8 && units * cluster * 2 <= ctas;) cluster *= 2;
+    return units <= ctas && keys <= static_cast<int64_t>(kClusterKeys) * kWarps * cluster;
+  };
   // A cluster per unit where the CTAs that are resident at a time give every warp kClusterKeys keys or fewer: one launch, no
   // partial results through HBM.  With more keys the line is safer, which does not care how long each sequence is.  Token on
   // 4 bits, 16 sequences of 32/8 heads, line and clusters in us: 2048 positions each 20.6 / 16.3, 4096 28.6 / 22.6; up to 8192
   // of different lengths 30.9 / 34.9 (1280 keys a warp).
-  const int64_t units = static_cast<int64_t>(a->batch) * a->n_kv_heads * pl.row_tiles;
-  int cluster = 1;
-  while (cluster < 8 && units * cluster * 2 <= ctas) cluster *= 2;
-  const int64_t keys = window > 0 && static_cast<int64_t>(window) + a->rows + sinks < a->cache_len ? static_cast<int64_t>(window) + a->rows + sinks : a->cache_len;
-  if (units <= ctas && keys <= static_cast<int64_t>(kClusterKeys) * kWarps * cluster) {
+  bool clusters = deal(unit_rows_for(rows, a->head_dim, kv4));
+  // fewer units than the SMs hold in the largest clusters: 16 rows use more SMs (4 sequences of 71 heads, 2048 positions: 8.1
+  // against 9.3 us)
+  if (pl.unit_rows == 24 && clusters && cluster == 8) clusters = deal(16) || deal(24);
+  if (clusters) {
     pl.cluster = cluster;
     pl.stretches = static_cast<int>(units * cluster);
     return pl;
@@ -699,6 +705,9 @@ int launch_decode(const CacheAttnParams& p, cudaStream_t stream) {
 template <typename T, int D>
 int run_kv4(const CacheAttnParams& p, int unit_rows, cudaStream_t stream) {
   if (unit_rows == 4) return launch_decode<T, D, 1, 2>(p, stream);
+  if constexpr (D == 64) {
+    if (unit_rows == 24) return launch_decode<T, D, 3, 1>(p, stream);
+  }
   return unit_rows == 8 ? launch_decode<T, D, 1, 1>(p, stream) : launch_decode<T, D, 2, 1>(p, stream);
 }
 template <typename T>
@@ -708,14 +717,19 @@ int run_kv4(const CacheAttnParams& p, int head_dim, int unit_rows, cudaStream_t 
 
 template <typename T, int D, int R>
 int launch_combine(const CacheAttnParams& p, cudaStream_t stream) {
-  if (launch_chained(cache_combine_kernel<T, D, R>, dim3(p.stretches, R / kCombineRows), dim3(kCombineThreads),
-                     kCombineRows * p.stretches * sizeof(float), stream, p) != cudaSuccess)
-    return TB200_ERR_CUDA;
-  return cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
+  constexpr int kRows = 256 / D;
+  const unsigned records = static_cast<unsigned>(p.record_per_unit ? p.B * p.Hkv * p.row_tiles : p.stretches);
+  const cudaError_t e = records * 16 <= static_cast<unsigned>(p.stretches)
+                            ? launch_chained(cache_combine_kernel<T, D, R, 1>, dim3(records, R), dim3(kCombineThreads), 0, stream, p)
+                            : launch_chained(cache_combine_kernel<T, D, R, kRows>, dim3(records, R / kRows), dim3(kCombineThreads), 0, stream, p);
+  return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? TB200_OK : TB200_ERR_CUDA;
 }
 template <typename T, int D>
 int launch_combine(const CacheAttnParams& p, int unit_rows, cudaStream_t stream) {
   if (unit_rows == 4) return launch_combine<T, D, 4>(p, stream);
+  if constexpr (D == 64) {
+    if (unit_rows == 24) return launch_combine<T, D, 24>(p, stream);
+  }
   return unit_rows == 8 ? launch_combine<T, D, 8>(p, stream) : launch_combine<T, D, 16>(p, stream);
 }
 template <typename T>
@@ -779,6 +793,7 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   ChainScope chain;
   if (pl.prompt) return run_prompt(a, kv4, pl, p, ws, st->num_sms, stream);
   p.stretches = pl.stretches;
+  p.record_per_unit = static_cast<int64_t>(a->batch) * a->n_kv_heads * pl.row_tiles <= pl.stretches;
   p.row_tiles = pl.row_tiles;
   p.cluster = pl.cluster;
   p.part_o = reinterpret_cast<float*>(ws);

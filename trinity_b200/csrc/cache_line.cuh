@@ -29,6 +29,7 @@ struct CacheAttnParams {
   int B, S, Hq, Hkv, group, cache_len, window, sinks;
   int row_tiles;             // units per (sequence, kv head) at most
   int cluster;               // 0: the line; else CTAs per unit
+  int record_per_unit;       // the line: what `split` is indexed by, the unit where there are no more units than stretches, else the stretch
   float scale_log2;
   const uint8_t* q;
   uint8_t* o;
@@ -38,7 +39,8 @@ struct CacheAttnParams {
   const uint8_t *k_codes, *v_codes, *k_meta, *v_meta;
   float* part_o;             // (2 grid, R, D)
   float* part_ml;            // (2 grid, R, 2)
-  int4* split;               // (grid): the unit that begins in a stretch and goes on behind it: sequence, kv head, row tile, stretches it lies in (0: none)
+  int4* split;               // (grid) units that lie in several stretches and in how many (0: no such unit): by stretch (sequence, kv head,
+                             // row tile, how many), for the one that begins there and goes on; by unit (stretch it begins in, -, -, how many)
   int stretches;             // CTAs of the decode kernel
   int* err;
   long long wait_limit;
@@ -150,7 +152,7 @@ struct Walk {
     x = ln.per * static_cast<int>(blockIdx.x);
     x_end = min(x + ln.per, ln.total);
     if (x >= x_end) {
-      if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+      if (threadIdx.x == 0 && !p.record_per_unit) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
       return false;
     }
     base = ln.base;
@@ -221,8 +223,14 @@ __device__ __forceinline__ void merge_segment(const CacheAttnParams& p, const ui
   constexpr int R = M::kR / H;
   using S = ShareSmem<D, R>;
   const bool whole = p.cluster > 0 ? p.cluster == 1 : sg.v0 == 0 && sg.v1 == wk.sq.tiles;
-  if (p.cluster == 0 && threadIdx.x == 0 && wk.x + sg.v1 - sg.v0 >= wk.x_end)   // the stretch's last segment
-    p.split[blockIdx.x] = make_int4(sg.b, sg.h, sg.rt, sg.v0 == 0 && !whole ? (wk.x + wk.sq.tiles - 1) / wk.ln.per - static_cast<int>(blockIdx.x) + 1 : 0);
+  if (p.cluster == 0 && threadIdx.x == 0) {
+    const int c = static_cast<int>(blockIdx.x), parts = sg.v0 == 0 && !whole ? (wk.x + wk.sq.tiles - 1) / wk.ln.per - c + 1 : 0;
+    if (p.record_per_unit) {
+      if (sg.v0 == 0) p.split[(sg.b * p.Hkv + sg.h) * p.row_tiles + sg.rt] = make_int4(c, 0, 0, parts);
+    } else if (wk.x + sg.v1 - sg.v0 >= wk.x_end) {   // the stretch's last segment
+      p.split[c] = make_int4(sg.b, sg.h, sg.rt, parts);
+    }
+  }
   const float* mall = reinterpret_cast<const float*>(smem);
   const float2* mlall = reinterpret_cast<const float2*>(smem + M::kMlOff);
   const int slot_out = 2 * blockIdx.x + (sg.v0 == 0 ? 1 : 0);
