@@ -330,7 +330,8 @@ int tb200_kv_compact(const tb200_kv_compact_args* args, void* stream);
  * start[b] + i.  Rows i >= n_rows[b] and rows whose position lies outside [0, cache_len) are left as
  * they are (append: the cache; read: k and v).  n_rows[b] outside [0, rows] is taken as the nearer end.
  * k and v are addressed by element strides of their batch, head and row axes (multiples of 8; head_dim
- * contiguous); the rows of a tensor that is written must not overlap one another. */
+ * contiguous); the rows of a tensor that is written must not overlap one another, nor what else the call
+ * reads or writes. */
 typedef struct {
   int dtype;                 /* TB200_F16 or TB200_BF16: k, v, meta */
   int batch, n_kv_heads, rows, head_dim; /* head_dim 64 or 128 */
@@ -369,7 +370,7 @@ int tb200_kv4_rows_check(const tb200_kv4_rows_args* args);
  * sequence in the same call.
  *
  * tb200_attn_window: 16-bit caches, tb200_kv4_attn: 4-bit caches as above.  q, o and the 16-bit caches
- * are addressed by element strides (multiples of 8, head_dim contiguous).  Workspace: as the
+ * are addressed by element strides (multiples of 8, head_dim contiguous); o overlaps no input.  Workspace: as the
  * *_workspace_bytes queries say for the same arguments (pointers and lengths are not looked at). */
 typedef struct {
   int dtype;                 /* TB200_F16 or TB200_BF16: q, o, 16-bit caches, meta */

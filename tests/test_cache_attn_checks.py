@@ -57,6 +57,18 @@ def test_read_refuses_rows_that_overlap(lib):
         assert lib.tb200_kv4_rows_check(C.byref(rows_args(k_stride=stride))) == 0      # as a source they may
 
 
+def test_two_outputs_in_one_place_are_refused(lib):
+    assert lib.tb200_kv4_read(C.byref(rows_args(v=0x1000)), None) == INVALID
+    for same in (dict(v_codes=0x3000), dict(v_meta=0x5000)):
+        assert lib.tb200_kv4_append(C.byref(rows_args(**same)), None) == INVALID
+        assert lib.tb200_kv4_rows_check(C.byref(rows_args(**same))) == 0      # one cache for both may be read
+
+
+@pytest.mark.parametrize("change", [dict(rows=(1 << 30) + 1), dict(cache_len=(1 << 30) + 4), dict(batch=(1 << 30) + 1), dict(n_kv_heads=(1 << 30) + 1)])
+def test_rows_extents_are_bounded(lib, change):
+    assert lib.tb200_kv4_rows_check(C.byref(rows_args(**change))) == INVALID
+
+
 COMMON = [
     ({}, 0), (dict(dtype=L.F32), UNSUPPORTED), (dict(head_dim=256), UNSUPPORTED), (dict(n_q_heads=9), INVALID), (dict(n_q_heads=0), INVALID),
     (dict(cache_len=0), INVALID), (dict(window=-1), INVALID), (dict(sinks=-1), INVALID), (dict(sm_scale=0.0), INVALID), (dict(sm_scale=float("nan")), INVALID),

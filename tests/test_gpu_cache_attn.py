@@ -438,6 +438,39 @@ def test_two_streams_at_once():
         assert all(torch.equal(o, want[i]) for o in got[i])
 
 
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("kv4", [True, False])
+def test_two_captured_graphs_at_once(kv4, new):
+    """Graphs captured one after the other on one stream have workspaces of their own, and none with eager calls."""
+    shape = (4, 32, 8, 128, new, 24000, [24000, 4000, 100, 9999], [new] * 4, 0, 0)
+    b, hq, hkv, d, s, length, lens, rows, window, sinks = shape
+    lens = ints(lens)
+    q, _, kw = case(shape, torch.bfloat16)
+    del kw["out"]
+    g = torch.Generator(device=DEV).manual_seed(3)
+    if kv4:
+        caches = [filled_cache(b, hkv, length, d, torch.bfloat16, i) for i in range(3)]
+        calls = [lambda c=c: ops.kv4_attn(q, c, lens, **kw) for c in caches]
+    else:
+        caches = [torch.randn(b, hkv, length, d, generator=g, device=DEV).bfloat16() for _ in range(3)]
+        calls = [lambda c=c: ops.attn_window(q, c, c, lens, **kw) for c in caches]
+    want = [f().clone() for f in calls]
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph, f in zip(graphs, calls):
+        with torch.cuda.graph(graph):
+            outs.append(f())
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        eager = calls[2]()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals_on_the_device():
     dt = torch.bfloat16
@@ -455,6 +488,15 @@ def test_refusals_on_the_device():
         ops.kv4_append(cache, torch.zeros(2, 2, 3, 68, dtype=dt, device=DEV)[..., :64], x, 0)
     with pytest.raises(TypeError):
         ops.kv4_append(cache, x, x, torch.zeros(2, dtype=torch.int64, device=DEV))
+    for bad in (None, 1.5, [0, 0]):
+        with pytest.raises(TypeError):
+            ops.kv4_append(cache, x, x, bad)
+        with pytest.raises(TypeError):
+            ops.kv4_attn(q, cache, bad)
+    with pytest.raises(ValueError):
+        ops.kv4_append(cache, x, x, 1 << 40)
+    with pytest.raises(L.Tb200Error):       # both results in one place
+        ops.kv4_read(cache, 0, 3, k_out=x, v_out=x)
     with pytest.raises(L.Tb200Error):       # written rows that overlap
         ops.kv4_read(cache, 0, 3, k_out=torch.zeros(1, 2, 3, 64, dtype=dt, device=DEV).expand(2, 2, 3, 64), v_out=x.clone())
     with pytest.raises(ValueError):
@@ -465,7 +507,7 @@ def test_refusals_on_the_device():
         ops.kv4_attn(q, cache, ints([3]))
     with pytest.raises(TypeError):
         ops.kv4_attn(q.half(), cache, lens)
-    for bad in (dict(sm_scale=0.0), dict(sm_scale=math.inf), dict(sm_scale=-1.0), dict(window=-1), dict(sinks=-1, window=4), dict(out=q)):
+    for bad in (dict(sm_scale=0.0), dict(sm_scale=math.inf), dict(sm_scale=1e300), dict(sm_scale=-1.0), dict(window=-1), dict(sinks=-1, window=4), dict(out=q)):
         with pytest.raises(L.Tb200Error):
             ops.kv4_attn(q, cache, lens, **bad)
     with pytest.raises(L.Tb200Error):       # three query heads on two key/value heads

@@ -388,11 +388,14 @@ int check_strides(const int64_t (&st)[3], const int64_t (&ext)[3], int head_dim,
 
 namespace {
 
+constexpr int kMaxExtent = 1 << 30;
+
 int check_rows(const tb200_kv4_rows_args* a) {
   if (a == nullptr) return TB200_ERR_INVALID;
   if (a->dtype != TB200_BF16 && a->dtype != TB200_F16) return TB200_ERR_UNSUPPORTED;
   if (a->head_dim != 64 && a->head_dim != 128) return TB200_ERR_UNSUPPORTED;
   if (a->batch < 0 || a->rows < 0 || a->n_kv_heads < 1 || a->cache_len < 0 || (a->cache_len & 3) || a->reserved != 0) return TB200_ERR_INVALID;
+  if (a->batch > kMaxExtent || a->rows > kMaxExtent || a->n_kv_heads > kMaxExtent || a->cache_len > kMaxExtent) return TB200_ERR_INVALID;
   if (a->batch == 0 || a->rows == 0 || a->cache_len == 0) return TB200_OK;   // nothing to read or write: empty tensors have no address
   if (!a->k || !a->v || !a->k_codes || !a->v_codes || !a->k_meta || !a->v_meta) return TB200_ERR_INVALID;
   if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_codes) || !aligned16(a->v_codes) || !aligned16(a->k_meta) || !aligned16(a->v_meta))
@@ -491,6 +494,8 @@ extern "C" int tb200_kv4_rows_check(const tb200_kv4_rows_args* a) { return check
 extern "C" int tb200_kv4_append(const tb200_kv4_rows_args* a, void* stream) {
   const int bad = check_rows(a);
   if (bad != TB200_OK) return bad;
+  const bool any = a->batch > 0 && a->rows > 0 && a->cache_len > 0;
+  if (any && (a->k_codes == a->v_codes || a->k_meta == a->v_meta)) return TB200_ERR_INVALID;   // written from two sources
   int status = TB200_OK;
   DeviceState* st = device_state(&status);
   if (!st) return status;
@@ -501,6 +506,8 @@ extern "C" int tb200_kv4_read(const tb200_kv4_rows_args* a, void* stream) {
   const int bad = check_rows(a);
   if (bad != TB200_OK) return bad;
   const int64_t ext[3] = {a->batch, a->n_kv_heads, a->rows};   // k and v are written here
+  const bool any = a->batch > 0 && a->rows > 0 && a->cache_len > 0;
+  if (any && a->k == a->v) return TB200_ERR_INVALID;
   if (check_strides(a->k_stride, ext, a->head_dim, true) != TB200_OK || check_strides(a->v_stride, ext, a->head_dim, true) != TB200_OK)
     return TB200_ERR_INVALID;
   int status = TB200_OK;

@@ -354,8 +354,8 @@ def _rows4(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int):
 def _ints(t: Optional[torch.Tensor], name: str, batch: int, index: int) -> int:
     if t is None:
         return 0
-    if t.dtype is not torch.int32 or t.shape != (batch,):
-        raise TypeError(f"{name} must be int32 of shape ({batch},)")
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.shape != (batch,):
+        raise TypeError(f"{name} must be an int32 tensor of shape ({batch},)")
     if t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor on cuda:{index}")
     return t.data_ptr()
@@ -400,6 +400,8 @@ def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int) -> None
     shape = (b, h, count, d)
     ks, vs = _rows4(k, "k", shape, dt, index), _rows4(v, "v", shape, dt, index)
     one = isinstance(start, int)
+    if start is None:
+        raise TypeError("start must be an int or an int32 tensor")
     kc, vc, km, vm = cache
     try:
         packed = _KV4_ROWS.pack(
@@ -468,7 +470,8 @@ def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dim
     ref = C.byref(args)
     need = getattr(lib, _WORKSPACE_BYTES[name])(ref)
     if need:
-        ws = Workspace.get(q.device, need, name)
+        # a graph gets scratch of its own, out of its memory pool: graphs captured on one stream may run side by side
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if torch._C._cuda_isCurrentStreamCapturing() else Workspace.get(q.device, need, name)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
     status = getattr(lib, name)(ref, _raw_stream(index))
     if status:
@@ -484,8 +487,9 @@ def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
     ``kv_lens`` int32 ``(B,)``: positions in the cache, the new ones included; ``q_rows`` int32 ``(B,)``: how many of the
     ``S`` query rows belong to the sequence (default all); they are the last positions.  A query sees the positions up to
     its own, with ``window > 0`` only the last ``window`` of these and the first ``sinks`` ones.  A row that sees nothing
-    gives zeros.  Rows from ``q_rows`` on are left as they are in ``out`` (zero when it is not given).  Returns ``out``,
-    ``(B, Hq, S, D)``; by default laid out so that ``out.transpose(1, 2).reshape(B, S, Hq * D)`` is a view."""
+    gives zeros.  Rows from ``q_rows`` on are left as they are in ``out`` (zero when it is not given).  ``out`` overlaps
+    none of the inputs.  Returns ``out``, ``(B, Hq, S, D)``; by default laid out so that
+    ``out.transpose(1, 2).reshape(B, S, Hq * D)`` is a view.  Forward only."""
     index = _device_index(q)
     shape = k_cache.shape
     if len(shape) != 4:
