@@ -443,6 +443,7 @@ def kv4_read(cache: Kv4Cache, start: Union[int, torch.Tensor], count: int, rows:
     return k_out, v_out
 
 
+_KEPT_SCRATCH = 64 << 20   # decode calls need a few MB
 _WORKSPACE_BYTES = {n: n + "_workspace_bytes" for n in ("tb200_attn_window", "tb200_kv4_attn")}
 
 
@@ -470,8 +471,10 @@ def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dim
     ref = C.byref(args)
     need = getattr(lib, _WORKSPACE_BYTES[name])(ref)
     if need:
-        # a graph gets scratch of its own, out of its memory pool: graphs captured on one stream may run side by side
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if torch._C._cuda_isCurrentStreamCapturing() else Workspace.get(q.device, need, name)
+        # a graph gets scratch of its own, out of its memory pool: graphs captured on one stream may run side by side.  A 16-bit
+        # copy of a large cache is not kept between calls.
+        own = need > _KEPT_SCRATCH or torch._C._cuda_isCurrentStreamCapturing()
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if own else Workspace.get(q.device, need, name)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
     status = getattr(lib, name)(ref, _raw_stream(index))
     if status:
