@@ -327,9 +327,22 @@ def kv4_cache(batch: int, kv_heads: int, cache_len: int, head_dim: int, dtype: t
     return Kv4Cache(*codes, *meta)
 
 
-# The argument blocks, packed in one call: a ctypes structure filled field by field costs more than the launch of a small kernel.
+# The argument blocks of L.Kv4RowsArgs and L.CacheAttnArgs, packed in one call and handed over as bytes: a ctypes structure
+# filled field by field costs more than the launch of a small kernel.
 _KV4_ROWS = struct.Struct("@8i2P2P3q3q4P")
 _CACHE_ATTN = struct.Struct("@9if2P3q3q2P2P3q3q4PPN")
+assert _KV4_ROWS.size == C.sizeof(L.Kv4RowsArgs) and _CACHE_ATTN.size == C.sizeof(L.CacheAttnArgs)
+_ENTRIES: dict = {}
+
+
+def _entry(name: str, restype=C.c_int, argtypes=(C.c_char_p, C.c_void_p)):
+    """A function of the library that takes its argument block as bytes."""
+    f = _ENTRIES.get(name)
+    if f is None:
+        f = L.load()[name]     # (an object of its own: the one behind the attribute takes the structure)
+        f.restype, f.argtypes = restype, argtypes
+        _ENTRIES[name] = f
+    return f
 
 
 def _refuse_rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int):
@@ -409,7 +422,7 @@ def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int) -> None
             k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr())
     except struct.error as e:
         raise ValueError(f"an argument is no whole number or out of range: {e}") from None
-    status = getattr(L.load(), name)(C.byref(L.Kv4RowsArgs.from_buffer_copy(packed)), _raw_stream(index))
+    status = _entry(name)(packed, _raw_stream(index))
     if status:
         L.check(status, name)
 
@@ -444,11 +457,11 @@ def kv4_read(cache: Kv4Cache, start: Union[int, torch.Tensor], count: int, rows:
 
 
 _KEPT_SCRATCH = 64 << 20   # decode calls need a few MB
-_WORKSPACE_BYTES = {n: n + "_workspace_bytes" for n in ("tb200_attn_window", "tb200_kv4_attn")}
+_NEEDS_WORKSPACE = -4      # TB200_ERR_WORKSPACE
+_WORKSPACE = struct.Struct("@PN")   # the end of _CACHE_ATTN
 
 
 def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index: int):
-    lib = L.load()
     b, h, length, d, dt = dims
     if q.dim() != 4:
         raise ValueError(f"q must have shape (B, Hq, S, D), not {tuple(q.shape)}")
@@ -467,16 +480,14 @@ def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dim
             _ints(kv_lens, "kv_lens", b, index), _ints(q_rows, "q_rows", b, index), *caches, 0, 0)
     except struct.error as e:
         raise ValueError(f"an argument is no whole number or out of range: {e}") from None
-    args = L.CacheAttnArgs.from_buffer_copy(packed)
-    ref = C.byref(args)
-    need = getattr(lib, _WORKSPACE_BYTES[name])(ref)
-    if need:
+    status = _entry(name)(packed, _raw_stream(index))
+    if status == _NEEDS_WORKSPACE:   # nothing has been launched; calls on short caches need none
+        need = _entry(name + "_workspace_bytes", C.c_size_t, (C.c_char_p,))(packed)
         # a graph gets scratch of its own, out of its memory pool: graphs captured on one stream may run side by side.  A 16-bit
         # copy of a large cache is not kept between calls.
         own = need > _KEPT_SCRATCH or torch._C._cuda_isCurrentStreamCapturing()
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if own else Workspace.get(q.device, need, name)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    status = getattr(lib, name)(ref, _raw_stream(index))
+        status = _entry(name)(packed[:-_WORKSPACE.size] + _WORKSPACE.pack(ws.data_ptr(), need), _raw_stream(index))
     if status:
         L.check(status, name)
     return out
