@@ -18,6 +18,10 @@
 //   H = 2    four query rows or fewer (one token of up to four query heads per kv head): they fill half of the eight columns,
 //            so columns 4 to 7 repeat them, and each column takes the probabilities of half the keys: a thread then has two
 //            scores of sixteen keys to work on instead of four, and a row comes in two shares like those of two warps.
+//   measured one token of 24 sequences of 1 to 16384 positions, 32/8 heads of 128, bf16: 52.7 us for 223 MB, 65 % of the copy
+//            bandwidth; an instruction issues in half of the cycles, the tensor pipe is busy in a quarter of them: what is
+//            left is the latency of each warp's chain scores -> maximum -> exponentials -> products, with the 8 to 12 warps
+//            per SM that the registers allow.
 #include <math.h>
 
 #include <type_traits>

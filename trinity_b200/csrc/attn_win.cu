@@ -2,6 +2,8 @@
 // the decode form of tb200_attn_window (units, line and stretches: cache_line.cuh).
 //
 // Bound: HBM, the visible cache rows are read once per key/value head; a window makes calls short, so launch latency next.
+// One token of 32 sequences of 1 to 4096 positions, window 1024 and 4 first ones, 32/8 heads of 128, bf16: 24.7 us for 133 MB,
+// 82 % of the copy bandwidth.
 // Sixteen keys per tile and warp: K and V arrive as TMA boxes of 16 keys x 64 columns (128-byte swizzle) in the warp's own
 // ring, S^T = K Q^T and O^T = V^T P^T are m16n8k16 MMAs with the query rows as the 8 columns (a 16-row tile of queries
 // would be half empty at eight query heads per key/value head), P goes from one to the other through movmatrix.

@@ -263,7 +263,8 @@ int launch_kv_compact(const tb200_kv_compact_args& a, cudaStream_t stream);
 // not overlap.  Axes of one element are not looked at.
 int check_strides(const int64_t (&stride)[3], const int64_t (&ext)[3], int head_dim, bool written);
 // A prompt's operands out of a 4-bit cache: the positions that some query row of its sequence sees as contiguous 16-bit
-// caches (B, Hkv, cache_len, D), other positions left as they are.  fp16: the values, rounded.  bf16: in fp16, divided by a
+// caches (B, Hkv, cache_len, D), other positions left as they are.  fp16: the values, rounded (by half a step of the type
+// the output is rounded to as well).  bf16: in fp16, divided by a
 // power of two per head (head_factor (B, Hkv, 4): 1 / factor and factor of K, of V), and q (B, Hq, rows, D) likewise by one
 // per row (q_factor); q16, q_factor and head_factor are not used for fp16.
 struct Kv4PromptOperands {
