@@ -34,7 +34,7 @@ def quantise64(x):
     """Codes and (s, lo) of rows x (..., D), quotients in 64 bits."""
     g = x.unflatten(-1, (-1, 64))
     lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    s = ((hi.float() - lo.float()) / 15).to(x.dtype)
+    s = ((hi.float() - lo.float()) / torch.full_like(hi, 15, dtype=torch.float32)).to(x.dtype)    # (a scalar divisor would become a factor 1/15)
     c = torch.where(s > 0, ((g.double() - lo.double()) / s.double()).round().clamp(0, 15), torch.zeros((), dtype=torch.float64, device=x.device))
     return c.flatten(-2), s.squeeze(-1), lo.squeeze(-1)
 
