@@ -42,8 +42,9 @@ template <> struct Bits<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t rn(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 };
 
-// Two 16-bit values at once: minimum (a NaN wins), and their sign flipped.
+// Two 16-bit values at once: minimum and maximum (a NaN wins).
 template <typename T> __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b);
+template <typename T> __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b);
 template <> __device__ __forceinline__ uint32_t min2_nan<__half>(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -53,6 +54,24 @@ template <> __device__ __forceinline__ uint32_t min2_nan<__nv_bfloat16>(uint32_t
   uint32_t r;
   asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
+}
+template <> __device__ __forceinline__ uint32_t max2_nan<__half>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t max2_nan<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// x / 15 correctly rounded: the Newton step of encode8, with 1/15 rounded by the compiler; where the remainder would leave
+// fp32's normal range, a division.
+__device__ __forceinline__ float fifteenth(float x) {
+  constexpr float kInv = 1.f / 15.f;
+  const float q = __fmul_rn(x, kInv);
+  const float r = __fmaf_rn(__fmaf_rn(q, -15.f, x), kInv, q);
+  return x < 1e-30f ? __fdiv_rn(x, 15.f) : r;
 }
 // Below this scale its rounding to the type is so coarse that a quotient may pass 15.5.
 template <typename T> struct SmallScale;
@@ -154,20 +173,21 @@ __global__ void __launch_bounds__(kThreads, 4) kv4_append_kernel(const __grid_co
       for (int w = 0; w < 2; ++w) {
         const uint32_t v[2][4] = {{raw[k][w][0].x, raw[k][w][0].y, raw[k][w][0].z, raw[k][w][0].w},
                                   {raw[k][w][1].x, raw[k][w][1].y, raw[k][w][1].z, raw[k][w][1].w}};
-        // minimum, and minus the maximum as the minimum of the negated values, side by side in one register
-        uint32_t lo2 = v[0][0], hi2 = v[0][0] ^ 0x80008000u;
+        // minimum, and minus the maximum (from here on a minimum, too) side by side in one register
+        uint32_t lo2 = v[0][0], hi2 = v[0][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) {
           lo2 = min2_nan<T>(lo2, v[i >> 2][i & 3]);
-          hi2 = min2_nan<T>(hi2, v[i >> 2][i & 3] ^ 0x80008000u);
+          hi2 = max2_nan<T>(hi2, v[i >> 2][i & 3]);
         }
+        hi2 ^= 0x80008000u;
         uint32_t both = min2_nan<T>(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
         both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, 1));
         both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, 2));
         const float2 f = Pack2<T>::unpack(both);
         const float lo = f.x, range = __fsub_rn(-f.y, f.x);
         const bool odd = !(range < INFINITY);    // an infinity or a NaN among the 64, or a range past fp32
-        const uint32_t sb = odd ? 0x7fffu : Bits<T>::rn(__fdiv_rn(range, 15.f));
+        const uint32_t sb = odd ? 0x7fffu : Bits<T>::rn(fifteenth(range));
         const uint32_t lb = odd ? 0x7fffu : (both & 0xffffu);
         const float s = odd ? 0.f : Bits<T>::f(sb);
         const uint32_t word0 = encode8<T>(v[0], lo, s), word1 = encode8<T>(v[1], lo, s);
