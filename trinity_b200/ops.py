@@ -2,7 +2,8 @@
 
 PyTorch is plumbing here (device memory, streams); every operator below runs in libtrinity_b200.so.
 All wrappers launch on ``torch.cuda.current_stream()`` and allocate nothing once their workspace has
-been cached, so they can be captured in a CUDA graph after one warm-up call.
+been cached (attention over caches: but for a 16-bit copy of a large 4-bit cache, and in a capture, where
+scratch comes out of the graph's pool), so they can be captured in a CUDA graph after one warm-up call.
 """
 from __future__ import annotations
 
@@ -38,9 +39,12 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_current_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _raw_stream(index: int) -> int:
     """The current stream of device `index`, without a Stream object (which costs about 3 us)."""
-    return torch._C._cuda_getCurrentRawStream(index)
+    return _current_raw_stream(index)
 
 
 class Workspace:
@@ -359,14 +363,18 @@ def _refuse_rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: i
 
 def _rows4(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int):
     """Strides of a ``(B, heads, rows, D)`` tensor whose last axis is contiguous, in elements."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or t.stride(3) != 1:
-        _refuse_rows(t, name, shape, dtype, index)
-    return t.stride()
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index:
+        strides = t.stride()
+        if strides[3] == 1:
+            return strides
+    _refuse_rows(t, name, shape, dtype, index)
 
 
 def _ints(t: Optional[torch.Tensor], name: str, batch: int, index: int) -> int:
     if t is None:
         return 0
+    if t.__class__ is torch.Tensor and t.dtype is torch.int32 and t.shape == (batch,) and t.get_device() == index and t.is_contiguous():
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.shape != (batch,):
         raise TypeError(f"{name} must be an int32 tensor of shape ({batch},)")
     if t.get_device() != index or not t.is_contiguous():
@@ -377,13 +385,13 @@ def _ints(t: Optional[torch.Tensor], name: str, batch: int, index: int) -> int:
 def _kv4_parts(cache: Kv4Cache, index: int):
     """(batch, kv heads, cache length, head_dim, type) of a 4-bit cache."""
     kc, vc, km, vm = cache
-    shape = kc.shape
+    shape, dt = kc.shape, km.dtype
     if len(shape) != 4:
         raise ValueError(f"k_codes must have shape (B, Hkv, L, D / 2), not {tuple(shape)}")
     b, h, length, half = shape
-    meta, dt = (b, h, length, half // 32, 2), km.dtype
-    if (kc.dtype is not torch.uint8 or vc.dtype is not torch.uint8 or vm.dtype is not dt or vc.shape != shape or km.shape != meta or vm.shape != meta
-            or half % 32):
+    meta = (b, h, length, half // 32, 2)
+    if not (kc.dtype is torch.uint8 and vc.dtype is torch.uint8 and vm.dtype is dt and vc.shape == shape and km.shape == meta and vm.shape == meta
+            and half % 32 == 0):
         raise ValueError(f"codes must be uint8 (B, Hkv, L, D / 2), meta 16-bit (B, Hkv, L, D / 64, 2), alike for k and v; not "
                          + ", ".join(f"{t.dtype} {tuple(t.shape)}" for t in cache))
     if not (kc.get_device() == vc.get_device() == km.get_device() == vm.get_device() == index
@@ -399,17 +407,13 @@ def _device_index(t: torch.Tensor) -> int:
     return index
 
 
-def _on_device(index: int, call, *args):
-    """call(*args) with device `index` the current one."""
-    if index == torch._C._cuda_getDevice():
-        return call(*args)
-    with torch.cuda.device(index):
-        return call(*args)
+_current_device = torch._C._cuda_getDevice
 
 
-def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int) -> None:
+def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int, count: Optional[int] = None) -> None:
     b, h, length, d, dt = _kv4_parts(cache, index)
-    count = k.shape[2] if k.dim() == 4 else -1
+    if count is None:
+        count = k.shape[2] if k.dim() == 4 else -1
     shape = (b, h, count, d)
     ks, vs = _rows4(k, "k", shape, dt, index), _rows4(v, "v", shape, dt, index)
     one = isinstance(start, int)
@@ -422,7 +426,11 @@ def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int) -> None
             k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr())
     except struct.error as e:
         raise ValueError(f"an argument is no whole number or out of range: {e}") from None
-    status = _entry(name)(packed, _raw_stream(index))
+    if index == _current_device():
+        status = _entry(name)(packed, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = _entry(name)(packed, _raw_stream(index))
     if status:
         L.check(status, name)
 
@@ -434,8 +442,7 @@ def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: Union[i
     ``(x @ wk).view(B, S, Hkv, D).transpose(1, 2)``, needs no copy.  ``start``: an int for all sequences or int32 ``(B,)``;
     ``rows`` int32 ``(B,)``: how many of the ``S`` rows of each sequence are meant (default all).  Other rows, and rows
     whose position lies outside the cache, are not written."""
-    index = _device_index(k)
-    _on_device(index, _kv4_rows, "tb200_kv4_append", cache, k, v, start, rows, index)
+    _kv4_rows("tb200_kv4_append", cache, k, v, start, rows, _device_index(k))
 
 
 def kv4_read(cache: Kv4Cache, start: Union[int, torch.Tensor], count: int, rows: Optional[torch.Tensor] = None,
@@ -450,9 +457,7 @@ def kv4_read(cache: Kv4Cache, start: Union[int, torch.Tensor], count: int, rows:
         make = lambda: torch.zeros(b, h, count, 2 * half, dtype=cache.k_meta.dtype, device=cache.k_codes.device)
         k_out = make() if k_out is None else k_out
         v_out = make() if v_out is None else v_out
-    if k_out.dim() != 4 or k_out.shape[2] != count:
-        raise ValueError(f"k_out must have shape (B, Hkv, {count}, D), not {tuple(k_out.shape)}")
-    _on_device(index, _kv4_rows, "tb200_kv4_read", cache, k_out, v_out, start, rows, index)
+    _kv4_rows("tb200_kv4_read", cache, k_out, v_out, start, rows, index, count)
     return k_out, v_out
 
 
@@ -462,12 +467,16 @@ _WORKSPACE = struct.Struct("@PN")   # the end of _CACHE_ATTN
 
 
 def _cache_attn(name: str, q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index: int):
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return _cache_attn(name, q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index)
     b, h, length, d, dt = dims
-    if q.dim() != 4:
-        raise ValueError(f"q must have shape (B, Hq, S, D), not {tuple(q.shape)}")
     if kv_lens is None:
         raise TypeError("kv_lens must be an int32 tensor")
-    hq, s = q.shape[1], q.shape[2]
+    try:
+        _, hq, s, _ = q.shape
+    except ValueError:
+        raise ValueError(f"q must have shape (B, Hq, S, D), not {tuple(q.shape)}") from None
     if out is None:
         out = torch.empty(b, s, hq, d, dtype=dt, device=q.device).transpose(1, 2)
         if q_rows is not None:
@@ -510,7 +519,7 @@ def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
         raise ValueError(f"k_cache must have shape (B, Hkv, L, D), not {tuple(shape)}")
     ks, vs = _rows4(k_cache, "k_cache", shape, q.dtype, index), _rows4(v_cache, "v_cache", shape, q.dtype, index)
     caches = (k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], 0, 0, 0, 0)
-    return _on_device(index, _cache_attn, "tb200_attn_window", q, out, kv_lens, q_rows, window, sinks, sm_scale, (*shape, q.dtype), caches, index)
+    return _cache_attn("tb200_attn_window", q, out, kv_lens, q_rows, window, sinks, sm_scale, (*shape, q.dtype), caches, index)
 
 
 def kv4_attn(q: torch.Tensor, cache: Kv4Cache, kv_lens: torch.Tensor, *, window: int = 0, sinks: int = 0, sm_scale: float = 1.0,
@@ -520,7 +529,7 @@ def kv4_attn(q: torch.Tensor, cache: Kv4Cache, kv_lens: torch.Tensor, *, window:
     dims = _kv4_parts(cache, index)
     kc, vc, km, vm = cache
     caches = (0, 0, 0, 0, 0, 0, 0, 0, kc.data_ptr(), vc.data_ptr(), km.data_ptr(), vm.data_ptr())
-    return _on_device(index, _cache_attn, "tb200_kv4_attn", q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index)
+    return _cache_attn("tb200_kv4_attn", q, out, kv_lens, q_rows, window, sinks, sm_scale, dims, caches, index)
 
 
 def device_status() -> int:
