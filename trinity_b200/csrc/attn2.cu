@@ -776,8 +776,13 @@ __global__ void attn_combine_kernel(const float* __restrict__ part_o, const floa
   const int lane = threadIdx.x & 31;
   for (long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; row < rows;
        row += (static_cast<long long>(gridDim.x) * blockDim.x) >> 5) {
-    if constexpr (SEQ) {
-      if (seq.q_rows && static_cast<int>(row % S) >= __ldg(seq.q_rows + row / (static_cast<long long>(S) * Hq))) continue;
+    int qi = 0, hq = 0, b = 0;
+    if constexpr (SEQ) {   // 32 bits do: keys are shared out only where blocks of rows are fewer than SMs
+      const uint32_t r = static_cast<uint32_t>(row), bh = r / static_cast<uint32_t>(S);
+      qi = static_cast<int>(r - bh * S);
+      b = static_cast<int>(bh / static_cast<uint32_t>(Hq));
+      hq = static_cast<int>(bh - static_cast<uint32_t>(b) * Hq);
+      if (seq.q_rows && qi >= __ldg(seq.q_rows + b)) continue;
     }
     // all the shares' loads are in flight together: one trip to L2, not one per share
     float2 ml[kMaxSplits];
@@ -809,9 +814,11 @@ __global__ void attn_combine_kernel(const float* __restrict__ part_o, const floa
       for (int i = 0; i < V; ++i) acc[i] = fmaf(w, po[s][i], acc[i]);
     }
     const float inv_l = l > 0.f ? 1.f / l : 0.f;
-    const int qi = static_cast<int>(row % S);
-    const int hq = static_cast<int>((row / S) % Hq);
-    const int b = static_cast<int>(row / (static_cast<long long>(S) * Hq));
+    if constexpr (!SEQ) {
+      qi = static_cast<int>(row % S);
+      hq = static_cast<int>((row / S) % Hq);
+      b = static_cast<int>(row / (static_cast<long long>(S) * Hq));
+    }
     T* at = o2 + ((static_cast<long long>(b) * S + qi) * Hq + hq) * D;
     if constexpr (SEQ) at = o2 + b * seq.o_stride[0] + hq * seq.o_stride[1] + qi * seq.o_stride[2];
     uint32_t* dst = reinterpret_cast<uint32_t*>(at + lane * V);
