@@ -1,0 +1,84 @@
+"""Attention over 16-bit and 4-bit caches against 64 bits, within a bound that follows the data (tests/cache_attn_bound.py):
+long contexts, where the output is small beside the values, included.  Rows at the borders of tiles, windows and first
+positions are sixteen times larger than the others; tests/test_cache_attn_bound.py shows what the bound notices."""
+import pytest
+import torch
+
+from tests import cache_attn_bound as B
+from tests.test_cache_attn_bound import SHAPES as CPU_SHAPES
+from tests.test_gpu_cache_attn import SHAPES as GPU_SHAPES
+from trinity_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float16]
+EPS16 = B.half_step(torch.float16)
+
+# b, hq, hkv, d, s, cache length, lens, rows, window, sinks
+SHAPES = GPU_SHAPES + CPU_SHAPES[-2:] + [
+    (24, 32, 8, 128, 1, 3000, [3000 - 117 * i for i in range(24)], [1] * 24, 0, 0),
+    (3, 32, 4, 128, 3, 20000, [20000, 7001, 13000], [3, 1, 2], 0, 0),
+    (1, 16, 1, 64, 6, 33000, [32999], [6], 0, 0),
+    (5, 24, 2, 128, 70, 5000, [5000, 70, 4097, 69, 1300], [70, 70, 1, 33, 64], 0, 0),
+    (2, 40, 8, 64, 2, 17000, [17000, 16001], [2, 2], 9000, 63),
+]
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def held4(k, v):
+    """A 4-bit cache of the 16-bit rows k, v, and (k, v, weight of v) in 64 bits."""
+    b, h, length, d = k.shape
+    cache = ops.kv4_cache(b, h, length, d, k.dtype, DEV)
+    wide = []
+    for x, codes, meta in ((k, cache.k_codes, cache.k_meta), (v, cache.v_codes, cache.v_meta)):
+        c, s, lo = B.quantise64(x)
+        codes[:, :, :length], meta[:, :, :length] = B.pack4(c), torch.stack([s, lo], -1)
+        wide.append(B.values64(codes[:, :, :length], meta[:, :, :length]))
+    return cache, wide[0][0], wide[1][0], wide[1][1]
+
+
+def run4(q, cache, k, v, w, lens, rows, window, sinks, scale):
+    """kv4_attn and how far it is off, as a multiple of the bound."""
+    b, hq, s, d = q.shape
+    out = torch.full((b, s, hq, d), 7.0, dtype=q.dtype, device=DEV).transpose(1, 2)
+    ops.kv4_attn(q, cache, ints(lens), window=window, sinks=sinks, sm_scale=scale, q_rows=ints(rows), out=out)
+    assert ops.device_status() == 0
+    prompt = s > 1 and s * hq // k.shape[1] > 64       # the form that rounds keys and values to 11 bits
+    want, bound = B.attention_and_bound(q, k, v, lens, rows, window, sinks, scale, q.dtype, EPS16, weight=w * 2 ** 0.5 if prompt else w,
+                                        eps_k=EPS16 if prompt else 0.0)
+    return B.worst(out, want, bound)
+
+
+def run16(q, k, v, lens, rows, window, sinks, scale):
+    b, hq, s, d = q.shape
+    out = torch.full((b, s, hq, d), 7.0, dtype=q.dtype, device=DEV).transpose(1, 2)
+    ops.attn_window(q, k, v, ints(lens), window=window, sinks=sinks, sm_scale=scale, q_rows=ints(rows), out=out)
+    assert ops.device_status() == 0
+    want, bound = B.attention_and_bound(q, k.double(), v.double(), lens, rows, window, sinks, scale, q.dtype, B.half_step(q.dtype))
+    return B.worst(out, want, bound)
+
+
+def data(shape, dt, seed=5):
+    b, hq, hkv, d, s, length, lens, rows, window, sinks = shape
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q = torch.randn(b, s, hq, d, generator=g, device=DEV).to(dt).transpose(1, 2)
+    k = (torch.randn(b, hkv, length, d, generator=g, device=DEV) + torch.randn(1, hkv, 1, d, generator=g, device=DEV)).to(dt)
+    v = B.marked(torch.randn(b, hkv, length, d, generator=g, device=DEV), lens, rows, window, sinks).to(dt)
+    return q, k, v
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_kv4_attn(shape, dt):
+    q, k, v = data(shape, dt)
+    assert run4(q, *held4(k, v), *shape[6:], shape[3] ** -0.5) <= 1
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_attn_window(shape, dt):
+    q, k, v = data(shape, dt)
+    assert run16(q, k, v, *shape[6:], shape[3] ** -0.5) <= 1
