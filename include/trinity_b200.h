@@ -366,8 +366,8 @@ int tb200_kv4_rows_check(const tb200_kv4_rows_args* args);
  * sees; a row that sees nothing (n < r, n = 0) gives zeros.  Rows i >= r of o are left as they are.
  * kv_lens[b] outside [0, cache_len] and q_rows[b] outside [0, rows] are taken as the nearer end.
  * Cache rows that no query row of their sequence sees have no influence, whatever they hold; an
- * infinity or a NaN in a row that some query row sees may also reach the other new rows of that
- * sequence in the same call.
+ * infinity or a NaN in a row that some query row sees, or a score past fp32's range, may also reach the
+ * other new rows of that sequence in the same call.
  *
  * tb200_attn_window: 16-bit caches, tb200_kv4_attn: 4-bit caches as above.  q, o and the 16-bit caches
  * are addressed by element strides (multiples of 8, head_dim contiguous); o overlaps no input.  Workspace: as the

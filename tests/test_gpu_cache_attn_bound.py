@@ -82,3 +82,18 @@ def test_kv4_attn(shape, dt):
 def test_attn_window(shape, dt):
     q, k, v = data(shape, dt)
     assert run16(q, k, v, *shape[6:], shape[3] ** -0.5) <= 1
+
+
+@pytest.mark.parametrize("kv4", [True, False])
+@pytest.mark.parametrize("s", [1, 3, 10, 40])
+@pytest.mark.parametrize("e", [-120, -90, -64, 63, 64, 100, 107, 112, 120, 124])
+def test_queries_and_keys_of_any_size(e, s, kv4):
+    """bf16 queries 2^e times larger and keys as much smaller: the same scores.  One query row is of ordinary size, some keys
+    are zeros."""
+    shape = (2, 4, 1, 128, s, 512, [500, 77], [s, s], 0, 0)
+    q, k, v = data(shape, torch.bfloat16)
+    q, k = (q.float() * 2.0 ** e).to(q.dtype), (k.float() * 2.0 ** -e).to(k.dtype)
+    q[0, 1, 0] = (q[0, 1, 0].float() * 2.0 ** -e).to(q.dtype) if e > 0 else q[0, 1, 0]
+    k[:, :, 3::7] = 0
+    off = run4(q, *held4(k, v), *shape[6:], 128 ** -0.5) if kv4 else run16(q, k, v, *shape[6:], 128 ** -0.5)
+    assert off <= 1

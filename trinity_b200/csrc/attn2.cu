@@ -505,8 +505,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd2_kernel(const __grid_con
             const float4 f = __ldcg(p.head_factor + it.b * p.Hkv + it.hkv);
             const int tok = fdiv(r_in, p.d_pack);
             const long long row = (static_cast<long long>(it.b) * p.Hq + it.hq) * p.pack + r_in - tok * p.pack;
-            // never 0: a hidden score is -inf times this
-            if (qi < it.rows && tok < p.tokens) scale_log2 = fmaxf(p.scale_log2 * f.y * __ldcg(p.q_factor + row * p.S + qi), 1.17549435e-38f);
+            // never 0 nor infinite: a hidden score is -inf times this, one of a key of zeros 0
+            if (qi < it.rows && tok < p.tokens)
+              scale_log2 = fminf(fmaxf(p.scale_log2 * __ldcg(p.q_factor + row * p.S + qi) * f.y, 1.17549435e-38f), 3.402823466e38f);
             v_factor = f.w;
           }
         }

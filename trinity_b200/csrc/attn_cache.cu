@@ -139,8 +139,9 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
 
     // ---- the unit's query rows: MMA column m is row rt * R + m, i.e. (token, query head of the group)
     uint32_t qf[NT][NG][4][2];
-    float qs[NT][NG][2], cf[NT][2];
+    float qs[NT][NG][2], cf[NT][2], up[NT], down[NT], sum[NT][NG];
     int cpos[NT][2];
+    uint32_t unit_top = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int m = rt * R + (nt * 8 + g) % R;
@@ -149,10 +150,9 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
       const int hq = h * p.group + (live ? m - tok * p.group : 0);
       const T* qp = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + hq * p.qs[1] + tok * p.qs[2] + t * 16;
       float v[NG][16];
-      float top = 0.f, sum[NG];
+      float top = 0.f;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        sum[gr] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint4 raw = live ? __ldg(reinterpret_cast<const uint4*>(qp + gr * 64) + i) : make_uint4(0u, 0u, 0u, 0u);
@@ -165,39 +165,46 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
           }
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          top = fmaxf(top, fabsf(v[gr][e]));
-          sum[gr] += v[gr][e];
-        }
-        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(v[gr][e]));
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      unit_top = max(unit_top, __float_as_uint(top));
       // a power of two that brings the row's largest magnitude to [8, 16)
-      const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 30);
-      const float up = __uint_as_float(static_cast<uint32_t>(257 - ex) << 23);        // 2^(130 - ex)
-      const float down = __uint_as_float(static_cast<uint32_t>(ex - 3) << 23);        // its inverse
+      const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 4);
+      up[nt] = __uint_as_float(static_cast<uint32_t>(257 - ex) << 23);        // 2^(130 - ex)
+      down[nt] = __uint_as_float(static_cast<uint32_t>(ex - 3) << 23);        // its inverse
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
+      for (int gr = 0; gr < NG; ++gr) {
+        float x = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x += v[gr][e] *= up[nt];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        sum[nt][gr] = x + __shfl_xor_sync(0xffffffffu, x, 2);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           const int e = (ks >> 1) * 8 + (ks & 1) * 2;
-          qf[nt][gr][ks][0] = Pack2<__half>::pack(v[gr][e] * up, v[gr][e + 4] * up);
-          qf[nt][gr][ks][1] = Pack2<__half>::pack(v[gr][e + 1] * up * 0.0625f, v[gr][e + 5] * up * 0.0625f);
+          qf[nt][gr][ks][0] = Pack2<__half>::pack(v[gr][e], v[gr][e + 4]);
+          qf[nt][gr][ks][1] = Pack2<__half>::pack(v[gr][e + 1] * 0.0625f, v[gr][e + 5] * 0.0625f);
         }
+      }
+    }
+    // The products come out times 2^-24.  Its inverse belongs to the row's factor cf, where large keys leave room for it; rows
+    // from 2^64 on have none in cf and take it with s and lo (keys that would be too large for that have no finite score).
+    const bool large = __reduce_max_sync(0xffffffffu, unit_top) >= (191u << 23);
+    const float kf = large ? 16777216.f : 1.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {   // what columns 2t and 2t + 1 need of their rows
         const int src = (2 * t + c) * 4;
-        const float u = __shfl_sync(0xffffffffu, up, src);
-        // 2^24, and never 0: a hidden score is -inf times this
-        cf[nt][c] = fmaxf(__shfl_sync(0xffffffffu, down, src) * (p.scale_log2 * 16777216.f), 1.17549435e-38f);
+        // never 0 nor infinite: a hidden score is -inf times this, one of a key of zeros 0
+        cf[nt][c] = fminf(fmaxf(__shfl_sync(0xffffffffu, down[nt], src) * (large ? p.scale_log2 : p.scale_log2 * 16777216.f), 1.17549435e-38f), 3.402823466e38f);
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[gr], src) * u * 5.9604644775390625e-8f;   // 2^-24
+        for (int gr = 0; gr < NG; ++gr) qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[nt][gr], src) * (large ? 1.f : 5.9604644775390625e-8f);   // 2^-24
         const int mc = rt * R + (nt * 8 + 2 * t + c) % R;
         cpos[nt][c] = mc < n_rows ? sq.n - sq.r + mc / p.group : -1;
       }
-    }
 
     // o, z, l: relative to 2^(maximum) and, all alike, times 2^(5 - exponent of the largest V scale so far), see `ev`
     float o[NT][NG][4][4], o8[NT][NG][2], z[NT][NG][2], l[NT][2], mx[NT][2], shift[NT][2];
@@ -263,6 +270,8 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
             const int key = H == 2 ? key0 + (t >> 1) * 8 : key0 + j * 8;
             float2 m[NG];
             load_meta<T, NG>(km + key * (NG * 4), m);
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) m[gr].x *= kf;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -236,9 +236,9 @@ __device__ __forceinline__ uint4 decode8_scaled(uint32_t word, uint32_t meta, fl
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// A power of two that brings `top` to [2^to, 2^(to + 1)), and its inverse.
-__device__ __forceinline__ float2 power_for(float top, int to) {
-  const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 40);
+// A power of two that brings `top`, or 2^(least - 127) where that is more, to [2^to, 2^(to + 1)), and its inverse; least > to.
+__device__ __forceinline__ float2 power_for(float top, int to, int least) {
+  const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), least);
   return make_float2(__uint_as_float(static_cast<uint32_t>(254 + to - ex) << 23), __uint_as_float(static_cast<uint32_t>(ex - to) << 23));
 }
 
@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(kFactorThreads) kv4_factors_kernel(const __gri
 #pragma unroll
           for (int g = 0; g < D / 64; ++g) {
             const float2 sl = Pack2<__nv_bfloat16>::unpack(u[g]);
-            const float x = fmaxf(fabsf(sl.y), fabsf(fmaf(15.f, sl.x, sl.y)));
-            top[w] = fmaxf(top[w], x < INFINITY ? x : 0.f);
+            const float x = fmaxf(fabsf(sl.y), fabsf(fmaf(15.f, sl.x, sl.y)));   // (s is rounded: lo + 15 s may pass fp32's range)
+            if (sl.x < INFINITY && fabsf(sl.y) < INFINITY) top[w] = fmaxf(top[w], fminf(x, 3.402823466e38f));
           }
         }
       }
@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(kFactorThreads) kv4_factors_kernel(const __gri
 #pragma unroll
           for (int d = 16; d > 0; d >>= 1) top[w] = fmaxf(top[w], __shfl_xor_sync(0xffffffffu, top[w], d));
         }
-        const float2 k = power_for(top[0], 14), v = power_for(top[1], 14);   // below 2^15: fp16 ends at 65504
+        // below 2^15: fp16 ends at 65504.  V's inverse is divided by a sum of up to 2^39 before it meets the output: above 2^-102
+        const float2 k = power_for(top[0], 14, 16), v = power_for(top[1], 14, 40);
         if (lane == 0) f.head_factor[bh] = make_float4(k.x, k.y, v.x, v.y);
       }
       __syncthreads();
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(kFactorThreads) kv4_factors_kernel(const __gri
       }
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float2 pw = power_for(top, 3);
+      const float2 pw = power_for(top, 3, 5);
       const long long out = static_cast<long long>(b) * rows + row;
       uint32_t* dst = reinterpret_cast<uint32_t*>(f.q16 + out * D * 2) + lane * (V / 2);
 #pragma unroll
