@@ -97,3 +97,36 @@ def test_queries_and_keys_of_any_size(e, s, kv4):
     k[:, :, 3::7] = 0
     off = run4(q, *held4(k, v), *shape[6:], 128 ** -0.5) if kv4 else run16(q, k, v, *shape[6:], 128 ** -0.5)
     assert off <= 1
+
+
+@pytest.mark.parametrize("s", [1, 3, 10, 40])
+@pytest.mark.parametrize("size", [1e30, 1e12, 1e-12, 1e-24, 1e-27, 1e-30, 1e-33])
+def test_kv4_attn_values_of_any_size(size, s):
+    """The products with V are fp16: V far from 1 altogether."""
+    shape = (2, 4, 1, 128, s, 512, [500, 77], [s, s], 0, 0)
+    q, k, v = data(shape, torch.bfloat16)
+    assert run4(q, *held4(k, (v.float() * size).to(v.dtype)), *shape[6:], 128 ** -0.5) <= 1
+
+
+@pytest.mark.parametrize("dt,s,first,second", [(torch.bfloat16, s, 1.0, x) for s in (1, 3, 10) for x in (1e6, 1e-4, 1e-6, 1e-9, 1e-24)]
+                         + [(torch.float16, s, 100.0, x) for s in (1, 3, 10, 40) for x in (1.0, 1e-2, 1e-3)]
+                         + [(torch.bfloat16, 40, 1.0, x) for x in (1e6, 1e-4, 1e-6)])
+def test_kv4_attn_groups_of_unlike_size(dt, s, first, second):
+    """64 channels of V many times smaller than the others keep their digits."""
+    shape = (2, 4, 1, 128, s, 512, [500, 77], [s, s], 0, 0)
+    q, k, v = data(shape, dt)
+    v = torch.cat([v[..., :64].float() * first, v[..., 64:].float() * second], -1).to(dt)
+    assert run4(q, *held4(k, v), *shape[6:], 128 ** -0.5) <= 1
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("s", [1, 3])
+def test_kv4_attn_values_that_grow(s, dt):
+    """Larger values the later a key comes: what has been summed is brought to the new scale, group by group."""
+    shape = (1, 8, 2, 128, s, 12000, [11999], [s], 0, 0)
+    q, k, v = data(shape, dt)
+    grow = 2.0 ** torch.linspace(-10, 10 if dt == torch.bfloat16 else 6, 12000, device=DEV)
+    f = v.float()
+    f[..., :64] *= grow[:, None]
+    f[..., 64:] *= grow.flip(0)[:, None]
+    assert run4(q, *held4(k, f.to(dt)), *shape[6:], 128 ** -0.5) <= 1

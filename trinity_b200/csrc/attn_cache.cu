@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
   constexpr int R = L::kR, kTile = L::kTile, kStages = L::kStages;
   // fp16 outputs are worth the centred codes (see above); bf16's own rounding is sixteen times coarser than what they gain
   constexpr bool kCentre = !IsBf16<T>::value;
+  constexpr bool kGroupScale = NG > 1 || IsBf16<T>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
         cpos[nt][c] = mc < n_rows ? sq.n - sq.r + mc / p.group : -1;
       }
 
-    // o, z, l: relative to 2^(maximum) and, all alike, times 2^(5 - exponent of the largest V scale so far), see `ev`
+    // z, l: relative to 2^(maximum) and times 2^(5 - ev), o and o8 of a group times vf besides, see below
     float o[NT][NG][4][4], o8[NT][NG][2], z[NT][NG][2], l[NT][2], mx[NT][2], shift[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -222,6 +223,11 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
         l[nt][c] = shift[nt][c] = 0.f;
       }
     int ev = 60;   // biased exponent of the largest V scale so far, at least this
+    // 2^(ev - exponent of the largest V scale so far of the group): groups of unlike size, and V below 2^(60 - 127) altogether,
+    // bring p s near 2^14 all the same.  At most 2^120.  One group of fp16 needs none
+    float vf[NG];
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) vf[gr] = kGroupScale ? 576460752303423488.f : 1.f;   // 2^59
 
     for (int v = v0 + warp; v < v1; v += kWarps) {
       const uint32_t slot = used % kStages;
@@ -291,24 +297,26 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
 
         // ---- running maximum of the scores and of the V scales: what a thread sees of either decides whether the warp has
         //      to look closer
+        auto scales = [&](auto take) {   // each lane two keys of 64: s and lo of their groups in V, as bits
+#pragma unroll
+          for (int i = 0; i < kTile / 32; ++i) {
+            const int key = i * 32 + lane;
+            bool alive = true;
+            if (!full) {
+              const int a = k0 + key;
+              alive = a < sq.n && (p.window == 0 || a > sq.n - sq.r - p.window || a < p.sinks);
+            }
+            float2 mv[NG];
+            load_meta<T, NG>(vm + key * (NG * 4), mv);
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+              const int u = __float_as_int(mv[gr].x), w = __float_as_int(fabsf(mv[gr].y));
+              if (alive && u < 0x7f800000 && w < 0x7f800000) take(gr, u, w - (60 << 23));   // lo counts where it is 2^60 times the scale: the sums of p lo have to stay in fp32 too
+            }
+          }
+        };
         int big = 0;
-#pragma unroll
-        for (int i = 0; i < kTile / 32; ++i) {
-          const int key = i * 32 + lane;
-          bool alive = true;
-          if (!full) {
-            const int a = k0 + key;
-            alive = a < sq.n && (p.window == 0 || a > sq.n - sq.r - p.window || a < p.sinks);
-          }
-          float2 mv[NG];
-          load_meta<T, NG>(vm + key * (NG * 4), mv);
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-            const int u = __float_as_int(mv[gr].x), w = __float_as_int(fabsf(mv[gr].y));
-            // lo counts where it is 2^60 times the scale: the sums of p lo have to stay in fp32 too
-            if (alive && u < 0x7f800000 && w < 0x7f800000) big = max(big, max(u, w - (60 << 23)));
-          }
-        }
+        scales([&](int gr, int u, int w) { big = max(big, max(kGroupScale ? __float_as_int(__int_as_float(u) * vf[gr]) : u, w)); });
         float top[NT][2];
         bool grown = (big >> 23) > ev;
 #pragma unroll
@@ -324,8 +332,29 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
             grown |= top[nt][c] > mx[nt][c] + kSlack;
           }
         if (__any_sync(0xffffffffu, grown)) {
+          [[maybe_unused]] int own[NG];
+          if constexpr (kGroupScale) {   // (`big` may have passed the range of a float's bits)
+            big = 0;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) own[gr] = 0;
+            scales([&](int gr, int u, int w) {
+              own[gr] = max(own[gr], u);
+              big = max(big, max(u, w));
+            });
+          }
           const int ev_new = max(ev, __reduce_max_sync(0xffffffffu, big) >> 23);
           const float shrink = __uint_as_float(static_cast<uint32_t>(max(127 + ev - ev_new, 0)) << 23);   // 2^(ev - ev_new)
+          float shrink_o[NG];
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            shrink_o[gr] = shrink;
+            if constexpr (kGroupScale) {
+              const int eg = ev + 127 - static_cast<int>(__float_as_uint(vf[gr]) >> 23);   // the group's exponent so far
+              const int eg_new = max(max(eg, __reduce_max_sync(0xffffffffu, own[gr]) >> 23), ev_new - 120);
+              shrink_o[gr] = __uint_as_float(static_cast<uint32_t>(max(127 + eg - eg_new, 0)) << 23);
+              vf[gr] = __uint_as_float(static_cast<uint32_t>(127 + ev_new - eg_new) << 23);
+            }
+          }
           ev = ev_new;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -335,18 +364,19 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
               m_new = fmaxf(m_new, mx[nt][c]);
-              const float a = (m_new == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - m_new)) * shrink;
+              const float e = m_new == -INFINITY ? 1.f : fast_exp2(mx[nt][c] - m_new), a = e * shrink;
               mx[nt][c] = m_new;
               shift[nt][c] = static_cast<float>(132 - ev) - (m_new == -INFINITY ? 0.f : m_new);   // 5 - (ev - 127): with p <= 2^kSlack, p s < 2^14
               l[nt][c] *= a;
 #pragma unroll
               for (int gr = 0; gr < NG; ++gr) {
                 z[nt][gr][c] *= a;
-                if (kCentre) o8[nt][gr][c] *= a;
+                const float ao = e * shrink_o[gr];
+                if (kCentre) o8[nt][gr][c] *= ao;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  o[nt][gr][i][c] *= a;
-                  o[nt][gr][i][2 + c] *= a;
+                  o[nt][gr][i][c] *= ao;
+                  o[nt][gr][i][2 + c] *= ao;
                 }
               }
             }
@@ -377,6 +407,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
             for (int j = 0; j < KN; ++j) {
               m[j] = Pack2<T>::unpack(*reinterpret_cast<const uint32_t*>(vm + ((key0 + j * 8) * NG + gr) * 4));
               lo8[j] = kCentre ? fmaf(8.f, m[j].x, m[j].y) : m[j].y;
+              if (kGroupScale) m[j].x *= vf[gr];
             }
             uint32_t pf[NT][2];
 #pragma unroll
@@ -465,10 +496,11 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) zs += __shfl_xor_sync(0xffffffffu, zs, d);
           const float a8 = kCentre ? o8[nt][gr][c] : 0.f;
+          const float out = __uint_as_float((278u << 23) - __float_as_uint(vf[gr]));   // 2^24 / vf
 #pragma unroll
-          for (int i = 0; i < 4; ++i)   // 2^24; row g + 8 holds codes times 2^-20
+          for (int i = 0; i < 4; ++i)   // row g + 8 holds codes times 2^-20
             *reinterpret_cast<float2*>(wm + m * M::kPitch + gr * 64 + g * 8 + 2 * i) =
-                make_float2(fmaf(o[nt][gr][i][c] - a8, 16777216.f, zs) * fe, fmaf(o[nt][gr][i][2 + c] * 0.0625f - a8, 16777216.f, zs) * fe);
+                make_float2(fmaf(o[nt][gr][i][c] - a8, out, zs) * fe, fmaf(o[nt][gr][i][2 + c] * 0.0625f - a8, out, zs) * fe);
         }
       }
     __syncthreads();
