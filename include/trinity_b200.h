@@ -319,8 +319,10 @@ int tb200_kv_compact(const tb200_kv_compact_args* args, void* stream);
  *
  * A group is 64 consecutive values x of a row.  lo = min x, s = (max x - min x) / 15, computed in
  * fp32 and rounded to the cache's 16-bit type; c = the whole number nearest to the fp32 quotient
- * (x - lo) / s, at most 15 (halves to even; 0 where s is 0).  The group stands for lo + c * s.  A group that holds an infinity
- * or a NaN, or whose max - min is not finite in fp32, stands for NaN throughout.
+ * (x - lo) / s, at most 15 (halves to even; 0 where s is 0).  Difference and quotient are each rounded to
+ * fp32: an x within 2^-19 s of the middle between two codes may get either.  The group stands for
+ * lo + c * s.  A group that holds an infinity or a NaN, or whose max - min is not finite in fp32, stands
+ * for NaN throughout.
  *   codes  (B, Hkv, cache_len, D/2) bytes: element 2i in the low, 2i+1 in the high four bits of byte i
  *   meta   (B, Hkv, cache_len, D/64, 2) of the cache's type: s, lo
  * cache_len is a multiple of 4; codes and meta are contiguous and 16-byte aligned.

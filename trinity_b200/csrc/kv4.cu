@@ -73,16 +73,18 @@ __device__ __forceinline__ float fifteenth(float x) {
   const float r = __fmaf_rn(__fmaf_rn(q, -15.f, x), kInv, q);
   return x < 1e-30f ? __fdiv_rn(x, 15.f) : r;
 }
-// Below this scale its rounding to the type is so coarse that a quotient may pass 15.5.
+// Below this scale encode8 divides.  fp16, 2^-19: s is rounded so coarsely (steps of 2^-24) that a quotient may pass 15.5.
+// bf16, 2^-120: the Newton step's remainder may need digits below fp32's smallest.
 template <typename T> struct SmallScale;
-template <> struct SmallScale<__half> { static constexpr float value = 1.9073486328125e-06f; };        // 2^-19: steps of 2^-24
-template <> struct SmallScale<__nv_bfloat16> { static constexpr float value = 1.17549435e-38f; };      // 2^-126
+template <> struct SmallScale<__half> { static constexpr float value = 1.9073486328125e-06f; };
+template <> struct SmallScale<__nv_bfloat16> { static constexpr float value = 7.52316385e-37f; };
 
-// Codes of eight values of a group: round((x - lo) / s), halves to even.  bf16 values lie on few places, so a quotient is
-// exactly k + 1/2 in about one group of eight out of twenty, and it has to come out as just that: the approximate quotient
-// q0 = t inv is followed by one Newton step, q = q0 + (t - q0 s) inv with the remainder exact in a fused multiply-add
-// (P. Markstein, IBM J. Res. Dev. 34, 1990), which is the correctly rounded quotient.  Adding 1.5 * 2^23 rounds q to a
-// whole number and leaves the code in the sum's low bits.
+// Codes of eight values of a group: round(t / s), halves to even, with t = x - lo rounded to fp32.  bf16 values lie on few
+// places, so a quotient is exactly k + 1/2 in about one group of eight out of twenty, and it has to come out as just that: the
+// approximate quotient q0 = t inv is followed by one Newton step, q = q0 + (t - q0 s) inv with the remainder exact in a fused
+// multiply-add (P. Markstein, IBM J. Res. Dev. 34, 1990), which is t / s correctly rounded.  Adding 1.5 * 2^23 rounds q to a
+// whole number and leaves the code in the sum's low bits.  (An x that is tiny beside lo is gone from t: where -lo / s is
+// k + 1/2, its code is the even one, whatever its sign.  Both codes are as far from x, to 2^-19 s.)
 // (Approximate quotients re-examined in 64 bits wherever one lay next to a border took twice as long.)
 template <typename T>
 __device__ __forceinline__ uint32_t encode8(const uint32_t (&w)[4], float lo, float s) {
@@ -102,7 +104,7 @@ __device__ __forceinline__ uint32_t encode8(const uint32_t (&w)[4], float lo, fl
   constexpr uint32_t kBits = 0x4b400000u;
   constexpr uint32_t kCarry = kBits * 0x11111111u;
   word -= kCarry;
-  if (!(s >= SmallScale<T>::value)) {   // 0, NaN, or so coarse that a quotient may pass 15.5
+  if (!(s >= SmallScale<T>::value)) {   // 0, NaN or small
     word = 0;
     if (s > 0.f) {
 #pragma unroll 1
