@@ -116,6 +116,7 @@ struct Attn2Params {
   const int32_t* kv_lens;
   const int32_t* q_rows;
   int cache_len, window, sinks;
+  int packed_head;   // >= 0: k and v hold the visible positions only, those of the window from this place on
   int pack, tokens;  // query heads of a query tile, tokens of a query tile (tokens * pack <= BQ)
   FastDiv d_pack, d_per_seq_blk;   // pack; Hq * kv_splits
   const float* q_factor;      // SEQ with Out != T: what the rows of q and the heads' K and V have been divided by (powers of two)
@@ -169,8 +170,11 @@ template <int SEQ> __device__ __forceinline__ Item decode_item(const Attn2Params
   it.hkv = fdiv(it.hq, p.d_group);
   it.q0 = (blocks - 1 - blk) * 2 * (SEQ ? p.tokens : BQ);   // SEQ: hq counts packs of heads
   if constexpr (SEQ) {
-    const int n = max(0, min(__ldg(p.kv_lens + it.b), p.cache_len));
+    int n = max(0, min(__ldg(p.kv_lens + it.b), p.cache_len));
     it.rows = p.q_rows ? max(0, min(__ldg(p.q_rows + it.b), p.S)) : p.S;
+    // Closed up: the positions behind the gap move, the sequence's end and every row with them, and each row sees what it saw
+    // (what lies between the first positions and packed_head is in nobody's window).
+    if (p.packed_head >= 0 && n - it.rows - p.window + 1 > p.sinks) n = it.rows + p.window - 1 + p.packed_head;
     it.past = n - it.rows;   // negative: the first rows stand before the first position and see nothing
     const int low = p.window > 0 ? max(0, it.past + it.q0 - p.window + 1) : 0;
     const bool apart = low > p.sinks;   // else the line is simply the sequence
@@ -969,7 +973,7 @@ int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
   p.tokens = BQ / a.pack;
   p.d_pack = make_fastdiv(static_cast<uint32_t>(a.pack));
   p.B = a.B; p.S = a.S; p.Hq = a.Hq / a.pack; p.Hkv = a.Hkv; p.kv_len = a.cache_len; p.causal = 1;
-  p.cache_len = a.cache_len; p.window = a.window; p.sinks = a.sinks;
+  p.cache_len = a.cache_len; p.window = a.window; p.sinks = a.sinks; p.packed_head = a.packed_head;
   p.kv_lens = a.kv_lens; p.q_rows = a.q_rows;
   p.q_factor = a.q_factor;
   p.head_factor = reinterpret_cast<const float4*>(a.head_factor);
@@ -999,11 +1003,11 @@ int launch_attn_fwd_seq(const AttnSeqLaunch& a, cudaStream_t stream) {
     return make_tensor_map(map, base, 5, dims, strides, box);
   };
   if ((status = map5(&p.map_q, a.q, a.q_stride)) != TB200_OK) return status;
-  if ((status = map4(&p.map_k, a.k_cache, a.cache_len, a.Hkv, a.k_stride, BQ)) != TB200_OK) return status;
-  if ((status = map4(&p.map_v, a.v_cache, a.cache_len, a.Hkv, a.v_stride, BQ)) != TB200_OK) return status;
+  if ((status = map4(&p.map_k, a.k_cache, a.len, a.Hkv, a.k_stride, BQ)) != TB200_OK) return status;
+  if ((status = map4(&p.map_v, a.v_cache, a.len, a.Hkv, a.v_stride, BQ)) != TB200_OK) return status;
   if (a.sinks > 0) {
-    if ((status = map4(&p.map_k16, a.k_cache, a.cache_len, a.Hkv, a.k_stride, 16)) != TB200_OK) return status;
-    if ((status = map4(&p.map_v16, a.v_cache, a.cache_len, a.Hkv, a.v_stride, 16)) != TB200_OK) return status;
+    if ((status = map4(&p.map_k16, a.k_cache, a.len, a.Hkv, a.k_stride, 16)) != TB200_OK) return status;
+    if ((status = map4(&p.map_v16, a.v_cache, a.len, a.Hkv, a.v_stride, 16)) != TB200_OK) return status;
   }
   if ((status = map5(&p.map_o, a.o, a.o_stride)) != TB200_OK) return status;
   const bool ragged = a.q_rows != nullptr && a.B > 1 && a.B <= kRaggedSeqs;

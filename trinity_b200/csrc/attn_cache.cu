@@ -640,6 +640,7 @@ int kv4_ctas(int head_dim, int unit_rows) {
 }
 
 constexpr int kClusterKeys = 640;
+constexpr size_t kCopyBytes = size_t{256} << 20, kCopyMost = size_t{1} << 30;
 
 struct AttnPlan {
   bool prompt = false;       // the prompt kernel (attn2.cu), on a 4-bit cache after reading it back into the workspace
@@ -648,6 +649,9 @@ struct AttnPlan {
   int cluster = 0;           // CTAs per unit, 0: the line
   int stretches = 0;
   int pack = 1, kv_splits = 1;   // prompt
+  // prompt on 4 bits: positions and layout of the 16-bit copy (Kv4PromptOperands), and of how many sequences and kv heads it is at
+  // a time.  What follows is the size of one such piece.
+  int copy_len = 0, packed_head = -1, piece_seqs = 0, piece_heads = 0;
   size_t part_o = 0, part_ml = 0, split = 0;               // bytes
   size_t cache16 = 0, q16 = 0, q_factor = 0, head_factor = 0;   // prompt on 4 bits: one of the two caches; bf16: q and the factors
   // + what brings the caller's address up to a multiple of 256
@@ -665,20 +669,53 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
   if (pl.prompt) {
     const int64_t seen = window > 0 ? static_cast<int64_t>(window) + a->rows + sinks : a->cache_len;
     pl.pack = attn_seq_pack(a->rows, a->n_q_heads, a->n_kv_heads, a->cache_len, window, sinks);
+    pl.piece_seqs = a->batch;
+    pl.piece_heads = a->n_kv_heads;
+    if (kv4) {
+      // The copy holds what a sequence can see, and a piece of the call at a time where it would be larger than kCopyBytes: a
+      // cache is held in 4 bits where 16 do not fit.  Up to kCopyMost where a piece would have fewer than two items per SM, with
+      // the keys in 16 shares; one (sequence, kv head) is the least.  32/8 heads of 128, bf16, the whole cache copied against
+      // this, MiB of scratch and us: 24 sequences of 16384 and 20 tokens 1540, 791 / 262, 790; 100 tokens 1556, 1115 / 272, 1251;
+      // 500 tokens 1632, 3170 / 272, 3465; 16 sequences of 131072 and 20 tokens 8195, 3700 / 1030, 4220; under a window of 1000
+      // 8195, 411 / 67, 48.
+      const int64_t head = (static_cast<int64_t>(sinks) + 15) & ~15;
+      const int64_t packed = head + window + a->rows;
+      pl.copy_len = a->cache_len;
+      if (window > 0 && packed < a->cache_len) {
+        pl.copy_len = static_cast<int>(packed);
+        pl.packed_head = static_cast<int>(head);
+      }
+      const size_t one = static_cast<size_t>(pl.copy_len) * a->head_dim * 4;   // K and V
+      const int group = a->n_q_heads / a->n_kv_heads, tokens = 2 * (128 / pl.pack);
+      const size_t items = static_cast<size_t>(group / pl.pack) * ((a->rows + tokens - 1) / tokens);   // of a (sequence, kv head)
+      const size_t busy = 2 * num_sms / (items * 16), most = kCopyMost / one;
+      size_t fit = busy < most ? busy : most;
+      if (fit < kCopyBytes / one) fit = kCopyBytes / one;
+      if (fit < 1) fit = 1;
+      if (fit < static_cast<size_t>(a->n_kv_heads)) {
+        const int parts = static_cast<int>((a->n_kv_heads + fit - 1) / fit);
+        pl.piece_seqs = 1;
+        pl.piece_heads = (a->n_kv_heads + parts - 1) / parts;
+      } else if (fit / a->n_kv_heads < static_cast<size_t>(a->batch)) {
+        const int seqs = static_cast<int>(fit / a->n_kv_heads), parts = (a->batch + seqs - 1) / seqs;
+        pl.piece_seqs = (a->batch + parts - 1) / parts;
+      }
+    }
+    const int q_heads = a->n_q_heads / a->n_kv_heads * pl.piece_heads;
     // the splits count blocks of 256 rows: tokens times packed heads
-    pl.kv_splits = attn_kv_splits(a->batch, (a->rows + 128 / pl.pack - 1) / (128 / pl.pack) * 128, a->n_q_heads / pl.pack,
+    pl.kv_splits = attn_kv_splits(pl.piece_seqs, (a->rows + 128 / pl.pack - 1) / (128 / pl.pack) * 128, q_heads / pl.pack,
                                   static_cast<int>(seen < a->cache_len ? seen : a->cache_len), num_sms);
     if (pl.kv_splits > 1) {
-      const size_t prows = static_cast<size_t>(pl.kv_splits) * a->batch * a->n_q_heads * a->rows;
+      const size_t prows = static_cast<size_t>(pl.kv_splits) * pl.piece_seqs * q_heads * a->rows;
       pl.part_o = align_up(prows * a->head_dim * sizeof(float), 256);
       pl.part_ml = align_up(prows * 2 * sizeof(float), 256);
     }
-    if (kv4) pl.cache16 = align_up(static_cast<size_t>(a->batch) * a->n_kv_heads * a->cache_len * a->head_dim * 2, 256);
+    if (kv4) pl.cache16 = align_up(static_cast<size_t>(pl.piece_seqs) * pl.piece_heads * pl.copy_len * a->head_dim * 2, 256);
     if (kv4 && a->dtype == TB200_BF16) {
-      const size_t q_rows = static_cast<size_t>(a->batch) * a->n_q_heads * a->rows;
+      const size_t q_rows = static_cast<size_t>(pl.piece_seqs) * q_heads * a->rows;
       pl.q16 = align_up(q_rows * a->head_dim * 2, 256);
       pl.q_factor = align_up(q_rows * sizeof(float), 256);
-      pl.head_factor = align_up(static_cast<size_t>(a->batch) * a->n_kv_heads * 4 * sizeof(float), 256);
+      pl.head_factor = align_up(static_cast<size_t>(pl.piece_seqs) * pl.piece_heads * 4 * sizeof(float), 256);
     }
     return pl;
   }
@@ -783,9 +820,10 @@ int launch_combine(const CacheAttnParams& p, int head_dim, int unit_rows, cudaSt
 }
 
 int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, const CacheAttnParams& p, uint8_t* ws, int num_sms, cudaStream_t stream) {
+  ChainScope chain;
   AttnSeqLaunch s;
   s.dtype = a->dtype;
-  s.B = a->batch; s.S = a->rows; s.Hq = a->n_q_heads; s.Hkv = a->n_kv_heads; s.D = a->head_dim; s.cache_len = a->cache_len;
+  s.B = a->batch; s.S = a->rows; s.Hq = a->n_q_heads; s.Hkv = a->n_kv_heads; s.D = a->head_dim; s.cache_len = s.len = a->cache_len;
   s.window = p.window; s.sinks = p.sinks;
   s.sm_scale = a->sm_scale;
   s.q = a->q; s.o = a->o;
@@ -799,6 +837,8 @@ int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, con
   if (kv4) {
     Kv4PromptOperands to;
     uint8_t* at = ws + pl.part_o + pl.part_ml;
+    to.len = s.len = pl.copy_len;
+    to.packed_head = s.packed_head = pl.packed_head;
     to.k16 = at;
     to.v16 = at += pl.cache16;
     at += pl.cache16;
@@ -817,10 +857,35 @@ int run_prompt(const tb200_cache_attn_args* a, bool kv4, const AttnPlan& pl, con
     if (status != TB200_OK) return status;
     s.k_cache = to.k16; s.v_cache = to.v16;
     s.k_stride[2] = s.v_stride[2] = a->head_dim;
-    s.k_stride[1] = s.v_stride[1] = static_cast<int64_t>(a->cache_len) * a->head_dim;
+    s.k_stride[1] = s.v_stride[1] = static_cast<int64_t>(pl.copy_len) * a->head_dim;
     s.k_stride[0] = s.v_stride[0] = s.k_stride[1] * a->n_kv_heads;
   }
   return launch_attn_fwd_seq(s, stream);
+}
+
+// A prompt on a 4-bit cache, piece by piece.  Each piece is a chain of its own: its first launch waits for the piece before,
+// whose copy it overwrites.
+int run_pieces(const tb200_cache_attn_args* a, const AttnPlan& pl, const CacheAttnParams& p, uint8_t* ws, int num_sms, cudaStream_t stream) {
+  const int group = a->n_q_heads / a->n_kv_heads;
+  for (int b0 = 0; b0 < a->batch; b0 += pl.piece_seqs)
+    for (int h0 = 0; h0 < a->n_kv_heads; h0 += pl.piece_heads) {
+      tb200_cache_attn_args x = *a;
+      x.batch = a->batch - b0 < pl.piece_seqs ? a->batch - b0 : pl.piece_seqs;
+      x.n_kv_heads = a->n_kv_heads - h0 < pl.piece_heads ? a->n_kv_heads - h0 : pl.piece_heads;
+      x.n_q_heads = x.n_kv_heads * group;
+      x.q = static_cast<const uint8_t*>(a->q) + 2 * (b0 * a->q_stride[0] + static_cast<int64_t>(h0) * group * a->q_stride[1]);
+      x.o = static_cast<uint8_t*>(a->o) + 2 * (b0 * a->o_stride[0] + static_cast<int64_t>(h0) * group * a->o_stride[1]);
+      x.kv_lens = a->kv_lens + b0;
+      if (a->q_rows) x.q_rows = a->q_rows + b0;
+      const int64_t crow = (static_cast<int64_t>(b0) * a->n_kv_heads + h0) * a->cache_len;   // (fewer heads: of one sequence)
+      x.k_codes = static_cast<const uint8_t*>(a->k_codes) + crow * (a->head_dim / 2);
+      x.v_codes = static_cast<const uint8_t*>(a->v_codes) + crow * (a->head_dim / 2);
+      x.k_meta = static_cast<const uint8_t*>(a->k_meta) + crow * (a->head_dim / 16);
+      x.v_meta = static_cast<const uint8_t*>(a->v_meta) + crow * (a->head_dim / 16);
+      const int status = run_prompt(&x, true, pl, p, ws, num_sms, stream);
+      if (status != TB200_OK) return status;
+    }
+  return TB200_OK;
 }
 
 int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
@@ -835,8 +900,8 @@ int run_attn(const tb200_cache_attn_args* a, bool kv4, void* stream_) {
   const AttnPlan pl = plan_attn(a, kv4, st->num_sms);
   if (pl.total() > 0 && (!a->workspace || a->workspace_bytes < pl.total())) return TB200_ERR_WORKSPACE;
   uint8_t* ws = reinterpret_cast<uint8_t*>(align_up(reinterpret_cast<size_t>(a->workspace), 256));
+  if (pl.prompt) return kv4 ? run_pieces(a, pl, p, ws, st->num_sms, stream) : run_prompt(a, false, pl, p, ws, st->num_sms, stream);
   ChainScope chain;
-  if (pl.prompt) return run_prompt(a, kv4, pl, p, ws, st->num_sms, stream);
   p.stretches = pl.stretches;
   p.record_per_unit = static_cast<int64_t>(a->batch) * a->n_kv_heads * pl.row_tiles <= pl.stretches;
   p.row_tiles = pl.row_tiles;

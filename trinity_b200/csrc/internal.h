@@ -187,6 +187,7 @@ int attn_kv_splits(int B, int S, int Hq, int kv_len, int num_sms);
 struct AttnSeqLaunch {
   int dtype = TB200_BF16;
   int B = 0, S = 0, Hq = 0, Hkv = 0, D = 0, cache_len = 0, window = 0, sinks = 0;
+  int len = 0, packed_head = -1;    // positions of k_cache and v_cache, and how they are laid out: see Kv4PromptOperands
   float sm_scale = 1.f;
   const void* q = nullptr;
   const void* k_cache = nullptr;
@@ -263,11 +264,14 @@ int launch_kv_compact(const tb200_kv_compact_args& a, cudaStream_t stream);
 // not overlap.  Axes of one element are not looked at.
 int check_strides(const int64_t (&stride)[3], const int64_t (&ext)[3], int head_dim, bool written);
 // A prompt's operands out of a 4-bit cache: the positions that some query row of its sequence sees as contiguous 16-bit
-// caches (B, Hkv, cache_len, D), other positions left as they are.  fp16: the values, rounded (by half a step of the type
+// caches (B, Hkv, len, D), other places left as they are.  packed_head -1: at their own places.  Else, where the window begins
+// behind the first positions that stay visible, the first positions at their places below packed_head, the others from
+// there on; len holds packed_head + window + rows.  fp16: the values, rounded (by half a step of the type
 // the output is rounded to as well).  bf16: in fp16, divided by a
 // power of two per head (head_factor (B, Hkv, 4): 1 / factor and factor of K, of V), and q (B, Hq, rows, D) likewise by one
 // per row (q_factor); q16, q_factor and head_factor are not used for fp16.
 struct Kv4PromptOperands {
+  int len = 0, packed_head = -1;
   void* k16 = nullptr;
   void* v16 = nullptr;
   void* q16 = nullptr;

@@ -27,8 +27,9 @@ struct RowsParams {
   long long stride[2][3];   // elements: batch, head, row
   uint8_t* codes[2];
   uint8_t* meta[2];
-  const int32_t* q_rows;    // SEEN
-  int q_rows_max, window, sinks;
+  // SEEN: n_rows are the sequences' lengths, rows the positions of the 16-bit copy
+  const int32_t* q_rows;
+  int q_rows_max, window, sinks, packed_head;
   const float4* head_factor;
 };
 
@@ -215,15 +216,21 @@ __global__ void __launch_bounds__(kThreads, 4) kv4_append_kernel(const __grid_co
   }
 }
 
-// The positions some query row of sequence b sees: [low, n) and those below few.
+// The positions some query row of sequence b sees: [low, n) and those below few.  In the copy, places below `head` are those
+// positions, places from there on to `places` are positions `off` further on.
 struct SeenRows {
-  int low, few;
+  int n, low, few, head, off, places;
 };
-__device__ __forceinline__ SeenRows seen_rows(const RowsParams& p, int b, int n) {
+__device__ __forceinline__ SeenRows seen_rows(const RowsParams& p, int b) {
   const int r = p.q_rows ? max(0, min(p.q_rows[b], p.q_rows_max)) : p.q_rows_max;
   SeenRows s;
-  s.low = r == 0 ? n : p.window > 0 ? n - r - p.window + 1 : 0;
+  s.n = max(0, min(p.n_rows[b], p.cache_len));
+  s.low = r == 0 ? s.n : p.window > 0 ? s.n - r - p.window + 1 : 0;
   s.few = r > 0 ? p.sinks : 0;
+  const bool packed = p.packed_head >= 0 && s.low > p.sinks;   // (as the attention kernel has it)
+  s.head = packed ? p.packed_head : 0;
+  s.off = packed ? s.low - s.head : 0;
+  s.places = s.n - s.off;
   return s;
 }
 
@@ -266,9 +273,8 @@ __global__ void __launch_bounds__(kFactorThreads) kv4_factors_kernel(const __gri
   for (int b = blockIdx.y; b < f.batch; b += gridDim.y) {
     if (blockIdx.x < p.heads) {
       const long long bh = static_cast<long long>(b) * p.heads + blockIdx.x;
-      const int n = max(0, min(p.n_rows[b], p.rows));
-      const SeenRows seen = seen_rows(p, b, n);
-      const int low = max(seen.low, 0), few = min(seen.few, low);
+      const SeenRows seen = seen_rows(p, b);
+      const int n = seen.n, low = max(seen.low, 0), few = min(seen.few, low);
       float top[2] = {0.f, 0.f};
 #pragma unroll 4
       for (int i = threadIdx.x; i < few + n - low; i += kFactorThreads) {
@@ -350,14 +356,15 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constan
   const int r_in = threadIdx.x / S::kLanes, lane = threadIdx.x % S::kLanes;
   const int chunk = (lane >> 2) * 8 + (lane & 3);
   for (long long u = blockIdx.x; u < p.units; u += gridDim.x) {
-    const Unit x = find_unit(p, u, S::kUnitRows);
+    Unit x = find_unit(p, u, S::kUnitRows);
+    SeenRows seen;
+    if constexpr (SEEN) {
+      seen = seen_rows(p, x.b);
+      x.n = seen.places;
+    }
     if (x.row0 >= x.n) continue;
-    int low = 0, few = 0;
     float down[2] = {1.f, 1.f};
     if constexpr (SEEN) {
-      const SeenRows seen = seen_rows(p, x.b, x.n);
-      low = seen.low;
-      few = seen.few;
       if constexpr (IsBf16<T>::value) {
         const float4 f = __ldcg(p.head_factor + x.bh);
         down[0] = f.x;
@@ -369,9 +376,12 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constan
 #pragma unroll
     for (int k = 0; k < kPerThread; ++k) {
       const int row = x.row0 + k * S::kRows + r_in;
-      const long long pos = static_cast<long long>(x.start) + row;
+      long long pos = static_cast<long long>(x.start) + row;
       live[k] = row < x.n && pos >= 0 && pos < p.cache_len;
-      if constexpr (SEEN) live[k] = live[k] && (row >= low || row < few);
+      if constexpr (SEEN) {
+        pos = row < seen.head ? row : row + seen.off;
+        live[k] = row < x.n && (row < seen.few || (row >= seen.head && pos >= seen.low));
+      }
       if (!live[k]) continue;
       const long long crow = x.bh * p.cache_len + pos;
 #pragma unroll
@@ -485,20 +495,20 @@ int launch_rows(const RowsParams& p, int dtype, int head_dim, int batch, RowsWor
 int launch_kv4_prompt_operands(const tb200_cache_attn_args& a, int window, int sinks, const Kv4PromptOperands& to, int num_sms, cudaStream_t stream) {
   RowsParams p;
   memset(&p, 0, sizeof(p));
-  p.n_rows = a.kv_lens; p.rows = a.cache_len; p.heads = a.n_kv_heads; p.cache_len = a.cache_len;
+  p.n_rows = a.kv_lens; p.rows = to.len; p.heads = a.n_kv_heads; p.cache_len = a.cache_len;
   p.n_bh = static_cast<long long>(a.batch) * a.n_kv_heads;
   p.x[0] = static_cast<uint8_t*>(to.k16);
   p.x[1] = static_cast<uint8_t*>(to.v16);
   for (int w = 0; w < 2; ++w) {
     p.stride[w][2] = a.head_dim;
-    p.stride[w][1] = static_cast<long long>(a.cache_len) * a.head_dim;
+    p.stride[w][1] = static_cast<long long>(to.len) * a.head_dim;
     p.stride[w][0] = p.stride[w][1] * a.n_kv_heads;
   }
   p.codes[0] = static_cast<uint8_t*>(const_cast<void*>(a.k_codes));
   p.codes[1] = static_cast<uint8_t*>(const_cast<void*>(a.v_codes));
   p.meta[0] = static_cast<uint8_t*>(const_cast<void*>(a.k_meta));
   p.meta[1] = static_cast<uint8_t*>(const_cast<void*>(a.v_meta));
-  p.q_rows = a.q_rows; p.q_rows_max = a.rows; p.window = window; p.sinks = sinks;
+  p.q_rows = a.q_rows; p.q_rows_max = a.rows; p.window = window; p.sinks = sinks; p.packed_head = to.packed_head;
   p.head_factor = reinterpret_cast<const float4*>(to.head_factor);
   if (a.dtype == TB200_BF16) {
     FactorParams f;
