@@ -383,7 +383,7 @@ typedef struct {
   int n_q_heads, n_kv_heads, head_dim; /* head_dim 64 or 128 */
   int cache_len;             /* positions per (sequence, head); 4-bit: a multiple of 4 */
   int window, sinks;
-  float sm_scale;            /* finite, at least 1e-30 */
+  float sm_scale;            /* 1e-30 to 1e38 */
   const void* q;             /* (B, Hq, rows, D) */
   void* o;                   /* (B, Hq, rows, D) */
   int64_t q_stride[3];       /* batch, head, row */

@@ -130,3 +130,15 @@ def test_kv4_attn_values_that_grow(s, dt):
     f[..., :64] *= grow[:, None]
     f[..., 64:] *= grow.flip(0)[:, None]
     assert run4(q, *held4(k, f.to(dt)), *shape[6:], 128 ** -0.5) <= 1
+
+
+@pytest.mark.parametrize("kv4", [True, False])
+@pytest.mark.parametrize("s", [1, 3, 10, 40])
+@pytest.mark.parametrize("scale", [1e-30, 1e-20, 1e20, 1e32, 1e37])
+def test_scales_of_any_size(scale, s, kv4):
+    """Queries as much smaller, or larger, as the scale is far from 1."""
+    shape = (1, 4, 1, 128, s, 512, [500], [s], 0, 0)
+    q, k, v = data(shape, torch.bfloat16)
+    q = (q.float() * (128 ** -0.5 / scale)).to(q.dtype)
+    off = run4(q, *held4(k, v), *shape[6:], scale) if kv4 else run16(q, k, v, *shape[6:], scale)
+    assert off <= 1

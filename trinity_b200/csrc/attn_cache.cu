@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
       for (int c = 0; c < 2; ++c) {   // what columns 2t and 2t + 1 need of their rows
         const int src = (2 * t + c) * 4;
         // never 0 nor infinite: a hidden score is -inf times this, one of a key of zeros 0
-        cf[nt][c] = fminf(fmaxf(__shfl_sync(0xffffffffu, down[nt], src) * (large ? p.scale_log2 : p.scale_log2 * 16777216.f), 1.17549435e-38f), 3.402823466e38f);
+        cf[nt][c] = fminf(fmaxf(__shfl_sync(0xffffffffu, down[nt], src) * p.scale_log2 * (large ? 1.f : 16777216.f), 1.17549435e-38f), 3.402823466e38f);
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[nt][gr], src) * (large ? 1.f : 5.9604644775390625e-8f);   // 2^-24
         const int mc = rt * R + (nt * 8 + 2 * t + c) % R;
@@ -597,7 +597,7 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   if (a->head_dim != 64 && a->head_dim != 128) return TB200_ERR_UNSUPPORTED;
   if (a->batch < 0 || a->rows < 0 || a->n_kv_heads < 1 || a->n_q_heads < 1 || a->n_q_heads % a->n_kv_heads || a->cache_len < 1) return TB200_ERR_INVALID;
   if (a->batch > kMaxExtent || a->cache_len > kMaxExtent || static_cast<int64_t>(a->n_q_heads) * a->rows > kMaxExtent) return TB200_ERR_INVALID;
-  if (a->window < 0 || a->sinks < 0 || !(a->sm_scale >= 1e-30f) || !(a->sm_scale < INFINITY)) return TB200_ERR_INVALID;
+  if (a->window < 0 || a->sinks < 0 || !(a->sm_scale >= 1e-30f) || !(a->sm_scale <= 1e38f)) return TB200_ERR_INVALID;
   if (a->batch == 0 || a->rows == 0) return TB200_OK;   // nothing to read or write: empty tensors have no address
   if (!a->q || !a->o || !a->kv_lens || a->q == a->o || !aligned16(a->q) || !aligned16(a->o) || !aligned4(a->kv_lens) || !aligned4(a->q_rows))
     return TB200_ERR_INVALID;
