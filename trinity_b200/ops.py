@@ -322,9 +322,14 @@ class Kv4Cache(NamedTuple):
 
 
 def kv4_cache(batch: int, kv_heads: int, cache_len: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device="cuda") -> Kv4Cache:
-    """An empty 4-bit cache of at least ``cache_len`` positions (rounded up to a multiple of 4)."""
-    if head_dim % 64:
-        raise ValueError(f"head_dim must be a multiple of 64, not {head_dim}")
+    """An empty 4-bit cache of at least ``cache_len`` positions (rounded up to a multiple of 4); ``head_dim`` 64 or 128,
+    ``dtype`` bfloat16 or float16."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, not {head_dim}")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"a 4-bit cache stands for bfloat16 or float16 rows, not {dtype}")
+    if cache_len < 0:
+        raise ValueError(f"cache_len must not be negative, not {cache_len}")
     length = (cache_len + 3) // 4 * 4
     codes = [torch.zeros(batch, kv_heads, length, head_dim // 2, dtype=torch.uint8, device=device) for _ in range(2)]
     meta = [torch.zeros(batch, kv_heads, length, head_dim // 64, 2, dtype=dtype, device=device) for _ in range(2)]
