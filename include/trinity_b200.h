@@ -328,11 +328,11 @@ int tb200_kv_compact(const tb200_kv_compact_args* args, void* stream);
  * cache_len is a multiple of 4; codes and meta are contiguous and 16-byte aligned.
  *
  * tb200_kv4_append quantises new rows into the cache, tb200_kv4_read turns cache rows back into
- * 16-bit rows (lo + c * s rounded once, at most the type's largest number).  Row i < n_rows[b] of sequence b is cache position
- * start[b] + i.  Rows i >= n_rows[b] and rows whose position lies outside [0, cache_len) are left as
+ * 16-bit rows (lo + c * s rounded once, at most the type's largest number).  Row i < n_rows[b] of
+ * sequence b is cache position start[b] + i.  Rows i >= n_rows[b] and rows whose position lies outside [0, cache_len) are left as
  * they are (append: the cache; read: k and v).  n_rows[b] outside [0, rows] is taken as the nearer end.
- * k and v are addressed by element strides of their batch, head and row axes (multiples of 8; head_dim
- * contiguous); the rows of a tensor that is written must not overlap one another, nor what else the call
+ * k and v are addressed by element strides of their batch, head and row axes (multiples of 8, at least
+ * head_dim; head_dim contiguous); the rows of a tensor that is written must not overlap one another, nor what else the call
  * reads or writes. */
 typedef struct {
   int dtype;                 /* TB200_F16 or TB200_BF16: k, v, meta */
@@ -375,7 +375,7 @@ int tb200_kv4_rows_check(const tb200_kv4_rows_args* args);
  * 64 channels (prompts, bf16: 2^-28, in the same kv head, and below 2^-110) is lost.
  *
  * tb200_attn_window: 16-bit caches, tb200_kv4_attn: 4-bit caches as above.  q, o and the 16-bit caches
- * are addressed by element strides (multiples of 8, head_dim contiguous); o overlaps no input.  Workspace: as the
+ * are addressed by element strides (multiples of 8, at least head_dim; head_dim contiguous); o overlaps no input.  Workspace: as the
  * *_workspace_bytes queries say for the same arguments (pointers and lengths are not looked at). */
 typedef struct {
   int dtype;                 /* TB200_F16 or TB200_BF16: q, o, 16-bit caches, meta */

@@ -25,8 +25,8 @@
 // from the window of the item's first query to its last query.  Tiles are cut from that line, so that neither a window that
 // begins inside a tile nor a handful of first positions costs a tile; the tile in which the two meet is fetched in boxes of
 // sixteen keys.  (4000 queries of 32/8 heads under a window of 1000, bf16, D = 128: 78 us, 58 GFLOP at 45 % of the tensor
-// peak; with tiles at multiples of 128 and a tile for the first positions 105 us.)  Rows of V that no query of the item sees are cleared in shared memory before they meet a probability of 0,
-// because a cache may hold anything there.
+// peak; with tiles at multiples of 128 and a tile for the first positions 105 us.)  Rows of V that no query of the item sees
+// are cleared in shared memory before they meet a probability of 0, because a cache may hold anything there.
 // A query tile packs `pack` query heads that share a kv head: row r is token r / pack of the tile's tokens, head r % pack of
 // the pack.  Few tokens then still fill a tile, and the tokens of a tile lie closer together, so that less of a window's or
 // the diagonal's tiles is masked; the host takes the pack with the fewest key tiles to walk.

@@ -68,7 +68,6 @@ template <int D, int NT, int H> struct DecSmem {
   static constexpr int kMeta = kTile * (D / 64) * 4;
   static constexpr int kStage = 2 * (kCodes + kMeta);      // K codes, V codes, K meta, V meta
   static constexpr int kRing = kStages * kStage;           // per warp
-  static constexpr int kMergePitch = D + 4;                // floats per row: 4 keep the rows' banks apart
   static constexpr int kBarOff = kWarps * kRing;
   // the merge buffers take the place of the rings, which are empty by then
   static_assert(MergeSmem<D, NT>::kBytes <= kBarOff, "the merge buffers must fit where the rings were");
@@ -200,9 +199,11 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
       for (int c = 0; c < 2; ++c) {   // what columns 2t and 2t + 1 need of their rows
         const int src = (2 * t + c) * 4;
         // never 0 nor infinite: a hidden score is -inf times this, one of a key of zeros 0
-        cf[nt][c] = fminf(fmaxf(__shfl_sync(0xffffffffu, down[nt], src) * p.scale_log2 * (large ? 1.f : 16777216.f), 1.17549435e-38f), 3.402823466e38f);
+        const float x = __shfl_sync(0xffffffffu, down[nt], src) * p.scale_log2 * (large ? 1.f : 16777216.f);
+        cf[nt][c] = fminf(fmaxf(x, 1.17549435e-38f), 3.402823466e38f);
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[nt][gr], src) * (large ? 1.f : 5.9604644775390625e-8f);   // 2^-24
+        for (int gr = 0; gr < NG; ++gr)
+          qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[nt][gr], src) * (large ? 1.f : 5.9604644775390625e-8f);   // 2^-24
         const int mc = rt * R + (nt * 8 + 2 * t + c) % R;
         cpos[nt][c] = mc < n_rows ? sq.n - sq.r + mc / p.group : -1;
       }
@@ -311,7 +312,8 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
               const int u = __float_as_int(mv[gr].x), w = __float_as_int(fabsf(mv[gr].y));
-              if (alive && u < 0x7f800000 && w < 0x7f800000) take(gr, u, w - (60 << 23));   // lo counts where it is 2^60 times the scale: the sums of p lo have to stay in fp32 too
+              // lo counts where it is 2^60 times the scale: the sums of p lo have to stay in fp32 too
+              if (alive && u < 0x7f800000 && w < 0x7f800000) take(gr, u, w - (60 << 23));
             }
           }
         };
@@ -397,7 +399,8 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
         for (int gr = 0; gr < NG; ++gr) {
           // a tile's products are summed from zero and then added in fp32: the tensor core's additions truncate, and over
           // thousands of keys with codes of one sign that would add up
-          float part[NT][4][4], part8[NT][4];
+          float part[NT][4][4];
+          [[maybe_unused]] float part8[NT][4];
 #pragma unroll
           for (int sp = 0; sp < kTile / 16; ++sp) {
             const int key0 = sp * 16 + (g >> 1) + (g & 1) * 4 + (H == 2 ? (t >> 1) * 8 : 0);
@@ -588,8 +591,6 @@ __global__ void __launch_bounds__(kCombineThreads) cache_combine_kernel(const __
   T* op = reinterpret_cast<T*>(p.o) + b * p.os[0] + (h * p.group + mr - tok * p.group) * p.os[1] + tok * p.os[2] + lane * 4;
   *reinterpret_cast<uint2*>(op) = make_uint2(Pack2<T>::pack(acc.x * inv, acc.y * inv), Pack2<T>::pack(acc.z * inv, acc.w * inv));
 }
-
-constexpr int kMaxExtent = 1 << 30;
 
 int check_attn(const tb200_cache_attn_args* a, bool kv4) {
   if (a == nullptr) return TB200_ERR_INVALID;

@@ -29,7 +29,8 @@ struct CacheAttnParams {
   int B, S, Hq, Hkv, group, cache_len, window, sinks;
   int row_tiles;             // units per (sequence, kv head) at most
   int cluster;               // 0: the line; else CTAs per unit
-  int record_per_unit;       // the line: what `split` is indexed by, the unit where there are no more units than stretches, else the stretch
+  int record_per_unit;       // the line: what `split` is indexed by, the unit where there are no more units than stretches,
+                             // else the stretch
   float scale_log2;
   const uint8_t* q;
   uint8_t* o;
@@ -39,8 +40,9 @@ struct CacheAttnParams {
   const uint8_t *k_codes, *v_codes, *k_meta, *v_meta;
   float* part_o;             // (2 grid, R, D)
   float* part_ml;            // (2 grid, R, 2)
-  int4* split;               // (grid) units that lie in several stretches and in how many (0: no such unit): by stretch (sequence, kv head,
-                             // row tile, how many), for the one that begins there and goes on; by unit (stretch it begins in, -, -, how many)
+  int4* split;               // (grid) units that lie in several stretches and in how many (0: no such unit): by stretch
+                             // (sequence, kv head, row tile, how many), for the one that begins there and goes on; by unit
+                             // (stretch it begins in, -, -, how many)
   int stretches;             // CTAs of the decode kernel
   int* err;
   long long wait_limit;

@@ -260,15 +260,15 @@ int launch_cast_f32(const float* src, void* dst, int64_t n, int dtype, cudaStrea
 int launch_kv_compact(const tb200_kv_compact_args& a, cudaStream_t stream);
 
 // ---------------------------------------------------------------- kv4.cu
+constexpr int kMaxExtent = 1 << 30;   // of an axis of a cache call
 // Element strides of the (batch, head, row) axes with extents ext: steps of 16 bytes, and with `written` rows that do
 // not overlap.  Axes of one element are not looked at.
 int check_strides(const int64_t (&stride)[3], const int64_t (&ext)[3], int head_dim, bool written);
 // A prompt's operands out of a 4-bit cache: the positions that some query row of its sequence sees as contiguous 16-bit
 // caches (B, Hkv, len, D), other places left as they are.  packed_head -1: at their own places.  Else, where the window begins
 // behind the first positions that stay visible, the first positions at their places below packed_head, the others from
-// there on; len holds packed_head + window + rows.  fp16: the values, rounded (by half a step of the type
-// the output is rounded to as well).  bf16: in fp16, divided by a
-// power of two per head (head_factor (B, Hkv, 4): 1 / factor and factor of K, of V), and q (B, Hq, rows, D) likewise by one
+// there on; len holds packed_head + window + rows.  fp16: the values, rounded (by half a step of the type the output is
+// rounded to as well).  bf16: in fp16, divided by a power of two per head (head_factor (B, Hkv, 4): 1 / factor and factor of K, of V), and q (B, Hq, rows, D) likewise by one
 // per row (q_factor); q16, q_factor and head_factor are not used for fp16.
 struct Kv4PromptOperands {
   int len = 0, packed_head = -1;

@@ -434,8 +434,6 @@ int check_strides(const int64_t (&st)[3], const int64_t (&ext)[3], int head_dim,
 
 namespace {
 
-constexpr int kMaxExtent = 1 << 30;
-
 int check_rows(const tb200_kv4_rows_args* a) {
   if (a == nullptr) return TB200_ERR_INVALID;
   if (a->dtype != TB200_BF16 && a->dtype != TB200_F16) return TB200_ERR_UNSUPPORTED;
@@ -474,7 +472,8 @@ template <typename T, int D>
 int launch_rows(RowsParams p, int batch, RowsWork work, int num_sms, cudaStream_t stream) {
   p.n_bh = static_cast<long long>(batch) * p.heads;
   p.units = p.n_bh * ((p.rows + RowsShape<D>::kUnitRows - 1) / RowsShape<D>::kUnitRows);
-  const long long most = static_cast<long long>(num_sms) * 32;   // several waves: the hardware deals CTAs out as SMs become free (8 per SM: 6 % slower)
+  // several waves: the hardware deals CTAs out as SMs become free (8 per SM: 6 % slower)
+  const long long most = static_cast<long long>(num_sms) * 32;
   const dim3 grid(static_cast<unsigned>(p.units < most ? p.units : most));
   cudaError_t e;
   if (work == kAppend) e = launch_chained(kv4_append_kernel<T, D>, grid, dim3(kThreads), 0, stream, p);

@@ -8,8 +8,8 @@ namespace tb200 {
 template <typename T> struct Kv4Decode;
 
 // A code in the low mantissa bits of a 16-bit float whose exponent makes one mantissa step a 1: 1024 + c in fp16,
-// 128 + c in bf16.  Subtracting the offset is exact, and lo + c s is one fused multiply-add: rounded once.  s is rounded, so lo + 15 s may pass the type's
-// largest number where max x is next to it: such a value is read as that number (a NaN stays one).
+// 128 + c in bf16.  Subtracting the offset is exact, and lo + c s is one fused multiply-add: rounded once.  s is rounded, so
+// lo + 15 s may pass the type's largest number where max x is next to it: such a value is read as that number (a NaN stays one).
 template <> struct Kv4Decode<__half> {
   static constexpr uint32_t kMagic = 0x64006400u;
   static __device__ __forceinline__ uint32_t pair(uint32_t two_codes, __half2 s, __half2 lo) {

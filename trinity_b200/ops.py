@@ -443,7 +443,7 @@ def _kv4_rows(name: str, cache: Kv4Cache, k, v, start, rows, index: int, count: 
 def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor], rows: Optional[torch.Tensor] = None) -> None:
     """Quantise new rows into a 4-bit cache: row ``i`` of ``k, v (B, Hkv, S, D)`` becomes position ``start[b] + i``.
 
-    ``k`` and ``v`` may have any strides (multiples of 8, last axis contiguous): what a projection leaves,
+    ``k`` and ``v`` may have any strides that are multiples of 8 and at least ``D`` (last axis contiguous): what a projection leaves,
     ``(x @ wk).view(B, S, Hkv, D).transpose(1, 2)``, needs no copy.  ``start``: an int for all sequences or int32 ``(B,)``;
     ``rows`` int32 ``(B,)``: how many of the ``S`` rows of each sequence are meant (default all).  Other rows, and rows
     whose position lies outside the cache, are not written."""
@@ -511,7 +511,8 @@ def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k
                 sm_scale: float = 1.0, q_rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``softmax(sm_scale * q K^T) V`` over 16-bit caches that already hold the new rows, with per-sequence lengths.
 
-    ``q (B, Hq, S, D)``, ``k_cache, v_cache (B, Hkv, L, D)``: any strides (multiples of 8, last axis contiguous).
+    ``q (B, Hq, S, D)``, ``k_cache, v_cache (B, Hkv, L, D)``: any strides that are multiples of 8 and at least ``D`` (last axis
+    contiguous).
     ``kv_lens`` int32 ``(B,)``: positions in the cache, the new ones included; ``q_rows`` int32 ``(B,)``: how many of the
     ``S`` query rows belong to the sequence (default all); they are the last positions.  A query sees the positions up to
     its own, with ``window > 0`` only the last ``window`` of these and the first ``sinks`` ones.  A row that sees nothing
