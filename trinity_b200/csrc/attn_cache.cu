@@ -10,15 +10,15 @@
 //            c * 2^-24, one nibble higher c * 2^-20, and the tensor core takes such (subnormal) numbers exactly.  One
 //            AND per two codes makes an operand.  With K = lo + c s per group of 64:  q.k = sum_g s_g (q.c)_g + lo_g sum(q)_g,
 //            so s and lo meet the scores in fp32 and no key is ever rounded.  With V:  o = sum_g [sum_j (p_j s_jg)(c_jd - 8) +
-//            sum_j p_j (lo_jg + 8 s_jg)]: the scale goes into the probability (rounded to fp16, after a power of two that
-//            keeps the largest p s below 2^14), the second sum is fp32, and for fp16 outputs the 8 is taken out with the SAME
+//            sum_j p_j (lo_jg + 8 s_jg)]: the scale goes into the probability (rounded to fp16, after a power of two per group
+//            that brings the largest p s near 2^14), the second sum is fp32, and for fp16 outputs the 8 is taken out with the SAME
 //            rounded probabilities (an MMA against a constant 8), so that the rounding error is that of centred codes, 2.6
 //            times smaller; bf16 outputs are rounded sixteen times more coarsely than that and do without.
 //            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
 //   H = 2    four query rows or fewer (one token of up to four query heads per kv head): they fill half of the eight columns,
 //            so columns 4 to 7 repeat them, and each column takes the probabilities of half the keys: a thread then has two
 //            scores of sixteen keys to work on instead of four, and a row comes in two shares like those of two warps.
-//   measured one token of 24 sequences of 1 to 16384 positions, 32/8 heads of 128, bf16: 52.7 us for 223 MB, 65 % of the copy
+//   measured one token of 24 sequences of 1 to 16384 positions, 32/8 heads of 128, bf16: 52.4 us for 223 MB, 65 % of the copy
 //            bandwidth; an instruction issues in half of the cycles, the tensor pipe is busy in a quarter of them: what is
 //            left is the latency of each warp's chain scores -> maximum -> exponentials -> products, with the 8 to 12 warps
 //            per SM that the registers allow.
@@ -622,7 +622,7 @@ int check_attn(const tb200_cache_attn_args* a, bool kv4) {
 // sequences of 2048 positions, 32/8 heads, decode and prompt kernel in us: 16 rows 34 / 37, 32 rows 37 / 37, 64 rows 62 / 37;
 // one head per kv head 16 rows 34 / 37; 71 heads on one, a single token, 4 x 16384 positions: 21 / 21.
 // 4 bits: the prompt kernel needs the visible rows in 16 bits first: 32 rows 40 / 65, 64 rows 68 / 66, 96 rows 97 / 66; 71
-// heads, a single token 23 / 25.  A single token never takes that copy (its workspace is that of all the cache).
+// heads, a single token 23 / 25.  A single token never takes that copy.
 bool takes_prompt_kernel(int64_t rows, int tokens, bool kv4) { return kv4 ? rows > 64 && tokens > 1 : rows > 16; }
 
 // Query rows of a unit: the smallest form that holds a sequence's rows of one kv head, else as many as there are.  Four rows:
@@ -677,7 +677,7 @@ AttnPlan plan_attn(const tb200_cache_attn_args* a, bool kv4, int num_sms) {
       // cache is held in 4 bits where 16 do not fit.  Up to kCopyMost where a piece would have fewer than two items per SM, with
       // the keys in 16 shares; one (sequence, kv head) is the least.  32/8 heads of 128, bf16, the whole cache copied against
       // this, MiB of scratch and us: 24 sequences of 16384 and 20 tokens 1540, 791 / 262, 790; 100 tokens 1556, 1115 / 272, 1251;
-      // 500 tokens 1632, 3170 / 272, 3465; 16 sequences of 131072 and 20 tokens 8195, 3700 / 1030, 4220; under a window of 1000
+      // 500 tokens 1632, 3170 / 272, 3490; 16 sequences of 131072 and 20 tokens 8195, 3700 / 1030, 4160; under a window of 1000
       // 8195, 411 / 67, 48.
       const int64_t head = (static_cast<int64_t>(sinks) + 15) & ~15;
       const int64_t packed = head + window + a->rows;
