@@ -370,9 +370,10 @@ int tb200_kv4_rows_check(const tb200_kv4_rows_args* args);
  * Cache rows that no query row of their sequence sees have no influence, whatever they hold; an
  * infinity or a NaN in a row that some query row sees, or a score past fp32's range, may also reach the
  * other new rows of that sequence in the same call.
- * On a 4-bit cache, probabilities (and prompts' keys and values) meet the products in fp16, scaled by powers
- * of two: what a value has below about 2^-26 of the largest one that the sequence's new rows see in the same
- * 64 channels (prompts, bf16: 2^-28, in the same kv head, and below 2^-110) is lost.
+ * fp16: a probability is held to 2^-25 of the row's largest.  On a 4-bit cache, probabilities (and the
+ * queries, and prompts' keys and values) meet the products in fp16, scaled by powers of two: what a value has
+ * below about 2^-26 of the largest one that the sequence's new rows see in the same 64 channels (prompts,
+ * bf16: 2^-28, in the same kv head, and below 2^-110), or a query below 2^-28 of its row's largest, is lost.
  *
  * tb200_attn_window: 16-bit caches, tb200_kv4_attn: 4-bit caches as above.  q, o and the 16-bit caches
  * are addressed by element strides (multiples of 8, at least head_dim; head_dim contiguous); o overlaps no input.  Workspace: as the

@@ -142,3 +142,21 @@ def test_scales_of_any_size(scale, s, kv4):
     q = (q.float() * (128 ** -0.5 / scale)).to(q.dtype)
     off = run4(q, *held4(k, v), *shape[6:], scale) if kv4 else run16(q, k, v, *shape[6:], scale)
     assert off <= 1
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("s", [1, 3, 10, 40])
+@pytest.mark.parametrize("e", [8, 12, 15, 20, 25])
+def test_queries_with_one_large_channel(e, s, dt):
+    """One channel of the queries 2^e times larger than the others, on keys that are zero there: the others keep their digits."""
+    shape = (1, 4, 1, 128, s, 512, [500], [s], 0, 0)
+    q, k, v = data(shape, dt)
+    if dt == torch.float16:
+        q = q * 2.0 ** -6      # (some of them below the type's smallest normal number)
+    q[..., 5] = min(2.0 ** e, 60000.0) if dt == torch.float16 else 2.0 ** e
+    k = k.abs()
+    k[..., 5] = 0
+    scale = 128 ** -0.5 * (64 if dt == torch.float16 else 1)
+    cache, k64, v64, w = held4(k, v)
+    assert (k64[..., 5] == 0).all()
+    assert run4(q, cache, k64, v64, w, *shape[6:], scale) <= 1

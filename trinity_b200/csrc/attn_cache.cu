@@ -14,7 +14,8 @@
 //            that brings the largest p s near 2^14), the second sum is fp32, and for fp16 outputs the 8 is taken out with the SAME
 //            rounded probabilities (an MMA against a constant 8), so that the rounding error is that of centred codes, 2.6
 //            times smaller; bf16 outputs are rounded sixteen times more coarsely than that and do without.
-//            q is brought to fp16 by a power of two per row: bf16 inputs lose nothing within 2^-14 of the row's largest.
+//            q is brought to fp16 by a power of two per row: inputs lose nothing within 2^-25 (bf16; fp16: 2^-22) of the row's
+//            largest.
 //   H = 2    four query rows or fewer (one token of up to four query heads per kv head): they fill half of the eight columns,
 //            so columns 4 to 7 repeat them, and each column takes the probabilities of half the keys: a thread then has two
 //            scores of sixteen keys to work on instead of four, and a row comes in two shares like those of two warps.
@@ -170,10 +171,10 @@ __global__ void __launch_bounds__(kThreads, DecShape<D, NT, H>::kCtas) cache_dec
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       unit_top = max(unit_top, __float_as_uint(top));
-      // a power of two that brings the row's largest magnitude to [8, 16)
-      const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 4);
-      up[nt] = __uint_as_float(static_cast<uint32_t>(257 - ex) << 23);        // 2^(130 - ex)
-      down[nt] = __uint_as_float(static_cast<uint32_t>(ex - 3) << 23);        // its inverse
+      // a power of two that brings the row's largest magnitude to [2^14, 2^15): small ones keep their digits beside a large one
+      const int ex = max(static_cast<int>(__float_as_uint(top) >> 23), 15);
+      up[nt] = __uint_as_float(static_cast<uint32_t>(268 - ex) << 23);        // 2^(141 - ex)
+      down[nt] = __uint_as_float(static_cast<uint32_t>(ex - 14) << 23);       // its inverse
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
         float x = 0.f;

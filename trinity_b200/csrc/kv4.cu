@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kFactorThreads) kv4_factors_kernel(const __gri
       }
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float2 pw = power_for(top, 3, 5);
+      const float2 pw = power_for(top, 14, 16);
       const long long out = static_cast<long long>(b) * rows + row;
       uint32_t* dst = reinterpret_cast<uint32_t*>(f.q16 + out * D * 2) + lane * (V / 2);
 #pragma unroll
